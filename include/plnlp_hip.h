@@ -629,6 +629,69 @@ int plnlp_dropout_f32(const float* x, float* y, int64_t n_rows, int64_t n_cols,
 int plnlp_transpose_f32(const float* x, int64_t ldx, float* y, int64_t ldy,
                         int64_t n_rows, int64_t n_cols, void* stream);
 
+/* ---- 16-bit storage: rows by id, a linear layer, gradient clipping (csrc/lookup.hip, linear_act.hip, grad_clip.hip) ------
+ * Additions within ABI 12 (nothing that was there changed).  Tensors may be f32, bf16 or f16 (PLNLP_DTYPE_*); every sum is
+ * held in f32 or f64 and every result is rounded once, to nearest even.  All entry points are deterministic, keep no state
+ * between calls and may be captured into a hipGraph (fill and copy nodes are never recorded). */
+#define PLNLP_DTYPE_F32  0
+#define PLNLP_DTYPE_BF16 1
+#define PLNLP_DTYPE_F16  2
+
+/* out[t, :] = scale * table[ids[t], :]; an id outside [0, n_rows) reads as a row of zeros.  ids: int32 (id_bytes 4) or int64 (8),
+ * [n_ids] consecutive; n_rows, n_ids <= 2^31 - 2.  table and out: rows ld / ldo elements apart, any of the three types, each
+ * aligned to its element.  (The reference indexes its table with h[edge], plnlp/model.py:155-156.) */
+int plnlp_embedding_lookup(const void* table, int64_t ld, int table_dtype, int64_t n_rows, int64_t width,
+                           const void* ids, int id_bytes, int64_t n_ids, float scale,
+                           void* out, int64_t ldo, int out_dtype, void* stream);
+/* grad[v, :] = scale * sum_{t: ids[t] = v} gy[t, :] for every row v in [0, n_rows) (all are written; columns past width are not);
+ * ids outside the table and ids equal to padding_id (-1: none) give nothing.  workspace: 16-byte aligned device memory of
+ * plnlp_embedding_grad_workspace_bytes(n_ids, width) bytes. */
+int64_t plnlp_embedding_grad_workspace_bytes(int64_t n_ids, int64_t width);
+int plnlp_embedding_grad(const void* gy, int64_t ldg, int gy_dtype, const void* ids, int id_bytes, int64_t n_ids,
+                         int64_t padding_id, float scale, void* grad, int64_t lde, int grad_dtype, int64_t n_rows,
+                         int64_t width, void* workspace, int64_t workspace_bytes, void* stream);
+
+#define PLNLP_ACT_NONE      0
+#define PLNLP_ACT_RELU      1
+#define PLNLP_ACT_GELU      2   /* z Phi(z)                                                  */
+#define PLNLP_ACT_GELU_TANH 3   /* z (1 + tanh(sqrt(2/pi) (z + 0.044715 z^3))) / 2           */
+#define PLNLP_ACT_SILU      4   /* z / (1 + exp(-z))                                         */
+/* out = act(x w^T + bias) + residual for x [m, k], w [n, k] (nn.Linear's layout), bias [n] (nullable), residual [m, n] (nullable),
+ * all of one 16-bit type (dtype BF16 or F16), rows ld* elements apart (at most 2^31), any alignment of whole elements; 16-byte
+ * aligned rows and k, n % 8 == 0 take the wide loads.  pre (nullable): z = x w^T + bias, what the backward pass reads.  out may
+ * be residual itself (same rows); otherwise outputs alias nothing.  workspace: plnlp_linear_act_workspace_bytes(m, n, k) bytes,
+ * 16-byte aligned (0: none needed). */
+int64_t plnlp_linear_act_workspace_bytes(int64_t m, int64_t n, int64_t k);
+int plnlp_linear_act(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, const void* residual, int64_t ldr,
+                     int act, int64_t m, int64_t n, int64_t k, void* pre, int64_t ldp, void* out, int64_t ldo, int dtype,
+                     void* workspace, int64_t workspace_bytes, void* stream);
+/* its gradients from gy = d out: dz = gy * act'(pre); dx = dz w, dw = dz^T x, db = column sums of dz (each nullable: not wanted);
+ * the residual's gradient is gy itself.  act NONE: pre is not read.  workspace as above, by its own byte count. */
+int64_t plnlp_linear_act_backward_workspace_bytes(int64_t m, int64_t n, int64_t k, int act);
+int plnlp_linear_act_backward(const void* gy, int64_t ldg, const void* pre, int64_t ldp, int act, const void* x, int64_t ldx,
+                              const void* w, int64_t ldw, int64_t m, int64_t n, int64_t k, void* dx, int64_t lddx,
+                              void* dw, int64_t lddw, void* db, int dtype, void* workspace, int64_t workspace_bytes,
+                              void* stream);
+
+#define PLNLP_NORM_L2  0
+#define PLNLP_NORM_L1  1
+#define PLNLP_NORM_MAX 2
+typedef struct plnlp_grad_tensor {
+    const void* src;          /* n consecutive elements                                            */
+    void*       dst;          /* where they go, scaled: src itself (one type then) or other memory   */
+    int64_t     n;
+    int32_t     src_dtype, dst_dtype;
+} plnlp_grad_tensor;
+/* *norm = the norm of all n_tensors (HOST array) tensors' elements taken as one vector; NaN and infinity go through.  workspace: device
+ * memory for plnlp_grad_norm_workspace_doubles(...) doubles (a function of the sizes alone). */
+int64_t plnlp_grad_norm_workspace_doubles(const plnlp_grad_tensor* tensors, int n_tensors);
+int plnlp_grad_norm(const plnlp_grad_tensor* tensors, int n_tensors, int norm_kind, double* workspace,
+                    int64_t workspace_doubles, float* norm, void* stream);
+/* ... and dst = src * min(1, max_norm / (*norm + 1e-6)), the clipping of clip_grad_norm_ (plnlp/model.py:163-165) with nothing read
+ * back by the host.  Written ranges must not overlap each other or another tensor's src. */
+int plnlp_grad_clip(const plnlp_grad_tensor* tensors, int n_tensors, int norm_kind, double max_norm, double* workspace,
+                    int64_t workspace_doubles, float* norm, void* stream);
+
 /* ---- diagnostics: which kernel families this process has launched -------------- */
 /* Process-wide counters (relaxed atomics; a count, not a synchronisation), one per kernel FAMILY an entry point can choose
  * between: the stationary-weights / tile split-bf16 GEMMs, the f32 tile GEMM, the aggregation's one-wave-per-row, slab,

@@ -29,9 +29,10 @@ GRAPH_REPLAY_SAFE = _os.environ.get(_PACKET_FLAG) == "0" and (_preset == "0" or 
 from .graph import Graph, gcn_normalization, adj_normalization  # noqa: F401,E402
 from . import ops  # noqa: F401
 from .ops import manual_seed  # noqa: F401
+from .mixed import clip_grads, embedding_lookup, grad_norm, linear_act  # noqa: F401
 from .layer import (BaseGNN, SAGE, GCN, WSAGE, Transformer, SAGEConv, GCNConv,  # noqa: F401
                     MLPPredictor, MLPCatPredictor, MLPDotPredictor, MLPBilPredictor,
-                    DotPredictor, BilinearPredictor)
+                    DotPredictor, BilinearPredictor, ScaledEmbedding, LinearAct)
 from .model import (BaseModel, create_input_layer, create_gnn_layer,  # noqa: F401
                     create_predictor_layer, adjust_lr)
 from . import loss, negative_sample, utils  # noqa: F401

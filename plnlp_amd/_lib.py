@@ -55,9 +55,19 @@ class AdamTensor(C.Structure):
                 ("step_scalars", C.c_void_p)]
 
 
+class GradTensor(C.Structure):
+    """mirror of plnlp_grad_tensor"""
+    _fields_ = [("src", C.c_void_p), ("dst", C.c_void_p), ("n", C.c_int64), ("src_dtype", C.c_int32),
+                ("dst_dtype", C.c_int32)]
+
+
 MULTI_MAX = 16
 GEMM_MATH_F32, GEMM_MATH_BF16X3 = 0, 1
 GEMM_FLAG_WIDE_WGRAD = 1          # plnlp_gemm_operand.flags
+DTYPE_F32, DTYPE_BF16, DTYPE_F16 = 0, 1, 2
+DTYPE_CODES = {torch.float32: DTYPE_F32, torch.bfloat16: DTYPE_BF16, torch.float16: DTYPE_F16}
+ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
+NORM_L2, NORM_L1, NORM_MAX = 0, 1, 2
 EPI_BIAS, EPI_RELU, EPI_DROPOUT, EPI_ACCUM, EPI_GATE, EPI_ADDEND, EPI_ADAM, EPI_ROWDOT = 1, 2, 4, 8, 16, 32, 64, 128
 REDUCE_SUM, REDUCE_MEAN = 0, 1
 AGG_LDS_STAGE = 2
@@ -170,6 +180,22 @@ SIGNATURES = {
     "plnlp_gate_f32": (C.c_int, [C.c_void_p, C.c_void_p, C.c_float, C.c_void_p, c_i64, C.c_void_p]),
     "plnlp_dropout_f32": (C.c_int, [C.c_void_p, C.c_void_p, c_i64, c_i64, C.c_float, C.c_uint64, C.c_void_p]),
     "plnlp_transpose_f32": (C.c_int, [C.c_void_p, c_i64, C.c_void_p, c_i64, c_i64, c_i64, C.c_void_p]),
+    "plnlp_embedding_lookup": (C.c_int, [C.c_void_p, c_i64, C.c_int, c_i64, c_i64, C.c_void_p, C.c_int, c_i64, C.c_float,
+                                         C.c_void_p, c_i64, C.c_int, C.c_void_p]),
+    "plnlp_embedding_grad_workspace_bytes": (c_i64, [c_i64, c_i64]),
+    "plnlp_embedding_grad": (C.c_int, [C.c_void_p, c_i64, C.c_int, C.c_void_p, C.c_int, c_i64, c_i64, C.c_float, C.c_void_p,
+                                       c_i64, C.c_int, c_i64, c_i64, C.c_void_p, c_i64, C.c_void_p]),
+    "plnlp_linear_act_workspace_bytes": (c_i64, [c_i64, c_i64, c_i64]),
+    "plnlp_linear_act": (C.c_int, [C.c_void_p, c_i64, C.c_void_p, c_i64, C.c_void_p, C.c_void_p, c_i64, C.c_int, c_i64, c_i64,
+                                   c_i64, C.c_void_p, c_i64, C.c_void_p, c_i64, C.c_int, C.c_void_p, c_i64, C.c_void_p]),
+    "plnlp_linear_act_backward_workspace_bytes": (c_i64, [c_i64, c_i64, c_i64, C.c_int]),
+    "plnlp_linear_act_backward": (C.c_int, [C.c_void_p, c_i64, C.c_void_p, c_i64, C.c_int, C.c_void_p, c_i64, C.c_void_p, c_i64,
+                                            c_i64, c_i64, c_i64, C.c_void_p, c_i64, C.c_void_p, c_i64, C.c_void_p, C.c_int,
+                                            C.c_void_p, c_i64, C.c_void_p]),
+    "plnlp_grad_norm_workspace_doubles": (c_i64, [C.POINTER(GradTensor), C.c_int]),
+    "plnlp_grad_norm": (C.c_int, [C.POINTER(GradTensor), C.c_int, C.c_int, C.c_void_p, c_i64, C.c_void_p, C.c_void_p]),
+    "plnlp_grad_clip": (C.c_int, [C.POINTER(GradTensor), C.c_int, C.c_int, C.c_double, C.c_void_p, c_i64, C.c_void_p,
+                                  C.c_void_p]),
 }
 
 _lib: Optional[C.CDLL] = None

@@ -40,6 +40,10 @@ def build(force: bool = False, verbose: bool = False) -> str:
     units.append(("gemm_wgw.hip", "gemm_wgw.o", ["-fno-slp-vectorize"]))
     units.append(("gemm_x3b.hip", "gemm_x3b.o", ["-fno-slp-vectorize"]))
     units.append(("aggregate_dense.hip", "aggregate_dense.o", ["-fno-slp-vectorize"]))
+    # (-packed-fp32-ops: the two-lane f32 instructions are not to be formed from these kernels' f32 arithmetic; the host pass
+    # warns that it does not know the feature)
+    no_packed = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+    units += [(src, src.replace(".hip", ".o"), no_packed) for src in ("lookup.hip", "linear_act.hip", "grad_clip.hip")]
     headers = [os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith(".h")]
     headers.append(os.path.join(os.path.dirname(HERE), "include", "plnlp_hip.h"))
     newest_header = max(os.path.getmtime(h) for h in headers)

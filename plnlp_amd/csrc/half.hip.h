@@ -1,0 +1,38 @@
+// 16-bit storage helpers shared by the lookup, linear_act and grad_clip kernels (gfx950, wave64).
+// Every computation is in f32 (or f64): a value is widened when it is read and rounded ONCE, to nearest even, when it is stored.
+#pragma once
+#include "common.hip.h"
+
+namespace plnlp {
+
+typedef __bf16   bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef float    f32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+inline bool is_dtype(int d) { return d == PLNLP_DTYPE_F32 || d == PLNLP_DTYPE_BF16 || d == PLNLP_DTYPE_F16; }
+inline int dtype_size(int d) { return d == PLNLP_DTYPE_F32 ? 4 : 2; }
+
+// V consecutive elements as one access (V * sizeof(T) bytes, at most 16 per load instruction; aligned to that)
+template <typename T, int V> struct alignas(V * sizeof(T) > 16 ? 16 : V * sizeof(T)) Pack { T v[V]; };
+
+template <typename T, int V> __device__ __forceinline__ void load_f32(const T* p, float (&x)[V]) {
+    const Pack<T, V> k = *reinterpret_cast<const Pack<T, V>*>(p);
+#pragma unroll
+    for (int i = 0; i < V; ++i) x[i] = (float)k.v[i];
+}
+template <typename T, int V> __device__ __forceinline__ void store_f32(T* p, const float (&x)[V]) {
+    Pack<T, V> k;
+#pragma unroll
+    for (int i = 0; i < V; ++i) k.v[i] = (T)x[i];
+    *reinterpret_cast<Pack<T, V>*>(p) = k;
+}
+
+// one call of f with the C++ types of a run-time dtype
+template <typename F> inline int with_dtype(int d, F&& f) {
+    if (d == PLNLP_DTYPE_F32) return f(float{});
+    if (d == PLNLP_DTYPE_BF16) return f(__bf16{});
+    return f(_Float16{});
+}
+
+}  // namespace plnlp

@@ -1,0 +1,661 @@
+// y = act(x W^T + bias) + residual for 16-bit x, W, bias, residual (bf16 or fp16), and its gradients:
+//   z = x W^T + bias;  y = act(z) + residual;   dz = dy * act'(z);  dx = dz W;  dW = dz^T x;  db = sum_rows dz;  d residual = dy
+// Products on the matrix cores with f32 accumulation; bias, activation and residual on the f32 accumulators, ONE rounding to the
+// stored type.  What is rounded besides: z, kept in 16 bits for the backward pass (its derivative is taken at the rounded z:
+// a relative 2^-9 / 2^-12 of z, below what rounding dz costs anyway), and dz, which the two gradient products read as 16-bit operands.
+//
+// One tile kernel serves the three products, written as C[m, n] = sum_k P(m, k) Q(n, k):
+//   forward  P = x   (k contiguous)            Q = W (k contiguous)
+//   dx       P = dz  (k contiguous)            Q = W read with k along its ROWS
+//   dW       P = dz, Q = x, both with k along their rows
+// A tile of P and of Q is staged global -> registers -> LDS as rows of 64 consecutive k (128 bytes); an operand with k along its
+// rows is transposed on the way, in registers (8 k x 4 columns a thread, sixteen v_perm_b32), so the product itself reads one
+// layout.  The 16-byte units of a row are XOR-swizzled (swz) so that the stores of both kinds and the reads hit all LDS banks.
+// Q is the MFMA's first operand and its rows are dealt so that a lane ends up with 16 CONSECUTIVE columns of one row of C: bias,
+// residual and result move as 16-byte accesses straight from the accumulators, with no pass through LDS.
+#include "half.hip.h"
+
+namespace plnlp {
+
+constexpr int BK = 64;
+
+template <typename T> struct Mfma;
+template <> struct Mfma<__bf16> {
+    typedef bf16x8 frag;
+    static __device__ __forceinline__ f32x4 go(frag a, frag b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+};
+template <> struct Mfma<_Float16> {
+    typedef f16x8 frag;
+    static __device__ __forceinline__ f32x4 go(frag a, frag b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+};
+
+// ---- activations ------------------------------------------------------------------------------------------
+__device__ __forceinline__ float sigmoid_f(float z) { return __builtin_amdgcn_rcpf(1.f + __expf(-z)); }
+
+// the normal distribution function: Phi(-|z|) = exp(-z^2/2) * P(t) / 2 with t = 1 / (1 + 0.39 |z| / sqrt 2) and P a polynomial fitted
+// to exp(u^2) erfc(u) on [0, 30] in RELATIVE error (2.4e-6; 4e-6 evaluated in f32), so the far negative tail keeps its digits
+__device__ __forceinline__ float gauss_half(float z) {          // exp(-z^2/2)
+    return __expf(-0.5f * z * z);
+}
+__device__ __forceinline__ float normal_cdf(float z, float g) {
+    const float t = __builtin_amdgcn_rcpf(fmaf(0.39f * 0.70710678f, fabsf(z), 1.f));
+    float p = -0.10887830704450607f;
+    p = fmaf(p, t, 0.25157830119132996f);
+    p = fmaf(p, t, 0.0152523098513484f);
+    p = fmaf(p, t, 0.20380336046218872f);
+    p = fmaf(p, t, 0.19776275753974915f);
+    p = fmaf(p, t, 0.2204565703868866f);
+    p = fmaf(p, t, 0.22002261877059937f);
+    const float q = 0.5f * p * t * g;
+    return z > 0.f ? 1.f - q : q;
+}
+constexpr float TANH_C = 1.5957691216057308f;                   // 2 sqrt(2 / pi)
+constexpr float TANH_A = 0.044715f;
+
+template <int ACT> __device__ __forceinline__ float act_of(float z) {
+    if (ACT == PLNLP_ACT_RELU) return z < 0.f ? 0.f : z;         // (a NaN stays)
+    if (ACT == PLNLP_ACT_SILU) return z * sigmoid_f(z);
+    if (ACT == PLNLP_ACT_GELU) return z * normal_cdf(z, gauss_half(z));
+    if (ACT == PLNLP_ACT_GELU_TANH) return z * sigmoid_f(TANH_C * fmaf(TANH_A * z * z, z, z));
+    return z;
+}
+template <int ACT> __device__ __forceinline__ float act_slope(float z) {
+    if (ACT == PLNLP_ACT_RELU) return z > 0.f ? 1.f : (z == z ? 0.f : z);
+    if (ACT == PLNLP_ACT_SILU) { const float s = sigmoid_f(z); return s * fmaf(z, 1.f - s, 1.f); }
+    if (ACT == PLNLP_ACT_GELU) { const float g = gauss_half(z); return fmaf(z * 0.3989422804014327f, g, normal_cdf(z, g)); }
+    if (ACT == PLNLP_ACT_GELU_TANH) {
+        const float s = sigmoid_f(TANH_C * fmaf(TANH_A * z * z, z, z));
+        return fmaf(z * s * (1.f - s), TANH_C * fmaf(3.f * TANH_A * z, z, 1.f), s);
+    }
+    return 1.f;
+}
+// f(std::integral_constant<int, ACT>{}) of a run-time activation
+template <typename F> __host__ __device__ __forceinline__ int with_act(int act, F&& f) {
+    switch (act) {
+        case PLNLP_ACT_RELU: return f(std::integral_constant<int, PLNLP_ACT_RELU>{});
+        case PLNLP_ACT_SILU: return f(std::integral_constant<int, PLNLP_ACT_SILU>{});
+        case PLNLP_ACT_GELU: return f(std::integral_constant<int, PLNLP_ACT_GELU>{});
+        case PLNLP_ACT_GELU_TANH: return f(std::integral_constant<int, PLNLP_ACT_GELU_TANH>{});
+        default: return f(std::integral_constant<int, PLNLP_ACT_NONE>{});
+    }
+}
+
+// ---- what happens to a finished sum ---------------------------------------------------------------------------
+template <typename T> struct Finish {
+    const T* bias;          // nullable [n]
+    const T* res;           // nullable [m, ldr]
+    T*       pre;           // nullable [m, ldp]: z, for the backward pass
+    T*       out;           // [m, ldo]
+    int64_t  ldr, ldp, ldo;
+    int      vec;           // 8-column groups may move as 16 bytes
+};
+constexpr int PARTIAL = -1; // in the place of an activation: the sum is one K slice's, stored as it is
+
+// V consecutive columns of row m from column n on (all inside the matrix); b = the bias there
+template <int ACT, typename T, int V> __device__ __forceinline__ void finish_cols(const Finish<T>& f, float (&v)[V], const float (&b)[V], int64_t m, int64_t n) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) v[j] += b[j];
+    if (f.pre) store_f32<T, V>(f.pre + m * f.ldp + n, v);
+#pragma unroll
+    for (int j = 0; j < V; ++j) v[j] = act_of<ACT>(v[j]);
+    if (f.res) {
+        float r[V];
+        load_f32<T, V>(f.res + m * f.ldr + n, r);
+#pragma unroll
+        for (int j = 0; j < V; ++j) v[j] += r[j];
+    }
+    store_f32<T, V>(f.out + m * f.ldo + n, v);
+}
+
+// ---- the tile kernel --------------------------------------------------------------------------------------------
+template <typename T> struct TileArgs {
+    const T* p; const T* q;
+    int64_t  ldp, ldq;
+    int64_t  m, n, k;
+    int      tiles_m, tiles_n, slices, steps;     // steps: BK-steps per K slice
+    float*   partial;                              // slices > 1: [slices, m, n]
+    Finish<T> fin;
+};
+
+// which 16-byte unit of LDS row r holds unit 0 (unit u sits at u ^ swz): eight lanes that read rows 0..7, or the permuted Q rows
+// {0..3, 16..19}, or that store a transposed block's rows 4 apart, touch eight different units
+__device__ __forceinline__ int swz(int r) { return (r & 7) ^ ((r >> 3) & 1) ^ (((r >> 4) & 1) * 6); }
+
+// registers of one operand's tile (R rows x BK), one thread's share
+template <int R, int THREADS> struct Stage { u32x4 r[R * 8 / THREADS]; };
+
+template <typename T, bool VEC> __device__ __forceinline__ u32x4 load_unit(const T* p, int valid) {     // 8 elements, `valid` of them real
+    if (VEC) return *reinterpret_cast<const u32x4*>(p);
+    union { T t[8]; u32x4 u; } x;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x.t[j] = j < valid ? p[j] : (T)0.f;
+    return x.u;
+}
+
+// rows r0 .. r0 + R of an operand with k contiguous (`base` = its element (r0, k0)); rows past `rows` repeat the last (their results are
+// not stored), k past `left` reads as zero
+template <typename T, int R, int THREADS, bool VEC>
+__device__ __forceinline__ void fetch_rows(Stage<R, THREADS>& s, const T* base, int64_t ld, int rows, int64_t left) {
+#pragma unroll
+    for (int i = 0; i < R * 8 / THREADS; ++i) {
+        const int unit = threadIdx.x + i * THREADS, row = min(unit >> 3, rows - 1), k = (unit & 7) * 8;
+        const T* p = base + (int64_t)row * ld;
+        if (left >= BK) s.r[i] = load_unit<T, VEC>(p + k, 8);
+        else {
+            const int valid = (int)min(left - k, (int64_t)8);
+            s.r[i] = valid > 0 ? load_unit<T, VEC>(p + k, valid) : u32x4{0, 0, 0, 0};
+        }
+    }
+}
+template <int R, int THREADS> __device__ __forceinline__ void store_rows(const Stage<R, THREADS>& s, char* lds) {
+#pragma unroll
+    for (int i = 0; i < R * 8 / THREADS; ++i) {
+        const int unit = threadIdx.x + i * THREADS, row = unit >> 3, u = unit & 7;
+        *reinterpret_cast<u32x4*>(lds + row * 128 + ((u ^ swz(row)) << 4)) = s.r[i];
+    }
+}
+
+// the same tile of an operand with k along its rows (`base` = its element (k0, r0), ld between k's): 8 k x 4 columns a thread
+template <typename T, int R, int THREADS, bool VEC>
+__device__ __forceinline__ void fetch_cols(Stage<R, THREADS>& s, const T* base, int64_t ld, int cols, int64_t left) {
+    static_assert(R * 2 == THREADS, "one 8 x 4 block a thread");
+    const int c = (threadIdx.x % (R / 4)) * 4, g = threadIdx.x / (R / 4);
+    uint64_t* d = reinterpret_cast<uint64_t*>(s.r);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const int k = g * 8 + i;
+        if (VEC) {
+            const T* p = base + min(c, cols - 4);          // (columns are whole groups of four here)
+            d[i] = k < left ? *reinterpret_cast<const uint64_t*>(p + (int64_t)k * ld) : 0;
+        } else {
+            union { T t[4]; uint64_t u; } x;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x.t[j] = (k < left && c + j < cols) ? base[(int64_t)k * ld + c + j] : (T)0.f;
+            d[i] = x.u;
+        }
+    }
+}
+template <int R, int THREADS> __device__ __forceinline__ void store_cols(const Stage<R, THREADS>& s, char* lds) {
+    const int c = (threadIdx.x % (R / 4)) * 4, g = threadIdx.x / (R / 4);
+    const uint32_t* d = reinterpret_cast<const uint32_t*>(s.r);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        u32x4 o;
+#pragma unroll
+        for (int h = 0; h < 4; ++h) {
+            const uint32_t a = d[(2 * h) * 2 + (j >> 1)], b = d[(2 * h + 1) * 2 + (j >> 1)];
+            o[h] = __builtin_amdgcn_perm(b, a, (j & 1) ? 0x07060302u : 0x05040100u);
+        }
+        const int row = c + j;
+        *reinterpret_cast<u32x4*>(lds + row * 128 + ((g ^ swz(row)) << 4)) = o;
+    }
+}
+
+template <typename T, int BM, int BN, int WM, int WN, bool PT, bool QT, bool VEC, int ACT>
+__global__ __launch_bounds__(WM * WN * 64) void tile_kernel(TileArgs<T> a) {
+    constexpr int THREADS = WM * WN * 64, TM = BM / WM / 16;         // 16-row pieces of a wave's part; it is 64 columns wide
+    static_assert(BN / WN == 64, "a wave covers 64 columns");
+    typedef typename Mfma<T>::frag frag;
+    extern __shared__ __attribute__((aligned(16))) char lds[];       // two buffers of P rows, then Q rows
+    constexpr int BUF = (BM + BN) * 128;
+
+    // Workgroups are dealt to the eight XCDs in turn: each XCD gets a contiguous run of tiles, so that its L2 holds the panels they share
+    const int tiles = a.tiles_m * a.tiles_n, total = tiles * a.slices;
+    const int per = total >> 3, extra = total & 7, xcd = blockIdx.x & 7, nth = blockIdx.x >> 3;
+    const int id = xcd * per + min(xcd, extra) + nth;
+    const int slice = id / tiles, tile = id % tiles;
+    // and walks groups of 8 row panels column by column
+    constexpr int GROUP = 8;
+    const int group = tile / (GROUP * a.tiles_n), in_group = tile % (GROUP * a.tiles_n);
+    const int g_rows = min(GROUP, a.tiles_m - group * GROUP);
+    const int64_t m0 = (int64_t)(group * GROUP + in_group % g_rows) * BM, n0 = (int64_t)(in_group / g_rows) * BN;
+
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
+    const int wm = (wave / WN) * (BM / WM), wn = (wave % WN) * 64;
+    const int64_t k_lo = (int64_t)slice * a.steps * BK, k_hi = min(a.k, k_lo + (int64_t)a.steps * BK);
+    const int steps = k_hi > k_lo ? (int)((k_hi - k_lo + BK - 1) / BK) : 0;
+    const int rows_p = (int)min((int64_t)BM, a.m - m0), rows_q = (int)min((int64_t)BN, a.n - n0);
+
+    f32x4 acc[TM][4];
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int t = 0; t < 4; ++t) acc[i][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+    Stage<BM, THREADS> sp;
+    Stage<BN, THREADS> sq;
+    auto fetch = [&](int step) {
+        const int64_t k = k_lo + (int64_t)step * BK, left = k_hi - k;
+        if (PT) fetch_cols<T, BM, THREADS, VEC>(sp, a.p + k * a.ldp + m0, a.ldp, rows_p, left);
+        else fetch_rows<T, BM, THREADS, VEC>(sp, a.p + m0 * a.ldp + k, a.ldp, rows_p, left);
+        if (QT) fetch_cols<T, BN, THREADS, VEC>(sq, a.q + k * a.ldq + n0, a.ldq, rows_q, left);
+        else fetch_rows<T, BN, THREADS, VEC>(sq, a.q + n0 * a.ldq + k, a.ldq, rows_q, left);
+    };
+    auto stage = [&](int buf) {
+        char* b = lds + buf * BUF;
+        if (PT) store_cols<BM, THREADS>(sp, b); else store_rows<BM, THREADS>(sp, b);
+        if (QT) store_cols<BN, THREADS>(sq, b + BM * 128); else store_rows<BN, THREADS>(sq, b + BM * 128);
+    };
+    if (steps > 0) {
+        fetch(0);
+        stage(0);
+        if (steps > 1) fetch(1);
+        __syncthreads();
+    }
+    for (int step = 0; step < steps; ++step) {
+        const char* b = lds + (step & 1) * BUF;
+        if (step + 1 < steps) stage((step + 1) & 1);      // the other buffer was read before the barrier that ended the last step
+        if (step + 2 < steps) fetch(step + 2);            // a whole step to arrive in
+#pragma unroll
+        for (int ks = 0; ks < BK / 32; ++ks) {
+            frag q[4];
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+                const int row = wn + 16 * (r >> 2) + 4 * t + (r & 3);
+                q[t] = *reinterpret_cast<const frag*>(b + (BM + row) * 128 + (((ks * 4 + g) ^ swz(row)) << 4));
+            }
+#pragma unroll
+            for (int i = 0; i < TM; ++i) {
+                const int row = wm + i * 16 + r;
+                const frag p = *reinterpret_cast<const frag*>(b + row * 128 + (((ks * 4 + g) ^ swz(row)) << 4));
+#pragma unroll
+                for (int t = 0; t < 4; ++t) acc[i][t] = Mfma<T>::go(q[t], p, acc[i][t]);
+            }
+        }
+        __syncthreads();
+    }
+
+    // lane (r, g) holds columns n .. n + 15 of rows wm + 16 i + r
+    const int64_t n = n0 + wn + 16 * g;
+    if (n >= a.n) return;
+    const int cols = (int)min((int64_t)16, a.n - n);
+    float bias[16];
+#pragma unroll
+    for (int j = 0; j < 16; ++j) bias[j] = (ACT != PARTIAL && a.fin.bias && j < cols) ? (float)a.fin.bias[n + j] : 0.f;
+#pragma unroll
+    for (int i = 0; i < TM; ++i) {
+        const int64_t m = m0 + wm + i * 16 + r;
+        if (m >= a.m) continue;
+        if constexpr (ACT == PARTIAL) {
+            float* o = a.partial + ((int64_t)slice * a.m + m) * a.n + n;
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+                if (VEC) {
+                    if (4 * t < cols) *reinterpret_cast<f32x4*>(o + 4 * t) = acc[i][t];
+                } else
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) if (4 * t + j < cols) o[4 * t + j] = acc[i][t][j];
+            }
+        } else if constexpr (VEC) {                       // (n and the strides are whole groups of eight)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                if (8 * h >= cols) continue;
+                float v[8], b[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) { v[j] = acc[i][2 * h + (j >> 2)][j & 3]; b[j] = bias[8 * h + j]; }
+                finish_cols<ACT, T, 8>(a.fin, v, b, m, n + 8 * h);
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+                if (j < cols) {
+                    float v[1] = {acc[i][j >> 2][j & 3]}, b[1] = {bias[j]};
+                    finish_cols<ACT, T, 1>(a.fin, v, b, m, n + j);
+                }
+        }
+    }
+}
+
+// sum of the K slices in slice order, then the finish
+template <typename T, int V, int ACT>
+__global__ __launch_bounds__(256) void slices_kernel(const float* __restrict__ partial, int slices, int64_t m, int64_t n, Finish<T> fin) {
+    const int64_t groups = n / V, total = m * groups;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+        const int64_t row = i / groups, col = (i - row * groups) * V;
+        float v[V] = {}, b[V] = {};
+        for (int s = 0; s < slices; ++s) {
+            const float* p = partial + ((int64_t)s * m + row) * n + col;
+#pragma unroll
+            for (int j = 0; j < V; ++j) v[j] += p[j];
+        }
+        if (fin.bias)
+#pragma unroll
+            for (int j = 0; j < V; ++j) b[j] = (float)fin.bias[col + j];
+        finish_cols<ACT, T, V>(fin, v, b, row, col);
+    }
+}
+
+// ---- few rows: the weights stream from memory once, straight into the MFMA's registers ---------------------------
+// A workgroup owns 16 columns of y and all (<= 16 * TM) rows; its waves share K, 64 at a time.  A lane reads 32 consecutive bytes of
+// a weight row (the four lanes of a row 128): which k a lane holds is free as long as x is read the same way.  The waves'
+// sums meet in LDS and are added in wave order.
+template <typename T, int TM, int WAVES, int ACT>
+__global__ __launch_bounds__(WAVES * 64) void few_rows_kernel(const T* __restrict__ x, int64_t ldx, const T* __restrict__ w, int64_t ldw, int m,
+                                                              int64_t n, int64_t k, Finish<T> fin) {
+    typedef typename Mfma<T>::frag frag;
+    constexpr int AHEAD = TM == 1 ? 4 : 2;                 // 64-k units in flight a wave
+    __shared__ float part[WAVES][TM][16][17];
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
+    const int64_t n0 = (int64_t)blockIdx.x * 16;
+    const T* wr = w + min(n0 + r, n - 1) * ldw + g * 16;
+    const T* xr[TM];
+#pragma unroll
+    for (int i = 0; i < TM; ++i) xr[i] = x + (int64_t)min(i * 16 + r, m - 1) * ldx + g * 16;
+    f32x4 acc[TM];
+#pragma unroll
+    for (int i = 0; i < TM; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const int64_t units = (k + 63) / 64;
+    for (int64_t u0 = wave; u0 < units; u0 += WAVES * AHEAD) {
+        frag a[AHEAD][2], b[AHEAD][TM][2];
+#pragma unroll
+        for (int j = 0; j < AHEAD; ++j) {
+            const int64_t at = (u0 + j * WAVES) * 64;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const bool in = at + g * 16 + h * 8 < k;   // (k is whole groups of eight)
+                const frag zero = {};
+                a[j][h] = in ? *reinterpret_cast<const frag*>(wr + at + h * 8) : zero;
+#pragma unroll
+                for (int i = 0; i < TM; ++i) b[j][i][h] = in ? *reinterpret_cast<const frag*>(xr[i] + at + h * 8) : zero;
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < AHEAD; ++j)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int i = 0; i < TM; ++i) acc[i] = Mfma<T>::go(a[j][h], b[j][i][h], acc[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) part[wave][i][r][4 * g + j] = acc[i][j];      // [row of x][column]
+    __syncthreads();
+    for (int e = threadIdx.x; e < TM * 256; e += WAVES * 64) {
+        const int i = e >> 8, row = (e >> 4) & 15, c = e & 15;
+        const int64_t mm = i * 16 + row, nn = n0 + c;
+        float v[1] = {0.f}, b[1] = {0.f};
+#pragma unroll
+        for (int s = 0; s < WAVES; ++s) v[0] += part[s][i][row][c];
+        if (mm >= m || nn >= n) continue;
+        if (fin.bias) b[0] = (float)fin.bias[nn];
+        finish_cols<ACT, T, 1>(fin, v, b, mm, nn);
+    }
+}
+
+// ---- dz = dy * act'(z), and the column sums of dz ---------------------------------------------------------------------
+// 256 / tx rows of tx lanes, V columns a lane; a workgroup takes `rows` consecutive rows and leaves their column sums in partial[block, :]
+template <typename T, int V, int ACT>
+__global__ __launch_bounds__(256) void act_back_kernel(const T* __restrict__ gy, int64_t ldg, const T* __restrict__ pre, int64_t ldp,
+                                                       T* __restrict__ dz, int64_t ldz, int64_t m, int packs, int tx, int64_t rows,
+                                                       float* __restrict__ partial) {
+    __shared__ float lds[256 * V];
+    const int x = threadIdx.x & (tx - 1), y = threadIdx.x / tx, ty = 256 / tx;
+    const int64_t lo = (int64_t)blockIdx.x * rows, hi = min(lo + rows, m);
+    for (int c0 = 0; c0 < packs; c0 += tx) {
+        const int c = c0 + x;
+        float s[V] = {};
+        if (c < packs) {
+            const int64_t col = (int64_t)c * V;
+            int64_t i = lo + y;
+            auto go = [&](auto count) {
+                constexpr int U = decltype(count)::value;
+                float d[U][V], z[U][V];
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    load_f32<T, V>(gy + (i + u * ty) * ldg + col, d[u]);
+                    if (ACT != PLNLP_ACT_NONE) load_f32<T, V>(pre + (i + u * ty) * ldp + col, z[u]);
+                }
+                if (ACT != PLNLP_ACT_NONE)
+#pragma unroll
+                    for (int u = 0; u < U; ++u) {
+#pragma unroll
+                        for (int j = 0; j < V; ++j) d[u][j] *= act_slope<ACT>(z[u][j]);
+                        store_f32<T, V>(dz + (i + u * ty) * ldz + col, d[u]);
+                    }
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+#pragma unroll
+                    for (int j = 0; j < V; ++j) s[j] += d[u][j];
+            };
+            for (; i + 3 * ty < hi; i += 4 * ty) go(std::integral_constant<int, 4>{});
+            for (; i < hi; i += ty) go(std::integral_constant<int, 1>{});
+        }
+        if (!partial) continue;
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < V; ++j) lds[(y * V + j) * tx + x] = s[j];
+        __syncthreads();
+        if (y == 0 && c < packs) {
+            for (int t = 1; t < ty; ++t)
+#pragma unroll
+                for (int j = 0; j < V; ++j) s[j] += lds[(t * V + j) * tx + x];
+#pragma unroll
+            for (int j = 0; j < V; ++j) partial[(int64_t)blockIdx.x * packs * V + (int64_t)c * V + j] = s[j];
+        }
+    }
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void col_join_kernel(const float* __restrict__ partial, int blocks, int64_t n, T* __restrict__ out) {
+    __shared__ float lds[256];
+    const int x = threadIdx.x & 15, y = threadIdx.x >> 4;
+    const int64_t col = (int64_t)blockIdx.x * 16 + x;
+    float s = 0.f;
+    if (col < n)
+        for (int b = y; b < blocks; b += 16) s += partial[(int64_t)b * n + col];
+    lds[threadIdx.x] = s;
+    __syncthreads();
+    if (y == 0 && col < n) {
+        for (int t = 1; t < 16; ++t) s += lds[t * 16 + x];
+        out[col] = (T)s;
+    }
+}
+
+// ---- host ---------------------------------------------------------------------------------------------------------------
+constexpr int FEW_ROWS = 64;
+constexpr int64_t LINEAR_MAX = (int64_t)1 << 31;
+
+static bool units_ok(const void* p, int64_t ld, int64_t along) { return (uintptr_t)p % 16 == 0 && ld % 8 == 0 && along % 8 == 0; }
+
+// tile shape and K slices of a product: 256 x 256 tiles (LDS reads per MFMA two thirds of 128 x 128's) where they alone fill the chip,
+// else 128 x 128, K cut until two workgroups a CU have work -- slices of at least four steps
+struct Plan { bool big; int tiles_m, tiles_n, slices, steps; };
+static Plan plan_product(int64_t m, int64_t n, int64_t k) {
+    Plan p{};
+    const int64_t steps = (k + BK - 1) / BK;
+    auto tiles = [](int64_t a, int64_t b) { return (a + b - 1) / b; };
+    p.big = tiles(m, 256) * tiles(n, 256) >= 256 && k >= 512 && n % 256 == 0;
+    const int b = p.big ? 256 : 128;
+    p.tiles_m = (int)tiles(m, b);
+    p.tiles_n = (int)tiles(n, b);
+    const int64_t t = (int64_t)p.tiles_m * p.tiles_n;
+    int64_t s = (p.big || t == 0) ? 1 : 512 / t;
+    s = std::max<int64_t>(1, std::min(s, steps / 4));
+    p.steps = (int)((steps + s - 1) / s);
+    p.slices = p.steps ? (int)((steps + p.steps - 1) / p.steps) : 1;
+    if (p.slices < 1) p.slices = 1;
+    return p;
+}
+static int64_t plan_bytes(const Plan& p, int64_t m, int64_t n) { return p.slices > 1 ? (int64_t)p.slices * m * n * 4 : 0; }
+
+template <typename T, int BM, int BN, int WM, int WN, bool PT, bool QT, bool VEC, int ACT>
+static int launch_tile(const TileArgs<T>& a, hipStream_t s) {
+    auto kernel = tile_kernel<T, BM, BN, WM, WN, PT, QT, VEC, ACT>;
+    constexpr int LDS = 2 * (BM + BN) * 128;
+    if (LDS > 65536) {
+        const hipError_t e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
+        if (e != hipSuccess) return (int)e;
+    }
+    hipLaunchKernelGGL(kernel, dim3((unsigned)(a.tiles_m * a.tiles_n * a.slices)), dim3(WM * WN * 64), LDS, s, a);
+    return launch_status();
+}
+
+// C = P Q^T on the tile kernel, with its finish (ACT: the activation of the finish)
+template <typename T, bool PT, bool QT, int ACT>
+static int product(const T* p, int64_t ldp, const T* q, int64_t ldq, int64_t m, int64_t n, int64_t k, const Finish<T>& fin, float* partial,
+                   hipStream_t s) {
+    const Plan pl = plan_product(m, n, k);
+    TileArgs<T> a{p, q, ldp, ldq, m, n, k, pl.tiles_m, pl.tiles_n, pl.slices, pl.steps, partial, fin};
+    auto cols_ok = [](const T* x, int64_t ld, int64_t cols) { return (uintptr_t)x % 8 == 0 && ld % 4 == 0 && cols % 4 == 0; };
+    const bool vec = fin.vec && (PT ? cols_ok(p, ldp, m) : units_ok(p, ldp, k)) && (QT ? cols_ok(q, ldq, n) : units_ok(q, ldq, k));
+    if (pl.slices > 1) {
+        const int rc = vec ? launch_tile<T, 128, 128, 2, 2, PT, QT, true, PARTIAL>(a, s) : launch_tile<T, 128, 128, 2, 2, PT, QT, false, PARTIAL>(a, s);
+        if (rc) return rc;
+        const int v = fin.vec ? 8 : 1;
+        const dim3 blocks((unsigned)std::min<int64_t>((m * (n / v) + 255) / 256, 2048));
+        if (v == 8) hipLaunchKernelGGL((slices_kernel<T, 8, ACT>), blocks, dim3(256), 0, s, partial, pl.slices, m, n, fin);
+        else hipLaunchKernelGGL((slices_kernel<T, 1, ACT>), blocks, dim3(256), 0, s, partial, pl.slices, m, n, fin);
+        return launch_status();
+    }
+    if (pl.big && vec) return launch_tile<T, 256, 256, 2, 4, PT, QT, true, ACT>(a, s);
+    if (pl.big) { a.tiles_m = (int)((m + 127) / 128); a.tiles_n = (int)((n + 127) / 128); }
+    return vec ? launch_tile<T, 128, 128, 2, 2, PT, QT, true, ACT>(a, s) : launch_tile<T, 128, 128, 2, 2, PT, QT, false, ACT>(a, s);
+}
+
+template <typename T> static Finish<T> make_finish(const void* bias, const void* res, int64_t ldr, void* pre, int64_t ldp, void* out, int64_t ldo,
+                                                   int64_t n) {
+    Finish<T> f{(const T*)bias, (const T*)res, (T*)pre, (T*)out, ldr, ldp, ldo, 0};
+    f.vec = units_ok(out, ldo, n) && (!res || units_ok(res, ldr, n)) && (!pre || units_ok(pre, ldp, n));
+    return f;
+}
+
+template <typename F> static int with_half(int d, F&& f) { return d == PLNLP_DTYPE_BF16 ? f(__bf16{}) : f(_Float16{}); }
+
+static int linear_check(int64_t m, int64_t n, int64_t k, int act, int dtype) {
+    if (m < 0 || n < 0 || k < 0 || m >= LINEAR_MAX || n >= LINEAR_MAX || k >= LINEAR_MAX) return PLNLP_E_SHAPE;
+    if (((m + 127) / 128) * ((n + 127) / 128) >= ((int64_t)1 << 30)) return PLNLP_E_SHAPE;
+    if (act < PLNLP_ACT_NONE || act > PLNLP_ACT_SILU) return PLNLP_E_UNSUPPORTED;
+    if (dtype != PLNLP_DTYPE_BF16 && dtype != PLNLP_DTYPE_F16) return PLNLP_E_UNSUPPORTED;
+    return 0;
+}
+static int matrix_check(const void* p, int64_t ld, int64_t rows, int64_t cols) {
+    if (!rows || !cols) return 0;
+    if (!p) return PLNLP_E_NULL;
+    if ((uintptr_t)p % 2) return PLNLP_E_ALIGN;
+    return ld < cols ? PLNLP_E_SHAPE : 0;
+}
+
+struct BackPlan { int64_t dz, sums, partial, bytes, rows, blocks; };
+static int64_t round256(int64_t b) { return (b + 255) / 256 * 256; }
+static BackPlan back_plan(int64_t m, int64_t n, int64_t k, int act) {
+    BackPlan b{};
+    // rows per workgroup of act_back_kernel: about 1024 workgroups, 64 rows at least
+    b.rows = std::max<int64_t>(64, (m + 1023) / 1024);
+    b.blocks = (m + b.rows - 1) / b.rows;
+    int64_t at = 0;
+    b.dz = at; at += act == PLNLP_ACT_NONE ? 0 : round256(m * ((n + 7) / 8 * 8) * 2);
+    b.sums = at; at += round256(b.blocks * n * 4);
+    b.partial = at;
+    at += round256(std::max(plan_bytes(plan_product(m, k, n), m, k), plan_bytes(plan_product(n, k, m), n, k)));
+    b.bytes = at;
+    return b;
+}
+
+}  // namespace plnlp
+
+extern "C" int64_t plnlp_linear_act_workspace_bytes(int64_t m, int64_t n, int64_t k) {
+    if (m <= 0 || n <= 0 || k < 0) return 0;
+    return plnlp::plan_bytes(plnlp::plan_product(m, n, k), m, n);
+}
+
+extern "C" int plnlp_linear_act(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, const void* residual, int64_t ldr,
+                                int act, int64_t m, int64_t n, int64_t k, void* pre, int64_t ldp, void* out, int64_t ldo, int dtype,
+                                void* workspace, int64_t workspace_bytes, void* stream) {
+    using namespace plnlp;
+    if (int rc = linear_check(m, n, k, act, dtype)) return rc;
+    if (m == 0 || n == 0) return 0;
+    int rc = matrix_check(x, ldx, m, k);
+    if (!rc) rc = matrix_check(w, ldw, n, k);
+    if (!rc) rc = matrix_check(out, ldo, m, n);
+    if (!rc && residual) rc = matrix_check(residual, ldr, m, n);
+    if (!rc && pre) rc = matrix_check(pre, ldp, m, n);
+    if (!rc && bias && (uintptr_t)bias % 2) rc = PLNLP_E_ALIGN;
+    if (rc) return rc;
+    const int64_t need = plnlp_linear_act_workspace_bytes(m, n, k);
+    hipStream_t s = (hipStream_t)stream;
+    return with_half(dtype, [&](auto tt) { return with_act(act, [&](auto at) {
+        using T = decltype(tt);
+        constexpr int A = decltype(at)::value;
+        const Finish<T> fin = make_finish<T>(bias, residual, ldr, pre, ldp, out, ldo, n);
+        if (m <= FEW_ROWS && units_ok(x, ldx, k) && units_ok(w, ldw, k)) {
+            const unsigned blocks = (unsigned)((n + 15) / 16);
+            auto run = [&](auto kernel, int waves) {
+                hipLaunchKernelGGL(kernel, dim3(blocks), dim3(waves * 64), 0, s, (const T*)x, ldx, (const T*)w, ldw, (int)m, n, k, fin);
+                return launch_status();
+            };
+            if (m <= 16) return k >= 1024 ? run(few_rows_kernel<T, 1, 8, A>, 8) : run(few_rows_kernel<T, 1, 4, A>, 4);
+            if (m <= 32) return run(few_rows_kernel<T, 2, 8, A>, 8);
+            return run(few_rows_kernel<T, 4, 8, A>, 8);
+        }
+        if (need && (!workspace || workspace_bytes < need)) return PLNLP_E_WORKSPACE;
+        if ((uintptr_t)workspace % 16) return PLNLP_E_ALIGN;
+        return product<T, false, false, A>((const T*)x, ldx, (const T*)w, ldw, m, n, k, fin, (float*)workspace, s);
+    }); });
+}
+
+extern "C" int64_t plnlp_linear_act_backward_workspace_bytes(int64_t m, int64_t n, int64_t k, int act) {
+    if (m <= 0 || n <= 0 || k < 0) return 0;
+    return plnlp::back_plan(m, n, k, act).bytes;
+}
+
+extern "C" int plnlp_linear_act_backward(const void* gy, int64_t ldg, const void* pre, int64_t ldp, int act, const void* x, int64_t ldx,
+                                         const void* w, int64_t ldw, int64_t m, int64_t n, int64_t k, void* dx, int64_t lddx, void* dw,
+                                         int64_t lddw, void* db, int dtype, void* workspace, int64_t workspace_bytes, void* stream) {
+    using namespace plnlp;
+    if (int rc = linear_check(m, n, k, act, dtype)) return rc;
+    int rc = matrix_check(gy, ldg, m, n);
+    if (!rc && act != PLNLP_ACT_NONE) rc = matrix_check(pre, ldp, m, n);
+    if (!rc && dw) rc = matrix_check(x, ldx, m, k);
+    if (!rc && dx) rc = matrix_check(w, ldw, n, k);
+    if (!rc && dx) rc = matrix_check(dx, lddx, m, k);
+    if (!rc && dw) rc = matrix_check(dw, lddw, n, k);
+    if (!rc && db && (uintptr_t)db % 2) rc = PLNLP_E_ALIGN;
+    if (rc) return rc;
+    const int64_t need = plnlp_linear_act_backward_workspace_bytes(m, n, k, act);
+    if (need && (!workspace || workspace_bytes < need)) return PLNLP_E_WORKSPACE;
+    if ((uintptr_t)workspace % 16) return PLNLP_E_ALIGN;
+    hipStream_t s = (hipStream_t)stream;
+    return with_half(dtype, [&](auto tt) {
+        using T = decltype(tt);
+        const BackPlan b = back_plan(m, n, k, act);
+        char* ws = (char*)workspace;
+        const T* dz = (const T*)gy;
+        int64_t ldz = ldg;
+        if (m > 0 && n > 0 && (act != PLNLP_ACT_NONE || db)) {
+            T* to = (T*)(ws + b.dz);
+            const int64_t ldt = (n + 7) / 8 * 8;
+            const bool vec = units_ok(gy, ldg, n) && (act == PLNLP_ACT_NONE || units_ok(pre, ldp, n));
+            const int v = vec ? 8 : 1;
+            const int64_t packs = n / v;
+            int tx = 1;
+            while (tx < 64 && tx < packs) tx <<= 1;
+            float* sums = db ? (float*)(ws + b.sums) : nullptr;
+            auto run = [&](auto kernel) {
+                hipLaunchKernelGGL(kernel, dim3((unsigned)b.blocks), dim3(256), 0, s, (const T*)gy, ldg, (const T*)pre, ldp, to, ldt, m,
+                                   (int)packs, tx, b.rows, sums);
+                return launch_status();
+            };
+            const int e = with_act(act, [&](auto at) {
+                constexpr int A = decltype(at)::value;
+                return vec ? run(act_back_kernel<T, 8, A>) : run(act_back_kernel<T, 1, A>);
+            });
+            if (e) return e;
+            if (act != PLNLP_ACT_NONE) { dz = to; ldz = ldt; }
+        }
+        if (db && n > 0) {
+            hipLaunchKernelGGL((col_join_kernel<T>), dim3((unsigned)((n + 15) / 16)), dim3(256), 0, s, (const float*)(ws + b.sums), (int)(m > 0 ? b.blocks : 0), n, (T*)db);
+            if (int e = launch_status()) return e;
+        }
+        float* partial = (float*)(ws + b.partial);
+        if (dx && m > 0 && k > 0) {
+            const Finish<T> fin = make_finish<T>(nullptr, nullptr, 0, nullptr, 0, dx, lddx, k);
+            if (int e = product<T, false, true, PLNLP_ACT_NONE>(dz, ldz, (const T*)w, ldw, m, k, n, fin, partial, s)) return e;
+        }
+        if (dw && n > 0 && k > 0) {
+            const Finish<T> fin = make_finish<T>(nullptr, nullptr, 0, nullptr, 0, dw, lddw, k);
+            if (int e = product<T, true, true, PLNLP_ACT_NONE>(dz, ldz, (const T*)x, ldx, n, k, m, fin, partial, s)) return e;
+        }
+        return 0;
+    });
+}

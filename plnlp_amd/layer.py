@@ -15,7 +15,7 @@ from __future__ import annotations
 import torch
 import torch.nn.functional as F
 
-from . import ops
+from . import mixed, ops
 from .graph import Graph
 from .ops import _Act
 
@@ -381,3 +381,40 @@ class BilinearPredictor(torch.nn.Module):
 
     def score_edges(self, h, src, dst):
         return self.forward(h[src], h[dst])
+
+
+# ------------------------------------------------- layers with 16-bit storage ------
+class ScaledEmbedding(torch.nn.Module):
+    """rows of a trainable table by id, times a constant (plnlp_amd.embedding_lookup); weight: [num_embeddings, embedding_dim]
+    of `dtype`; out_dtype: type of the rows handed out (default: the table's)"""
+
+    def __init__(self, num_embeddings: int, embedding_dim: int, scale: float = 1.0, padding_idx=None, dtype=torch.bfloat16,
+                 out_dtype=None):
+        super().__init__()
+        self.scale, self.padding_idx, self.out_dtype = float(scale), padding_idx, out_dtype
+        self.weight = torch.nn.Parameter(torch.empty(num_embeddings, embedding_dim, dtype=dtype))
+        self.reset_parameters()
+
+    def reset_parameters(self):
+        torch.nn.init.xavier_uniform_(self.weight)
+        if self.padding_idx is not None:
+            with torch.no_grad():
+                self.weight[self.padding_idx].fill_(0)
+
+    def forward(self, ids):
+        return mixed.embedding_lookup(self.weight, ids, scale=self.scale, padding_idx=self.padding_idx, out_dtype=self.out_dtype)
+
+
+class LinearAct(torch.nn.Module):
+    """activation(x W^T + bias) + residual in 16-bit storage (plnlp_amd.linear_act); parameters as torch.nn.Linear's"""
+
+    def __init__(self, in_channels: int, out_channels: int, bias: bool = True, activation: str = "none", dtype=torch.bfloat16):
+        super().__init__()
+        self.activation = activation
+        self.lin = torch.nn.Linear(in_channels, out_channels, bias=bias, dtype=dtype)
+
+    def reset_parameters(self):
+        self.lin.reset_parameters()
+
+    def forward(self, x, residual=None):
+        return mixed.linear_act(x, self.lin.weight, self.lin.bias, residual=residual, activation=self.activation)

@@ -6,7 +6,7 @@ from typing import Dict, Iterable, Optional, Sequence, Tuple
 
 import torch
 
-from . import ops
+from . import mixed, ops
 
 
 class FusedAdam(torch.optim.Optimizer):
@@ -96,3 +96,14 @@ def group_sqnorm(params: Sequence[torch.nn.Parameter]) -> Optional[torch.Tensor]
     grads = [g if g.is_contiguous() else g.contiguous() for g in grads]
     out = torch.empty(1, dtype=torch.float32, device=grads[0].device)
     return ops.sqnorm_into(grads, out)
+
+
+def clip_grad_norm_(parameters, max_norm: float, norm_type: float = 2.0) -> torch.Tensor:
+    """torch.nn.utils.clip_grad_norm_ for bf16, fp16 and fp32 gradients in any mix: two launches per 128 tensors and no host
+    synchronisation (plnlp_amd.clip_grads); parameters without a gradient are skipped"""
+    if isinstance(parameters, torch.Tensor):
+        parameters = [parameters]
+    grads = [p.grad for p in parameters if p.grad is not None]
+    if not grads:
+        return torch.tensor(0.0)
+    return mixed.clip_grads(grads, max_norm, norm_type=norm_type)
