@@ -638,7 +638,7 @@ int plnlp_transpose_f32(const float* x, int64_t ldx, float* y, int64_t ldy,
 #define PLNLP_DTYPE_F16  2
 
 /* out[t, :] = scale * table[ids[t], :]; an id outside [0, n_rows) reads as a row of zeros.  ids: int32 (id_bytes 4) or int64 (8),
- * [n_ids] consecutive; n_rows, n_ids <= 2^31 - 2.  table and out: rows ld / ldo elements apart, any of the three types, each
+ * [n_ids] consecutive; n_rows, n_ids <= 2^31 - 2, width <= 2^21.  table and out: rows ld / ldo elements apart, any of the three types, each
  * aligned to its element.  (The reference indexes its table with h[edge], plnlp/model.py:155-156.) */
 int plnlp_embedding_lookup(const void* table, int64_t ld, int table_dtype, int64_t n_rows, int64_t width,
                            const void* ids, int id_bytes, int64_t n_ids, float scale,
@@ -658,17 +658,17 @@ int plnlp_embedding_grad(const void* gy, int64_t ldg, int gy_dtype, const void* 
 #define PLNLP_ACT_SILU      4   /* z / (1 + exp(-z))                                         */
 /* out = act(x w^T + bias) + residual for x [m, k], w [n, k] (nn.Linear's layout), bias [n] (nullable), residual [m, n] (nullable),
  * all of one 16-bit type (dtype BF16 or F16), rows ld* elements apart (at most 2^31), any alignment of whole elements; 16-byte
- * aligned rows and k, n % 8 == 0 take the wide loads.  pre (nullable): z = x w^T + bias, what the backward pass reads.  out may
- * be residual itself (same rows); otherwise outputs alias nothing.  workspace: plnlp_linear_act_workspace_bytes(m, n, k) bytes,
+ * aligned rows and k, n % 8 == 0 take the wide loads.  slope (nullable): act'(x w^T + bias), what the backward pass reads, int16 in
+ * steps of 2^-14 (-32768: NaN).  out may be residual itself (same rows); otherwise outputs alias nothing.  workspace: plnlp_linear_act_workspace_bytes(m, n, k) bytes,
  * 16-byte aligned (0: none needed). */
 int64_t plnlp_linear_act_workspace_bytes(int64_t m, int64_t n, int64_t k);
 int plnlp_linear_act(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, const void* residual, int64_t ldr,
-                     int act, int64_t m, int64_t n, int64_t k, void* pre, int64_t ldp, void* out, int64_t ldo, int dtype,
+                     int act, int64_t m, int64_t n, int64_t k, int16_t* slope, int64_t lds, void* out, int64_t ldo, int dtype,
                      void* workspace, int64_t workspace_bytes, void* stream);
-/* its gradients from gy = d out: dz = gy * act'(pre); dx = dz w, dw = dz^T x, db = column sums of dz (each nullable: not wanted);
- * the residual's gradient is gy itself.  act NONE: pre is not read.  workspace as above, by its own byte count. */
+/* its gradients from gy = d out: dz = gy * slope; dx = dz w, dw = dz^T x, db = column sums of dz (each nullable: not wanted);
+ * the residual's gradient is gy itself.  act NONE: slope is not read.  workspace as above, by its own byte count. */
 int64_t plnlp_linear_act_backward_workspace_bytes(int64_t m, int64_t n, int64_t k, int act);
-int plnlp_linear_act_backward(const void* gy, int64_t ldg, const void* pre, int64_t ldp, int act, const void* x, int64_t ldx,
+int plnlp_linear_act_backward(const void* gy, int64_t ldg, const int16_t* slope, int64_t lds, int act, const void* x, int64_t ldx,
                               const void* w, int64_t ldw, int64_t m, int64_t n, int64_t k, void* dx, int64_t lddx,
                               void* dw, int64_t lddw, void* db, int dtype, void* workspace, int64_t workspace_bytes,
                               void* stream);

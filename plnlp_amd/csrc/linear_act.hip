@@ -1,8 +1,12 @@
 // y = act(x W^T + bias) + residual for 16-bit x, W, bias, residual (bf16 or fp16), and its gradients:
 //   z = x W^T + bias;  y = act(z) + residual;   dz = dy * act'(z);  dx = dz W;  dW = dz^T x;  db = sum_rows dz;  d residual = dy
 // Products on the matrix cores with f32 accumulation; bias, activation and residual on the f32 accumulators, ONE rounding to the
-// stored type.  What is rounded besides: z, kept in 16 bits for the backward pass (its derivative is taken at the rounded z:
-// a relative 2^-9 / 2^-12 of z, below what rounding dz costs anyway), and dz, which the two gradient products read as 16-bit operands.
+// stored type.  What is rounded besides:
+//   act'(z), kept for the backward pass as 16-bit FIXED point in steps of 2^-14 (|act'| <= 1.13): an absolute 2^-15, a sixth of what
+//     rounding z to fp16 (a fiftieth of what rounding it to bf16) would do to dz, for the same bytes -- and the backward pass evaluates
+//     no exponential;
+//   dz, which the two gradient products read as 16-bit operands: an error of the size of the result's own rounding, averaged over
+//     the sums.  A small dz (see TWO_TERMS) is kept as the sum of two 16-bit terms instead, its few roundings would not average.
 //
 // One tile kernel serves the three products, written as C[m, n] = sum_k P(m, k) Q(n, k):
 //   forward  P = x   (k contiguous)            Q = W (k contiguous)
@@ -11,7 +15,7 @@
 // A tile of P and of Q is staged global -> registers -> LDS as rows of 64 consecutive k (128 bytes); an operand with k along its
 // rows is transposed on the way, in registers (8 k x 4 columns a thread, sixteen v_perm_b32), so the product itself reads one
 // layout.  The 16-byte units of a row are XOR-swizzled (swz) so that the stores of both kinds and the reads hit all LDS banks.
-// Q is the MFMA's first operand and its rows are dealt so that a lane ends up with 16 CONSECUTIVE columns of one row of C: bias,
+// Q is the MFMA's first operand and its rows are dealt so that a lane ends up with groups of 8 CONSECUTIVE columns of one row of C: bias,
 // residual and result move as 16-byte accesses straight from the accumulators, with no pass through LDS.
 #include "half.hip.h"
 
@@ -52,23 +56,33 @@ __device__ __forceinline__ float normal_cdf(float z, float g) {
 constexpr float TANH_C = 1.5957691216057308f;                   // 2 sqrt(2 / pi)
 constexpr float TANH_A = 0.044715f;
 
-template <int ACT> __device__ __forceinline__ float act_of(float z) {
-    if (ACT == PLNLP_ACT_RELU) return z < 0.f ? 0.f : z;         // (a NaN stays)
-    if (ACT == PLNLP_ACT_SILU) return z * sigmoid_f(z);
-    if (ACT == PLNLP_ACT_GELU) return z * normal_cdf(z, gauss_half(z));
-    if (ACT == PLNLP_ACT_GELU_TANH) return z * sigmoid_f(TANH_C * fmaf(TANH_A * z * z, z, z));
-    return z;
-}
-template <int ACT> __device__ __forceinline__ float act_slope(float z) {
-    if (ACT == PLNLP_ACT_RELU) return z > 0.f ? 1.f : (z == z ? 0.f : z);
-    if (ACT == PLNLP_ACT_SILU) { const float s = sigmoid_f(z); return s * fmaf(z, 1.f - s, 1.f); }
-    if (ACT == PLNLP_ACT_GELU) { const float g = gauss_half(z); return fmaf(z * 0.3989422804014327f, g, normal_cdf(z, g)); }
+// act(z); SLOPE: and act'(z)
+template <int ACT, bool SLOPE> __device__ __forceinline__ float act_of(float z, float& slope) {
+    if (ACT == PLNLP_ACT_RELU) {
+        if (SLOPE) slope = z > 0.f ? 1.f : (z == z ? 0.f : z);
+        return z < 0.f ? 0.f : z;                                // (a NaN stays)
+    }
+    if (ACT == PLNLP_ACT_SILU) {
+        const float s = sigmoid_f(z);
+        if (SLOPE) slope = s * fmaf(z, 1.f - s, 1.f);
+        return z * s;
+    }
+    if (ACT == PLNLP_ACT_GELU) {
+        const float g = gauss_half(z), c = normal_cdf(z, g);
+        if (SLOPE) slope = fmaf(z * 0.3989422804014327f, g, c);
+        return z * c;
+    }
     if (ACT == PLNLP_ACT_GELU_TANH) {
         const float s = sigmoid_f(TANH_C * fmaf(TANH_A * z * z, z, z));
-        return fmaf(z * s * (1.f - s), TANH_C * fmaf(3.f * TANH_A * z, z, 1.f), s);
+        if (SLOPE) slope = fmaf(z * s * (1.f - s), TANH_C * fmaf(3.f * TANH_A * z, z, 1.f), s);
+        return z * s;
     }
-    return 1.f;
+    return z;
 }
+constexpr float SLOPE_STEP = 1.f / 16384.f;
+constexpr int SLOPE_NAN = -32768;
+__device__ __forceinline__ int16_t pack_slope(float s) { return s == s ? (int16_t)__float2int_rn(s * 16384.f) : (int16_t)SLOPE_NAN; }
+__device__ __forceinline__ float unpack_slope(int16_t q) { return q == SLOPE_NAN ? __builtin_nanf("") : (float)q * SLOPE_STEP; }
 // f(std::integral_constant<int, ACT>{}) of a run-time activation
 template <typename F> __host__ __device__ __forceinline__ int with_act(int act, F&& f) {
     switch (act) {
@@ -84,7 +98,7 @@ template <typename F> __host__ __device__ __forceinline__ int with_act(int act, 
 template <typename T> struct Finish {
     const T* bias;          // nullable [n]
     const T* res;           // nullable [m, ldr]
-    T*       pre;           // nullable [m, ldp]: z, for the backward pass
+    int16_t* slope;         // nullable [m, ldp]: act'(z), for the backward pass
     T*       out;           // [m, ldo]
     int64_t  ldr, ldp, ldo;
     int      vec;           // 8-column groups may move as 16 bytes
@@ -95,9 +109,15 @@ constexpr int PARTIAL = -1; // in the place of an activation: the sum is one K s
 template <int ACT, typename T, int V> __device__ __forceinline__ void finish_cols(const Finish<T>& f, float (&v)[V], const float (&b)[V], int64_t m, int64_t n) {
 #pragma unroll
     for (int j = 0; j < V; ++j) v[j] += b[j];
-    if (f.pre) store_f32<T, V>(f.pre + m * f.ldp + n, v);
+    float s[V];
+    if (ACT != PLNLP_ACT_NONE && f.slope) {
+        Pack<int16_t, V> q;
 #pragma unroll
-    for (int j = 0; j < V; ++j) v[j] = act_of<ACT>(v[j]);
+        for (int j = 0; j < V; ++j) { v[j] = act_of<ACT, true>(v[j], s[j]); q.v[j] = pack_slope(s[j]); }
+        *reinterpret_cast<Pack<int16_t, V>*>(f.slope + m * f.ldp + n) = q;
+    } else
+#pragma unroll
+        for (int j = 0; j < V; ++j) v[j] = act_of<ACT, false>(v[j], s[j]);
     if (f.res) {
         float r[V];
         load_f32<T, V>(f.res + m * f.ldr + n, r);
@@ -112,14 +132,20 @@ template <typename T> struct TileArgs {
     const T* p; const T* q;
     int64_t  ldp, ldq;
     int64_t  m, n, k;
-    int      tiles_m, tiles_n, slices, steps;     // steps: BK-steps per K slice
+    int64_t  plane;                                // P's second term lies this many elements behind its first
+    int      terms;                                // 1, or 2: C = (P + P2) Q^T as one sum over twice as many steps
+    int      tiles_m, tiles_n, slices, steps;      // steps: BK-steps per slice
     float*   partial;                              // slices > 1: [slices, m, n]
     Finish<T> fin;
 };
 
 // which 16-byte unit of LDS row r holds unit 0 (unit u sits at u ^ swz): eight lanes that read rows 0..7, or the permuted Q rows
-// {0..3, 16..19}, or that store a transposed block's rows 4 apart, touch eight different units
-__device__ __forceinline__ int swz(int r) { return (r & 7) ^ ((r >> 3) & 1) ^ (((r >> 4) & 1) * 6); }
+// {0..3, 8..11}, or that store a transposed block's rows 4 apart, touch eight different units
+__device__ __forceinline__ int swz(int r) { return (r & 7) ^ (((r >> 3) & 1) * 6) ^ ((r >> 4) & 1); }
+
+// Q row (column of C) behind row r of the MFMA's tile t: lane group g = r >> 2 gets columns 32 (t / 2) + 8 g + 4 (t & 1) + 0..3, so its
+// tiles 2h and 2h + 1 are eight consecutive columns, and the four groups' stores 64 consecutive bytes
+__device__ __forceinline__ int q_row(int t, int r) { return 32 * (t >> 1) + 8 * (r >> 2) + 4 * (t & 1) + (r & 3); }
 
 // registers of one operand's tile (R rows x BK), one thread's share
 template <int R, int THREADS> struct Stage { u32x4 r[R * 8 / THREADS]; };
@@ -212,8 +238,8 @@ __global__ __launch_bounds__(WM * WN * 64) void tile_kernel(TileArgs<T> a) {
 
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
     const int wm = (wave / WN) * (BM / WM), wn = (wave % WN) * 64;
-    const int64_t k_lo = (int64_t)slice * a.steps * BK, k_hi = min(a.k, k_lo + (int64_t)a.steps * BK);
-    const int steps = k_hi > k_lo ? (int)((k_hi - k_lo + BK - 1) / BK) : 0;
+    const int term_steps = (int)((a.k + BK - 1) / BK), first = slice * a.steps;
+    const int steps = min(a.steps, term_steps * a.terms - first);
     const int rows_p = (int)min((int64_t)BM, a.m - m0), rows_q = (int)min((int64_t)BN, a.n - n0);
 
     f32x4 acc[TM][4];
@@ -225,9 +251,11 @@ __global__ __launch_bounds__(WM * WN * 64) void tile_kernel(TileArgs<T> a) {
     Stage<BM, THREADS> sp;
     Stage<BN, THREADS> sq;
     auto fetch = [&](int step) {
-        const int64_t k = k_lo + (int64_t)step * BK, left = k_hi - k;
-        if (PT) fetch_cols<T, BM, THREADS, VEC>(sp, a.p + k * a.ldp + m0, a.ldp, rows_p, left);
-        else fetch_rows<T, BM, THREADS, VEC>(sp, a.p + m0 * a.ldp + k, a.ldp, rows_p, left);
+        const int at = first + step, term = at >= term_steps;
+        const int64_t k = (int64_t)(at - (term ? term_steps : 0)) * BK, left = a.k - k;
+        const T* p = a.p + (term ? a.plane : 0);
+        if (PT) fetch_cols<T, BM, THREADS, VEC>(sp, p + k * a.ldp + m0, a.ldp, rows_p, left);
+        else fetch_rows<T, BM, THREADS, VEC>(sp, p + m0 * a.ldp + k, a.ldp, rows_p, left);
         if (QT) fetch_cols<T, BN, THREADS, VEC>(sq, a.q + k * a.ldq + n0, a.ldq, rows_q, left);
         else fetch_rows<T, BN, THREADS, VEC>(sq, a.q + n0 * a.ldq + k, a.ldq, rows_q, left);
     };
@@ -251,7 +279,7 @@ __global__ __launch_bounds__(WM * WN * 64) void tile_kernel(TileArgs<T> a) {
             frag q[4];
 #pragma unroll
             for (int t = 0; t < 4; ++t) {
-                const int row = wn + 16 * (r >> 2) + 4 * t + (r & 3);
+                const int row = wn + q_row(t, r);
                 q[t] = *reinterpret_cast<const frag*>(b + (BM + row) * 128 + (((ks * 4 + g) ^ swz(row)) << 4));
             }
 #pragma unroll
@@ -265,64 +293,80 @@ __global__ __launch_bounds__(WM * WN * 64) void tile_kernel(TileArgs<T> a) {
         __syncthreads();
     }
 
-    // lane (r, g) holds columns n .. n + 15 of rows wm + 16 i + r
-    const int64_t n = n0 + wn + 16 * g;
-    if (n >= a.n) return;
-    const int cols = (int)min((int64_t)16, a.n - n);
-    float bias[16];
+    // lane (r, g) holds columns n + 32 h + 0..7 (h = 0, 1) of rows wm + 16 i + r
+    const int64_t n = n0 + wn + 8 * g;
+    int cols[2];
 #pragma unroll
-    for (int j = 0; j < 16; ++j) bias[j] = (ACT != PARTIAL && a.fin.bias && j < cols) ? (float)a.fin.bias[n + j] : 0.f;
+    for (int h = 0; h < 2; ++h) cols[h] = (int)max(min((int64_t)8, a.n - n - 32 * h), (int64_t)0);
+    float bias[2][8];
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) bias[h][j] = (ACT != PARTIAL && a.fin.bias && j < cols[h]) ? (float)a.fin.bias[n + 32 * h + j] : 0.f;
 #pragma unroll
     for (int i = 0; i < TM; ++i) {
         const int64_t m = m0 + wm + i * 16 + r;
         if (m >= a.m) continue;
-        if constexpr (ACT == PARTIAL) {
-            float* o = a.partial + ((int64_t)slice * a.m + m) * a.n + n;
 #pragma unroll
-            for (int t = 0; t < 4; ++t) {
-                if (VEC) {
-                    if (4 * t < cols) *reinterpret_cast<f32x4*>(o + 4 * t) = acc[i][t];
-                } else
+        for (int h = 0; h < 2; ++h) {
+            const int64_t col = n + 32 * h;
+            if (cols[h] <= 0) continue;
+            if constexpr (ACT == PARTIAL) {
+                float* o = a.partial + ((int64_t)slice * a.m + m) * a.n + col;
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) if (4 * t + j < cols) o[4 * t + j] = acc[i][t][j];
-            }
-        } else if constexpr (VEC) {                       // (n and the strides are whole groups of eight)
+                for (int t = 0; t < 2; ++t) {
+                    if (VEC) *reinterpret_cast<f32x4*>(o + 4 * t) = acc[i][2 * h + t];      // (n is whole groups of eight)
+                    else
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                if (8 * h >= cols) continue;
-                float v[8], b[8];
-#pragma unroll
-                for (int j = 0; j < 8; ++j) { v[j] = acc[i][2 * h + (j >> 2)][j & 3]; b[j] = bias[8 * h + j]; }
-                finish_cols<ACT, T, 8>(a.fin, v, b, m, n + 8 * h);
-            }
-        } else {
-#pragma unroll
-            for (int j = 0; j < 16; ++j)
-                if (j < cols) {
-                    float v[1] = {acc[i][j >> 2][j & 3]}, b[1] = {bias[j]};
-                    finish_cols<ACT, T, 1>(a.fin, v, b, m, n + j);
+                        for (int j = 0; j < 4; ++j) if (4 * t + j < cols[h]) o[4 * t + j] = acc[i][2 * h + t][j];
                 }
+            } else if constexpr (VEC) {
+                float v[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) v[j] = acc[i][2 * h + (j >> 2)][j & 3];
+                finish_cols<ACT, T, 8>(a.fin, v, bias[h], m, col);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    if (j < cols[h]) {
+                        float v[1] = {acc[i][2 * h + (j >> 2)][j & 3]}, b[1] = {bias[h][j]};
+                        finish_cols<ACT, T, 1>(a.fin, v, b, m, col + j);
+                    }
+            }
         }
     }
 }
 
-// sum of the K slices in slice order, then the finish
+// the slices' sums, then the finish: 64 lanes of V columns a workgroup, its four waves share the slices (wave w: w, w + 4, ...; joined in
+// wave order), so that a small result over many slices still has loads enough in flight
 template <typename T, int V, int ACT>
 __global__ __launch_bounds__(256) void slices_kernel(const float* __restrict__ partial, int slices, int64_t m, int64_t n, Finish<T> fin) {
-    const int64_t groups = n / V, total = m * groups;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-        const int64_t row = i / groups, col = (i - row * groups) * V;
-        float v[V] = {}, b[V] = {};
-        for (int s = 0; s < slices; ++s) {
-            const float* p = partial + ((int64_t)s * m + row) * n + col;
+    __shared__ float lds[4][V][64];
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const int64_t groups = n / V, i = (int64_t)blockIdx.x * 64 + lane, row = i / groups, col = (i - row * groups) * V;
+    const bool in = row < m;
+    float v[V] = {}, b[V] = {};
+    if (in) {
+        const float* p = partial + row * n + col;
+#pragma unroll 8
+        for (int s = wave; s < slices; s += 4) {
+            float x[V];
+            load_f32<float, V>(p + (int64_t)s * m * n, x);
 #pragma unroll
-            for (int j = 0; j < V; ++j) v[j] += p[j];
+            for (int j = 0; j < V; ++j) v[j] += x[j];
         }
-        if (fin.bias)
-#pragma unroll
-            for (int j = 0; j < V; ++j) b[j] = (float)fin.bias[col + j];
-        finish_cols<ACT, T, V>(fin, v, b, row, col);
     }
+#pragma unroll
+    for (int j = 0; j < V; ++j) lds[wave][j][lane] = v[j];
+    __syncthreads();
+    if (wave || !in) return;
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+        for (int w = 1; w < 4; ++w) v[j] += lds[w][j][lane];
+    if (fin.bias)
+#pragma unroll
+        for (int j = 0; j < V; ++j) b[j] = (float)fin.bias[col + j];
+    finish_cols<ACT, T, V>(fin, v, b, row, col);
 }
 
 // ---- few rows: the weights stream from memory once, straight into the MFMA's registers ---------------------------
@@ -384,10 +428,11 @@ __global__ __launch_bounds__(WAVES * 64) void few_rows_kernel(const T* __restric
 }
 
 // ---- dz = dy * act'(z), and the column sums of dz ---------------------------------------------------------------------
-// 256 / tx rows of tx lanes, V columns a lane; a workgroup takes `rows` consecutive rows and leaves their column sums in partial[block, :]
-template <typename T, int V, int ACT>
-__global__ __launch_bounds__(256) void act_back_kernel(const T* __restrict__ gy, int64_t ldg, const T* __restrict__ pre, int64_t ldp,
-                                                       T* __restrict__ dz, int64_t ldz, int64_t m, int packs, int tx, int64_t rows,
+// 256 / tx rows of tx lanes, V columns a lane; a workgroup takes `rows` consecutive rows and leaves their column sums (of dz before it
+// is rounded) in partial[block, :].  plane > 0: what rounding leaves of dz goes `plane` elements behind it.  SLOPE false: dz = dy, sums only.
+template <typename T, int V, bool SLOPE>
+__global__ __launch_bounds__(256) void act_back_kernel(const T* __restrict__ gy, int64_t ldg, const int16_t* __restrict__ slope, int64_t lds_,
+                                                       T* __restrict__ dz, int64_t ldz, int64_t plane, int64_t m, int packs, int tx, int64_t rows,
                                                        float* __restrict__ partial) {
     __shared__ float lds[256 * V];
     const int x = threadIdx.x & (tx - 1), y = threadIdx.x / tx, ty = 256 / tx;
@@ -400,23 +445,31 @@ __global__ __launch_bounds__(256) void act_back_kernel(const T* __restrict__ gy,
             int64_t i = lo + y;
             auto go = [&](auto count) {
                 constexpr int U = decltype(count)::value;
-                float d[U][V], z[U][V];
+                Pack<T, V> d[U];
+                Pack<int16_t, V> q[U];
 #pragma unroll
                 for (int u = 0; u < U; ++u) {
-                    load_f32<T, V>(gy + (i + u * ty) * ldg + col, d[u]);
-                    if (ACT != PLNLP_ACT_NONE) load_f32<T, V>(pre + (i + u * ty) * ldp + col, z[u]);
+                    d[u] = *reinterpret_cast<const Pack<T, V>*>(gy + (i + u * ty) * ldg + col);
+                    if (SLOPE) q[u] = *reinterpret_cast<const Pack<int16_t, V>*>(slope + (i + u * ty) * lds_ + col);
                 }
-                if (ACT != PLNLP_ACT_NONE)
 #pragma unroll
-                    for (int u = 0; u < U; ++u) {
+                for (int u = 0; u < U; ++u) {
+                    float z[V];
 #pragma unroll
-                        for (int j = 0; j < V; ++j) d[u][j] *= act_slope<ACT>(z[u][j]);
-                        store_f32<T, V>(dz + (i + u * ty) * ldz + col, d[u]);
+                    for (int j = 0; j < V; ++j) {
+                        z[j] = (float)d[u].v[j] * (SLOPE ? unpack_slope(q[u].v[j]) : 1.f);
+                        s[j] += z[j];
                     }
+                    if (SLOPE) {
+                        T* o = dz + (i + u * ty) * ldz + col;
+                        store_f32<T, V>(o, z);
+                        if (plane) {
 #pragma unroll
-                for (int u = 0; u < U; ++u)
-#pragma unroll
-                    for (int j = 0; j < V; ++j) s[j] += d[u][j];
+                            for (int j = 0; j < V; ++j) z[j] -= (float)(T)z[j];
+                            store_f32<T, V>(o + plane, z);
+                        }
+                    }
+                }
             };
             for (; i + 3 * ty < hi; i += 4 * ty) go(std::integral_constant<int, 4>{});
             for (; i < hi; i += ty) go(std::integral_constant<int, 1>{});
@@ -436,18 +489,22 @@ __global__ __launch_bounds__(256) void act_back_kernel(const T* __restrict__ gy,
     }
 }
 
+// the blocks' column sums, added: 16 columns a workgroup, 64 threads a column with up to 16 loads in flight each
 template <typename T>
-__global__ __launch_bounds__(256) void col_join_kernel(const float* __restrict__ partial, int blocks, int64_t n, T* __restrict__ out) {
-    __shared__ float lds[256];
+__global__ __launch_bounds__(1024) void col_join_kernel(const float* __restrict__ partial, int blocks, int64_t n, T* __restrict__ out) {
+    __shared__ float lds[16][16];
     const int x = threadIdx.x & 15, y = threadIdx.x >> 4;
     const int64_t col = (int64_t)blockIdx.x * 16 + x;
     float s = 0.f;
     if (col < n)
-        for (int b = y; b < blocks; b += 16) s += partial[(int64_t)b * n + col];
-    lds[threadIdx.x] = s;
+#pragma unroll 16
+        for (int b = y; b < blocks; b += 64) s += partial[(int64_t)b * n + col];
+    s += __shfl_xor(s, 16, 64);
+    s += __shfl_xor(s, 32, 64);
+    if ((threadIdx.x & 63) < 16) lds[threadIdx.x >> 6][x] = s;
     __syncthreads();
-    if (y == 0 && col < n) {
-        for (int t = 1; t < 16; ++t) s += lds[t * 16 + x];
+    if (threadIdx.x < 16 && col < n) {
+        for (int w = 1; w < 16; ++w) s += lds[w][x];
         out[col] = (T)s;
     }
 }
@@ -461,9 +518,9 @@ static bool units_ok(const void* p, int64_t ld, int64_t along) { return (uintptr
 // tile shape and K slices of a product: 256 x 256 tiles (LDS reads per MFMA two thirds of 128 x 128's) where they alone fill the chip,
 // else 128 x 128, K cut until two workgroups a CU have work -- slices of at least four steps
 struct Plan { bool big; int tiles_m, tiles_n, slices, steps; };
-static Plan plan_product(int64_t m, int64_t n, int64_t k) {
+static Plan plan_product(int64_t m, int64_t n, int64_t k, int terms = 1) {
     Plan p{};
-    const int64_t steps = (k + BK - 1) / BK;
+    const int64_t steps = (k + BK - 1) / BK * terms;
     auto tiles = [](int64_t a, int64_t b) { return (a + b - 1) / b; };
     p.big = tiles(m, 256) * tiles(n, 256) >= 256 && k >= 512 && n % 256 == 0;
     const int b = p.big ? 256 : 128;
@@ -493,17 +550,18 @@ static int launch_tile(const TileArgs<T>& a, hipStream_t s) {
 
 // C = P Q^T on the tile kernel, with its finish (ACT: the activation of the finish)
 template <typename T, bool PT, bool QT, int ACT>
-static int product(const T* p, int64_t ldp, const T* q, int64_t ldq, int64_t m, int64_t n, int64_t k, const Finish<T>& fin, float* partial,
-                   hipStream_t s) {
-    const Plan pl = plan_product(m, n, k);
-    TileArgs<T> a{p, q, ldp, ldq, m, n, k, pl.tiles_m, pl.tiles_n, pl.slices, pl.steps, partial, fin};
+static int product(const T* p, int64_t ldp, int64_t plane, const T* q, int64_t ldq, int64_t m, int64_t n, int64_t k, const Finish<T>& fin,
+                   float* partial, hipStream_t s) {
+    const int terms = plane ? 2 : 1;
+    const Plan pl = plan_product(m, n, k, terms);
+    TileArgs<T> a{p, q, ldp, ldq, m, n, k, plane, terms, pl.tiles_m, pl.tiles_n, pl.slices, pl.steps, partial, fin};
     auto cols_ok = [](const T* x, int64_t ld, int64_t cols) { return (uintptr_t)x % 8 == 0 && ld % 4 == 0 && cols % 4 == 0; };
     const bool vec = fin.vec && (PT ? cols_ok(p, ldp, m) : units_ok(p, ldp, k)) && (QT ? cols_ok(q, ldq, n) : units_ok(q, ldq, k));
     if (pl.slices > 1) {
         const int rc = vec ? launch_tile<T, 128, 128, 2, 2, PT, QT, true, PARTIAL>(a, s) : launch_tile<T, 128, 128, 2, 2, PT, QT, false, PARTIAL>(a, s);
         if (rc) return rc;
         const int v = fin.vec ? 8 : 1;
-        const dim3 blocks((unsigned)std::min<int64_t>((m * (n / v) + 255) / 256, 2048));
+        const dim3 blocks((unsigned)((m * (n / v) + 63) / 64));
         if (v == 8) hipLaunchKernelGGL((slices_kernel<T, 8, ACT>), blocks, dim3(256), 0, s, partial, pl.slices, m, n, fin);
         else hipLaunchKernelGGL((slices_kernel<T, 1, ACT>), blocks, dim3(256), 0, s, partial, pl.slices, m, n, fin);
         return launch_status();
@@ -513,10 +571,10 @@ static int product(const T* p, int64_t ldp, const T* q, int64_t ldq, int64_t m, 
     return vec ? launch_tile<T, 128, 128, 2, 2, PT, QT, true, ACT>(a, s) : launch_tile<T, 128, 128, 2, 2, PT, QT, false, ACT>(a, s);
 }
 
-template <typename T> static Finish<T> make_finish(const void* bias, const void* res, int64_t ldr, void* pre, int64_t ldp, void* out, int64_t ldo,
+template <typename T> static Finish<T> make_finish(const void* bias, const void* res, int64_t ldr, int16_t* slope, int64_t ldp, void* out, int64_t ldo,
                                                    int64_t n) {
-    Finish<T> f{(const T*)bias, (const T*)res, (T*)pre, (T*)out, ldr, ldp, ldo, 0};
-    f.vec = units_ok(out, ldo, n) && (!res || units_ok(res, ldr, n)) && (!pre || units_ok(pre, ldp, n));
+    Finish<T> f{(const T*)bias, (const T*)res, slope, (T*)out, ldr, ldp, ldo, 0};
+    f.vec = units_ok(out, ldo, n) && (!res || units_ok(res, ldr, n)) && (!slope || units_ok(slope, ldp, n));
     return f;
 }
 
@@ -536,18 +594,26 @@ static int matrix_check(const void* p, int64_t ld, int64_t rows, int64_t cols) {
     return ld < cols ? PLNLP_E_SHAPE : 0;
 }
 
-struct BackPlan { int64_t dz, sums, partial, bytes, rows, blocks; };
+// a dz of at most this many elements is kept as two 16-bit terms: its products are latency-bound and the second term costs nothing to
+// speak of, while with few elements the rounding of a single one shows in the result
+constexpr int64_t TWO_TERMS = 16384;
+
+struct BackPlan { int64_t dz, plane, ldz, sums, partial, bytes, rows, blocks; };
 static int64_t round256(int64_t b) { return (b + 255) / 256 * 256; }
 static BackPlan back_plan(int64_t m, int64_t n, int64_t k, int act) {
     BackPlan b{};
     // rows per workgroup of act_back_kernel: about 1024 workgroups, 64 rows at least
     b.rows = std::max<int64_t>(64, (m + 1023) / 1024);
     b.blocks = (m + b.rows - 1) / b.rows;
+    b.ldz = (n + 7) / 8 * 8;
+    const bool two = act != PLNLP_ACT_NONE && m * n <= TWO_TERMS;
+    b.plane = two ? m * b.ldz : 0;
     int64_t at = 0;
-    b.dz = at; at += act == PLNLP_ACT_NONE ? 0 : round256(m * ((n + 7) / 8 * 8) * 2);
+    b.dz = at; at += act == PLNLP_ACT_NONE ? 0 : round256(m * b.ldz * 2 * (two ? 2 : 1));
     b.sums = at; at += round256(b.blocks * n * 4);
     b.partial = at;
-    at += round256(std::max(plan_bytes(plan_product(m, k, n), m, k), plan_bytes(plan_product(n, k, m), n, k)));
+    const int terms = two ? 2 : 1;
+    at += round256(std::max(plan_bytes(plan_product(m, k, n, terms), m, k), plan_bytes(plan_product(n, k, m, terms), n, k)));
     b.bytes = at;
     return b;
 }
@@ -560,7 +626,7 @@ extern "C" int64_t plnlp_linear_act_workspace_bytes(int64_t m, int64_t n, int64_
 }
 
 extern "C" int plnlp_linear_act(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, const void* residual, int64_t ldr,
-                                int act, int64_t m, int64_t n, int64_t k, void* pre, int64_t ldp, void* out, int64_t ldo, int dtype,
+                                int act, int64_t m, int64_t n, int64_t k, int16_t* slope, int64_t lds, void* out, int64_t ldo, int dtype,
                                 void* workspace, int64_t workspace_bytes, void* stream) {
     using namespace plnlp;
     if (int rc = linear_check(m, n, k, act, dtype)) return rc;
@@ -569,7 +635,7 @@ extern "C" int plnlp_linear_act(const void* x, int64_t ldx, const void* w, int64
     if (!rc) rc = matrix_check(w, ldw, n, k);
     if (!rc) rc = matrix_check(out, ldo, m, n);
     if (!rc && residual) rc = matrix_check(residual, ldr, m, n);
-    if (!rc && pre) rc = matrix_check(pre, ldp, m, n);
+    if (!rc && slope) rc = matrix_check(slope, lds, m, n);
     if (!rc && bias && (uintptr_t)bias % 2) rc = PLNLP_E_ALIGN;
     if (rc) return rc;
     const int64_t need = plnlp_linear_act_workspace_bytes(m, n, k);
@@ -577,7 +643,7 @@ extern "C" int plnlp_linear_act(const void* x, int64_t ldx, const void* w, int64
     return with_half(dtype, [&](auto tt) { return with_act(act, [&](auto at) {
         using T = decltype(tt);
         constexpr int A = decltype(at)::value;
-        const Finish<T> fin = make_finish<T>(bias, residual, ldr, pre, ldp, out, ldo, n);
+        const Finish<T> fin = make_finish<T>(bias, residual, ldr, slope, lds, out, ldo, n);
         if (m <= FEW_ROWS && units_ok(x, ldx, k) && units_ok(w, ldw, k)) {
             const unsigned blocks = (unsigned)((n + 15) / 16);
             auto run = [&](auto kernel, int waves) {
@@ -590,7 +656,7 @@ extern "C" int plnlp_linear_act(const void* x, int64_t ldx, const void* w, int64
         }
         if (need && (!workspace || workspace_bytes < need)) return PLNLP_E_WORKSPACE;
         if ((uintptr_t)workspace % 16) return PLNLP_E_ALIGN;
-        return product<T, false, false, A>((const T*)x, ldx, (const T*)w, ldw, m, n, k, fin, (float*)workspace, s);
+        return product<T, false, false, A>((const T*)x, ldx, 0, (const T*)w, ldw, m, n, k, fin, (float*)workspace, s);
     }); });
 }
 
@@ -599,13 +665,13 @@ extern "C" int64_t plnlp_linear_act_backward_workspace_bytes(int64_t m, int64_t 
     return plnlp::back_plan(m, n, k, act).bytes;
 }
 
-extern "C" int plnlp_linear_act_backward(const void* gy, int64_t ldg, const void* pre, int64_t ldp, int act, const void* x, int64_t ldx,
+extern "C" int plnlp_linear_act_backward(const void* gy, int64_t ldg, const int16_t* slope, int64_t lds, int act, const void* x, int64_t ldx,
                                          const void* w, int64_t ldw, int64_t m, int64_t n, int64_t k, void* dx, int64_t lddx, void* dw,
                                          int64_t lddw, void* db, int dtype, void* workspace, int64_t workspace_bytes, void* stream) {
     using namespace plnlp;
     if (int rc = linear_check(m, n, k, act, dtype)) return rc;
     int rc = matrix_check(gy, ldg, m, n);
-    if (!rc && act != PLNLP_ACT_NONE) rc = matrix_check(pre, ldp, m, n);
+    if (!rc && act != PLNLP_ACT_NONE) rc = matrix_check(slope, lds, m, n);
     if (!rc && dw) rc = matrix_check(x, ldx, m, k);
     if (!rc && dx) rc = matrix_check(w, ldw, n, k);
     if (!rc && dx) rc = matrix_check(dx, lddx, m, k);
@@ -620,41 +686,35 @@ extern "C" int plnlp_linear_act_backward(const void* gy, int64_t ldg, const void
         using T = decltype(tt);
         const BackPlan b = back_plan(m, n, k, act);
         char* ws = (char*)workspace;
-        const T* dz = (const T*)gy;
-        int64_t ldz = ldg;
-        if (m > 0 && n > 0 && (act != PLNLP_ACT_NONE || db)) {
-            T* to = (T*)(ws + b.dz);
-            const int64_t ldt = (n + 7) / 8 * 8;
-            const bool vec = units_ok(gy, ldg, n) && (act == PLNLP_ACT_NONE || units_ok(pre, ldp, n));
-            const int v = vec ? 8 : 1;
-            const int64_t packs = n / v;
+        const bool has_act = act != PLNLP_ACT_NONE;
+        const T* dz = has_act ? (const T*)(ws + b.dz) : (const T*)gy;
+        const int64_t ldz = has_act ? b.ldz : ldg, plane = b.plane;
+        if (m > 0 && n > 0 && (has_act || db)) {
+            const bool vec = units_ok(gy, ldg, n) && (!has_act || units_ok(slope, lds, n));
+            const int64_t packs = vec ? n / 8 : n;
             int tx = 1;
             while (tx < 64 && tx < packs) tx <<= 1;
-            float* sums = db ? (float*)(ws + b.sums) : nullptr;
             auto run = [&](auto kernel) {
-                hipLaunchKernelGGL(kernel, dim3((unsigned)b.blocks), dim3(256), 0, s, (const T*)gy, ldg, (const T*)pre, ldp, to, ldt, m,
-                                   (int)packs, tx, b.rows, sums);
+                hipLaunchKernelGGL(kernel, dim3((unsigned)b.blocks), dim3(256), 0, s, (const T*)gy, ldg, slope, lds, (T*)(ws + b.dz), ldz, plane, m,
+                                   (int)packs, tx, b.rows, db ? (float*)(ws + b.sums) : nullptr);
                 return launch_status();
             };
-            const int e = with_act(act, [&](auto at) {
-                constexpr int A = decltype(at)::value;
-                return vec ? run(act_back_kernel<T, 8, A>) : run(act_back_kernel<T, 1, A>);
-            });
+            const int e = has_act ? (vec ? run(act_back_kernel<T, 8, true>) : run(act_back_kernel<T, 1, true>))
+                                  : (vec ? run(act_back_kernel<T, 8, false>) : run(act_back_kernel<T, 1, false>));
             if (e) return e;
-            if (act != PLNLP_ACT_NONE) { dz = to; ldz = ldt; }
         }
         if (db && n > 0) {
-            hipLaunchKernelGGL((col_join_kernel<T>), dim3((unsigned)((n + 15) / 16)), dim3(256), 0, s, (const float*)(ws + b.sums), (int)(m > 0 ? b.blocks : 0), n, (T*)db);
+            hipLaunchKernelGGL((col_join_kernel<T>), dim3((unsigned)((n + 15) / 16)), dim3(1024), 0, s, (const float*)(ws + b.sums), (int)(m > 0 ? b.blocks : 0), n, (T*)db);
             if (int e = launch_status()) return e;
         }
         float* partial = (float*)(ws + b.partial);
         if (dx && m > 0 && k > 0) {
             const Finish<T> fin = make_finish<T>(nullptr, nullptr, 0, nullptr, 0, dx, lddx, k);
-            if (int e = product<T, false, true, PLNLP_ACT_NONE>(dz, ldz, (const T*)w, ldw, m, k, n, fin, partial, s)) return e;
+            if (int e = product<T, false, true, PLNLP_ACT_NONE>(dz, ldz, plane, (const T*)w, ldw, m, k, n, fin, partial, s)) return e;
         }
         if (dw && n > 0 && k > 0) {
             const Finish<T> fin = make_finish<T>(nullptr, nullptr, 0, nullptr, 0, dw, lddw, k);
-            if (int e = product<T, true, true, PLNLP_ACT_NONE>(dz, ldz, (const T*)x, ldx, n, k, m, fin, partial, s)) return e;
+            if (int e = product<T, true, true, PLNLP_ACT_NONE>(dz, ldz, plane, (const T*)x, ldx, n, k, m, fin, partial, s)) return e;
         }
         return 0;
     });

@@ -5,22 +5,20 @@
 // writes V rows.  Sums are f32, rounded once.
 //
 // The gradient takes no float atomics (their order would change its bits): the ids are SORTED -- (id, position) pairs, ties in
-// the order of the positions -- and every row of dE has ONE owner that finds its run of the sorted list, adds those rows of dy in a
-// fixed order and stores the row, so untouched rows need no clearing pass.
+// the order of the positions -- and the sorted list is cut into ranges of equal length, whatever the ids are.
 //   sort: up to SORT_SMALL ids in one workgroup's LDS (a bitonic network on unique 64-bit words: 1 launch); more in 1 .. 3
-//     counting passes of at most 11 bits, each stable (histogram of 4096-id tiles / offsets along the tiles / scatter).
-//   sum: a run longer than 2 * SEG (a frequent id) would make its owner's chain the launch's length, so every whole SEG-aligned
-//     piece of the sorted list that holds one id is summed beforehand by a workgroup of its own; the owner adds those partials
-//     and the two ragged ends.
+//     counting passes of at most 11 bits, each stable (histogram of the tiles / offsets along the tiles / scatter).
+//   runs: a group of lanes walks one range with eight rows of dy in flight, adds the rows of a run of equal ids and stores the row
+//     of dE when the run ends.  A run that crosses the ends of its range leaves an f32 partial there instead; the range in which
+//     it begins adds those up in order (grad_joins_kernel).  So a frequent id costs what its rows cost, spread over the chip.
+//     Further workgroups of the same launch look up which rows of dE have no id and clear them: every row is written once.
 #include "half.hip.h"
 
 namespace plnlp {
 
 constexpr int LOOKUP_THREADS = 256;
 constexpr int SORT_SMALL = 4096;          // ids one workgroup sorts in LDS
-constexpr int SORT_TILE = 4096;           // ids per workgroup and counting pass: 256 threads * 16
 constexpr int SORT_BITS = 11;             // widest digit: 2048 counters a wave, 4 waves = 32 KiB of LDS
-constexpr int SEG = 256;                  // sorted positions per partial sum of a long run
 
 template <typename I> __device__ __forceinline__ int64_t read_id(const I* ids, int64_t i) { return (int64_t)ids[i]; }
 
@@ -89,24 +87,50 @@ __global__ __launch_bounds__(1024) void sort_small_kernel(const I* __restrict__ 
     }
 }
 
-// one counting pass sorts by digit (key >> shift) & (bins - 1); FIRST: the keys come from the ids, the positions are 0 .. n-1
-template <typename I, bool FIRST>
+// One counting pass sorts by the digit (key >> shift) & (bins - 1).  A tile is 256 * ROUNDS ids; hist[tile][digit].
+// FIRST: the keys come from the ids, the positions are 0 .. n-1.
+template <typename I, bool FIRST, int ROUNDS>
 __global__ __launch_bounds__(LOOKUP_THREADS) void sort_count_kernel(const I* __restrict__ ids, const uint32_t* __restrict__ keys, int64_t n,
-                                                                    int64_t n_rows, int64_t padding, int shift, int bins, int tiles,
+                                                                    int64_t n_rows, int64_t padding, int shift, int bins,
                                                                     uint32_t* __restrict__ hist) {
     extern __shared__ uint32_t cnt[];
+    const int64_t lo = (int64_t)blockIdx.x * ROUNDS * LOOKUP_THREADS + threadIdx.x;
+    uint32_t key[ROUNDS];
+#pragma unroll
+    for (int u = 0; u < ROUNDS; ++u) {
+        const int64_t i = lo + u * LOOKUP_THREADS;
+        key[u] = i >= n ? 0 : FIRST ? sort_key(ids, i, n_rows, padding) : keys[i];
+    }
     for (int d = threadIdx.x; d < bins; d += LOOKUP_THREADS) cnt[d] = 0;
     __syncthreads();
-    const int64_t lo = (int64_t)blockIdx.x * SORT_TILE;
-#pragma unroll 4
-    for (int u = 0; u < SORT_TILE / LOOKUP_THREADS; ++u) {
-        const int64_t i = lo + u * LOOKUP_THREADS + threadIdx.x;
-        if (i >= n) break;
-        const uint32_t key = FIRST ? sort_key(ids, i, n_rows, padding) : keys[i];
-        atomicAdd(&cnt[(key >> shift) & (bins - 1)], 1u);
-    }
+#pragma unroll
+    for (int u = 0; u < ROUNDS; ++u)
+        if (lo + u * LOOKUP_THREADS < n) atomicAdd(&cnt[(key[u] >> shift) & (bins - 1)], 1u);
     __syncthreads();
-    for (int d = threadIdx.x; d < bins; d += LOOKUP_THREADS) hist[(int64_t)d * tiles + blockIdx.x] = cnt[d];
+    for (int d = threadIdx.x; d < bins; d += LOOKUP_THREADS) hist[(int64_t)blockIdx.x * bins + d] = cnt[d];
+}
+
+// counts -> exclusive offsets along the tiles, and the digits' totals: 64 digits a workgroup, its 16 waves share the tiles
+__global__ __launch_bounds__(1024) void sort_offsets_kernel(uint32_t* __restrict__ hist, int tiles, int bins, uint32_t* __restrict__ total) {
+    __shared__ uint32_t part[16][64];
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, d = blockIdx.x * 64 + lane;
+    const int per = (tiles + 15) / 16, lo = wave * per, hi = min(lo + per, tiles);
+    const bool in = d < bins;
+    uint32_t s = 0;
+#pragma unroll 8
+    for (int t = lo; t < hi; ++t) s += in ? hist[(int64_t)t * bins + d] : 0;
+    part[wave][lane] = s;
+    __syncthreads();
+    uint32_t run = 0;
+    for (int w = 0; w < wave; ++w) run += part[w][lane];
+    if (!in) return;
+    if (wave == 15) total[d] = run + s;
+#pragma unroll 8
+    for (int t = lo; t < hi; ++t) {
+        const uint32_t c = hist[(int64_t)t * bins + d];
+        hist[(int64_t)t * bins + d] = run;
+        run += c;
+    }
 }
 
 __device__ __forceinline__ uint32_t wave_scan(uint32_t v) {     // inclusive
@@ -118,58 +142,35 @@ __device__ __forceinline__ uint32_t wave_scan(uint32_t v) {     // inclusive
     return v;
 }
 
-// exclusive offsets of one digit along the tiles, and the digit's total
-__global__ __launch_bounds__(LOOKUP_THREADS) void sort_offsets_kernel(uint32_t* __restrict__ hist, int tiles, uint32_t* __restrict__ total) {
-    __shared__ uint32_t part[LOOKUP_THREADS / 64];
-    uint32_t* row = hist + (int64_t)blockIdx.x * tiles;
-    uint32_t carry = 0;
-    for (int lo = 0; lo < tiles; lo += LOOKUP_THREADS) {
-        const int i = lo + threadIdx.x;
-        const uint32_t v = i < tiles ? row[i] : 0;
-        uint32_t s = wave_scan(v);
-        if ((threadIdx.x & 63) == 63) part[threadIdx.x >> 6] = s;
-        __syncthreads();
-        uint32_t before = carry, all = 0;
-        for (int w = 0; w < LOOKUP_THREADS / 64; ++w) {
-            if (w < (int)(threadIdx.x >> 6)) before += part[w];
-            all += part[w];
-        }
-        if (i < tiles) row[i] = before + s - v;
-        carry += all;
-        __syncthreads();
-    }
-    if (threadIdx.x == 0) total[blockIdx.x] = carry;
-}
-
-template <typename I, bool FIRST>
+template <typename I, bool FIRST, int ROUNDS>
 __global__ __launch_bounds__(LOOKUP_THREADS) void sort_scatter_kernel(const I* __restrict__ ids, const uint32_t* __restrict__ keys,
                                                                       const int32_t* __restrict__ pos, int64_t n, int64_t n_rows,
-                                                                      int64_t padding, int shift, int bits, int tiles,
+                                                                      int64_t padding, int shift, int bits,
                                                                       const uint32_t* __restrict__ hist, const uint32_t* __restrict__ total,
                                                                       uint32_t* __restrict__ keys_out, int32_t* __restrict__ pos_out) {
-    constexpr int WAVES = LOOKUP_THREADS / 64, ROUNDS = SORT_TILE / LOOKUP_THREADS;
+    constexpr int WAVES = LOOKUP_THREADS / 64;
     extern __shared__ uint32_t lds[];                  // cnt[WAVES][bins]
     __shared__ uint32_t part[WAVES];
     const int bins = 1 << bits, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    for (int d = threadIdx.x; d < WAVES * bins; d += LOOKUP_THREADS) lds[d] = 0;
-    __syncthreads();
-    // ranks within the wave's own run of 1024 ids, in order: lanes of the same digit find each other by one ballot a bit
+    // ranks within the wave's own run of 64 * ROUNDS ids, in order: lanes of the same digit find each other by one ballot a bit
     uint32_t key[ROUNDS], rank[ROUNDS];
     int32_t p[ROUNDS];
     uint32_t* cnt = lds + wave * bins;
-    const int64_t lo = (int64_t)blockIdx.x * SORT_TILE + wave * (SORT_TILE / WAVES);
+    const int64_t lo = ((int64_t)blockIdx.x * WAVES + wave) * 64 * ROUNDS + lane;
 #pragma unroll
     for (int u = 0; u < ROUNDS; ++u) {
-        const int64_t i = lo + u * 64 + lane;
+        const int64_t i = lo + u * 64;
         key[u] = 0; p[u] = 0;
         if (i < n) {
             key[u] = FIRST ? sort_key(ids, i, n_rows, padding) : keys[i];
             p[u] = FIRST ? (int32_t)i : pos[i];
         }
     }
+    for (int d = threadIdx.x; d < WAVES * bins; d += LOOKUP_THREADS) lds[d] = 0;
+    __syncthreads();
 #pragma unroll
     for (int u = 0; u < ROUNDS; ++u) {
-        const bool in = lo + u * 64 + lane < n;
+        const bool in = lo + u * 64 < n;
         const uint32_t d = (key[u] >> shift) & (bins - 1);
         uint64_t same = __ballot(in);
         for (int b = 0; b < bits; ++b) {
@@ -189,7 +190,7 @@ __global__ __launch_bounds__(LOOKUP_THREADS) void sort_scatter_kernel(const I* _
     uint32_t carry = 0;
     for (int b0 = 0; b0 < bins; b0 += LOOKUP_THREADS) {
         const int d = b0 + threadIdx.x;
-        const uint32_t v = d < bins ? total[d] : 0;
+        const uint32_t v = d < bins ? total[d] : 0, h = d < bins ? hist[(int64_t)blockIdx.x * bins + d] : 0;
         const uint32_t s = wave_scan(v);
         if (lane == 63) part[wave] = s;
         __syncthreads();
@@ -199,7 +200,7 @@ __global__ __launch_bounds__(LOOKUP_THREADS) void sort_scatter_kernel(const I* _
             carry += part[w];
         }
         if (d < bins) {
-            uint32_t start = before + s - v + hist[(int64_t)d * tiles + blockIdx.x];
+            uint32_t start = before + s - v + h;
             for (int w = 0; w < WAVES; ++w) {
                 const uint32_t c = lds[w * bins + d];
                 lds[w * bins + d] = start;
@@ -210,7 +211,7 @@ __global__ __launch_bounds__(LOOKUP_THREADS) void sort_scatter_kernel(const I* _
     }
 #pragma unroll
     for (int u = 0; u < ROUNDS; ++u) {
-        if (lo + u * 64 + lane >= n) continue;
+        if (lo + u * 64 >= n) continue;
         const uint32_t at = cnt[(key[u] >> shift) & (bins - 1)] + rank[u];
         keys_out[at] = key[u];
         pos_out[at] = p[u];
@@ -218,126 +219,152 @@ __global__ __launch_bounds__(LOOKUP_THREADS) void sort_scatter_kernel(const I* _
 }
 
 // ---- gradient -----------------------------------------------------------------------------------------
-// s[j] += rows pos[b .. e) step `step` of gy, columns of this lane's pack; four rows in flight
-template <typename G, int V>
-__device__ __forceinline__ void add_rows(const G* __restrict__ gy, int64_t ldg, int64_t col, const int32_t* __restrict__ pos, int64_t b,
-                                         int64_t e, int64_t step, float (&s)[V]) {
-    int64_t i = b;
-    for (; i + 3 * step < e; i += 4 * step) {
-        float x[4][V];
-#pragma unroll
-        for (int u = 0; u < 4; ++u) load_f32<G, V>(gy + (int64_t)pos[i + u * step] * ldg + col, x[u]);
-#pragma unroll
-        for (int u = 0; u < 4; ++u)
-#pragma unroll
-            for (int j = 0; j < V; ++j) s[j] += x[u][j];
+constexpr int CLEAR_ROWS = LOOKUP_THREADS;      // rows of dE a clearing workgroup looks up, one a thread
+
+// [b, e) of sorted positions: the first position whose key is >= want
+__device__ __forceinline__ int64_t lower_bound(const uint32_t* __restrict__ keys, int64_t n, uint32_t want) {
+    int64_t lo = 0, hi = n;
+    while (lo < hi) {
+        const int64_t mid = (lo + hi) >> 1;
+        if (keys[mid] < want) lo = mid + 1; else hi = mid;
     }
-    for (; i < e; i += step) {
-        float x[V];
-        load_f32<G, V>(gy + (int64_t)pos[i] * ldg + col, x);
-#pragma unroll
-        for (int j = 0; j < V; ++j) s[j] += x[j];
-    }
+    return lo;
 }
 
-// joins the 256 / tx groups' sums in group order; group 0 holds the result
-template <int V> __device__ __forceinline__ void join_groups(float (&s)[V], float* lds, int tx) {
-    const int x = threadIdx.x & (tx - 1), y = threadIdx.x / tx, ty = LOOKUP_THREADS / tx;
-    __syncthreads();
-#pragma unroll
-    for (int j = 0; j < V; ++j) lds[(y * V + j) * tx + x] = s[j];
-    __syncthreads();
-    if (y == 0)
-        for (int g = 1; g < ty; ++g)
-#pragma unroll
-            for (int j = 0; j < V; ++j) s[j] += lds[(g * V + j) * tx + x];
-}
+template <typename G, typename E, int V> struct GradArgs {
+    const G* gy; int64_t ldg;
+    const uint32_t* keys; const int32_t* pos;
+    int64_t n, n_rows;
+    int packs, tx, slabs;             // a row is `packs` packs of V; a group of tx lanes takes one slab of tx packs
+    int range;                        // sorted positions per group
+    int64_t n_ranges, run_blocks;     // workgroups before run_blocks walk ranges, the others clear rows
+    float* head; float* tail;         // [n_ranges, packs * V]: sums of the runs that enter / leave a range
+    float scale;
+    E* grad; int64_t lde;
+};
 
-// piece i of the sorted list, [i * SEG, (i + 1) * SEG), where it holds one id: partial[i, :] = its rows of gy, added
-template <typename G, int V>
-__global__ __launch_bounds__(LOOKUP_THREADS) void grad_pieces_kernel(const G* __restrict__ gy, int64_t ldg, const uint32_t* __restrict__ keys,
-                                                                     const int32_t* __restrict__ pos, int64_t n_rows, int packs, int tx,
-                                                                     float* __restrict__ partial) {
-    __shared__ float lds[LOOKUP_THREADS * V];
-    const int64_t b = (int64_t)blockIdx.x * SEG;
-    const uint32_t key = keys[b];
-    if (key != keys[b + SEG - 1] || key >= (uint32_t)n_rows) return;
-    const int x = threadIdx.x & (tx - 1), y = threadIdx.x / tx, ty = LOOKUP_THREADS / tx;
-    for (int c0 = 0; c0 < packs; c0 += tx) {
-        const int c = c0 + x;
-        float s[V] = {};
-        if (c < packs) add_rows<G, V>(gy, ldg, (int64_t)c * V, pos, b + y, b + SEG, ty, s);
-        join_groups<V>(s, lds, tx);
-        if (y == 0 && c < packs) {
-            float* o = partial + (int64_t)blockIdx.x * packs * V + (int64_t)c * V;
+template <typename G, typename E, int V> __global__ __launch_bounds__(LOOKUP_THREADS) void grad_runs_kernel(GradArgs<G, E, V> a) {
+    const int x = threadIdx.x & (a.tx - 1), y = threadIdx.x / a.tx, ty = LOOKUP_THREADS / a.tx;
+    if (blockIdx.x >= a.run_blocks) {
+        __shared__ uint8_t none[CLEAR_ROWS];
+        const int64_t row0 = ((int64_t)blockIdx.x - a.run_blocks) * CLEAR_ROWS, row = row0 + threadIdx.x;
+        bool empty = row < a.n_rows;
+        if (empty && a.n > 0) {
+            const int64_t at = lower_bound(a.keys, a.n, (uint32_t)row);
+            empty = at == a.n || a.keys[at] != (uint32_t)row;
+        }
+        none[threadIdx.x] = empty;
+        __syncthreads();
+        const float zero[V] = {};
+        for (int r = y; r < CLEAR_ROWS; r += ty)
+            if (none[r])
+                for (int c = x; c < a.packs; c += a.tx) store_f32<E, V>(a.grad + (row0 + r) * a.lde + (int64_t)c * V, zero);
+        return;
+    }
+    const int64_t unit = (int64_t)blockIdx.x * ty + y, range = unit / a.slabs;
+    const int c = (int)(unit % a.slabs) * a.tx + x;
+    if (range >= a.n_ranges || c >= a.packs) return;
+    const int64_t b = range * a.range, e = min(b + a.range, a.n), col = (int64_t)c * V;
+    const uint32_t end = (uint32_t)a.n_rows;
+    uint32_t cur = a.keys[b];
+    bool entered = b > 0 && a.keys[b - 1] == cur;          // the current run began in an earlier range
+    float s[V] = {};
+    auto put = [&](bool leaves) {
+        if (cur >= end) return;
+        if (entered || leaves) {
+            float* o = (entered ? a.head : a.tail) + range * a.packs * V + col;
 #pragma unroll
             for (int j = 0; j < V; ++j) o[j] = s[j];
+        } else {
+#pragma unroll
+            for (int j = 0; j < V; ++j) s[j] *= a.scale;
+            store_f32<E, V>(a.grad + (int64_t)cur * a.lde + col, s);
+        }
+    };
+    constexpr int U = 8;
+    uint32_t k[U];
+    int32_t p[U];
+    auto ask = [&](int64_t i) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int64_t at = min(i + u, e - 1);
+            k[u] = a.keys[at];
+            p[u] = a.pos[at];
+        }
+    };
+    ask(b);
+    for (int64_t i = b; i < e; i += U) {
+        if (k[0] >= end) { if (cur < end) put(false); cur = end; break; }      // only ids without a gradient follow
+        Pack<G, V> row[U];
+        uint32_t key[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            key[u] = k[u];
+            row[u] = *reinterpret_cast<const Pack<G, V>*>(a.gy + (int64_t)p[u] * a.ldg + col);
+        }
+        if (i + U < e) ask(i + U);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (i + u >= e) break;
+            if (key[u] != cur) {
+                put(false);
+                cur = key[u];
+                entered = false;
+#pragma unroll
+                for (int j = 0; j < V; ++j) s[j] = 0.f;
+            }
+#pragma unroll
+            for (int j = 0; j < V; ++j) s[j] += (float)row[u].v[j];
         }
     }
+    put(e < a.n && a.keys[e] == cur);
 }
 
-constexpr int GRAD_ROWS = 64;             // rows of dE per workgroup
-constexpr int GRAD_POS = 1024;            // positions of those rows kept in LDS
-
-template <typename G, typename E, int V>
-__global__ __launch_bounds__(LOOKUP_THREADS) void grad_rows_kernel(const G* __restrict__ gy, int64_t ldg, const uint32_t* __restrict__ keys,
-                                                                   const int32_t* __restrict__ pos, int64_t n, int64_t n_rows, int packs,
-                                                                   int tx, const float* __restrict__ partial, float scale,
-                                                                   E* __restrict__ grad, int64_t lde) {
-    __shared__ int64_t beg[GRAD_ROWS + 1];
-    __shared__ int32_t near_pos[GRAD_POS];
+// the range in which a run begins that leaves it: its tail + the heads of the ranges the run enters, in order of the groups of lanes
+// that share them
+template <typename G, typename E, int V> __global__ __launch_bounds__(LOOKUP_THREADS) void grad_joins_kernel(GradArgs<G, E, V> a) {
     __shared__ float lds[LOOKUP_THREADS * V];
-    const int64_t row0 = (int64_t)blockIdx.x * GRAD_ROWS;
-    if (threadIdx.x <= GRAD_ROWS) {                   // first sorted position whose id is >= row0 + thread
-        const int64_t want = min(row0 + (int64_t)threadIdx.x, n_rows);
-        int64_t lo = 0, hi = n;
-        while (lo < hi) {
-            const int64_t mid = (lo + hi) >> 1;
-            if ((int64_t)keys[mid] < want) lo = mid + 1; else hi = mid;
+    const int64_t range = blockIdx.x, b = range * a.range, e = b + a.range;      // (not the last range: e < n)
+    const uint32_t key = a.keys[e - 1];
+    if (key >= (uint32_t)a.n_rows || a.keys[e] != key || (b > 0 && a.keys[b - 1] == key)) return;
+    const int64_t last = (lower_bound(a.keys, a.n, key + 1) - 1) / a.range;
+    const int x = threadIdx.x & (a.tx - 1), y = threadIdx.x / a.tx, ty = LOOKUP_THREADS / a.tx;
+    const int c = blockIdx.y * a.tx + x;
+    const int64_t width = (int64_t)a.packs * V, col = (int64_t)c * V;
+    float s[V] = {};
+    if (c < a.packs) {
+        if (y == 0)
+#pragma unroll
+            for (int j = 0; j < V; ++j) s[j] = a.tail[range * width + col + j];
+        int64_t i = range + 1 + y;
+        for (; i + 3 * ty <= last; i += 4 * ty) {
+            float h[4][V];
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+#pragma unroll
+                for (int j = 0; j < V; ++j) h[u][j] = a.head[(i + u * ty) * width + col + j];
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+#pragma unroll
+                for (int j = 0; j < V; ++j) s[j] += h[u][j];
         }
-        beg[threadIdx.x] = lo;
+        for (; i <= last; i += ty)
+#pragma unroll
+            for (int j = 0; j < V; ++j) s[j] += a.head[i * width + col + j];
     }
-    __syncthreads();
-    const int64_t p0 = beg[0], held = min(beg[GRAD_ROWS] - p0, (int64_t)GRAD_POS);
-    for (int i = threadIdx.x; i < held; i += LOOKUP_THREADS) near_pos[i] = pos[p0 + i];
-    __syncthreads();
-    const int x = threadIdx.x & (tx - 1), y = threadIdx.x / tx, ty = LOOKUP_THREADS / tx;
-    const int rows = (int)min((int64_t)GRAD_ROWS, n_rows - row0);
-    for (int r = y; r < rows; r += ty) {              // short runs: a group a row
-        const int64_t b = beg[r], e = beg[r + 1];
-        if (e - b > 2 * SEG) continue;
-        for (int c = x; c < packs; c += tx) {
-            float s[V] = {};
-            if (e - p0 <= GRAD_POS) add_rows<G, V>(gy, ldg, (int64_t)c * V, near_pos, b - p0, e - p0, 1, s);
-            else add_rows<G, V>(gy, ldg, (int64_t)c * V, pos, b, e, 1, s);
+    if (last - range > 1) {
 #pragma unroll
-            for (int j = 0; j < V; ++j) s[j] *= scale;
-            store_f32<E, V>(grad + (row0 + r) * lde + (int64_t)c * V, s);
-        }
+        for (int j = 0; j < V; ++j) lds[(y * V + j) * a.tx + x] = s[j];
+        __syncthreads();
+        if (y == 0)
+            for (int g = 1; g < ty; ++g)
+#pragma unroll
+                for (int j = 0; j < V; ++j) s[j] += lds[(g * V + j) * a.tx + x];
     }
-    for (int r = 0; r < rows; ++r) {                  // long runs: the workgroup a row
-        const int64_t b = beg[r], e = beg[r + 1];
-        if (e - b <= 2 * SEG) continue;
-        const int64_t i0 = (b + SEG - 1) / SEG, i1 = e / SEG;       // whole pieces [i0, i1)
-        for (int c0 = 0; c0 < packs; c0 += tx) {
-            const int c = c0 + x;
-            float s[V] = {};
-            if (c < packs) {
-                add_rows<G, V>(gy, ldg, (int64_t)c * V, pos, b + y, i0 * SEG, ty, s);
-                for (int64_t i = i0 + y; i < i1; i += ty) {
-                    const float* q = partial + i * packs * V + (int64_t)c * V;
+    if (y == 0 && c < a.packs) {
 #pragma unroll
-                    for (int j = 0; j < V; ++j) s[j] += q[j];
-                }
-                add_rows<G, V>(gy, ldg, (int64_t)c * V, pos, i1 * SEG + y, e, ty, s);
-            }
-            join_groups<V>(s, lds, tx);
-            if (y == 0 && c < packs) {
-#pragma unroll
-                for (int j = 0; j < V; ++j) s[j] *= scale;
-                store_f32<E, V>(grad + (row0 + r) * lde + (int64_t)c * V, s);
-            }
-        }
+        for (int j = 0; j < V; ++j) s[j] *= a.scale;
+        store_f32<E, V>(a.grad + (int64_t)key * a.lde + col, s);
     }
 }
 
@@ -365,25 +392,36 @@ template <typename F> static int with_pack(int v, F&& f) {
 }
 template <typename F> static int with_id(int bytes, F&& f) { return bytes == 8 ? f(int64_t{}) : f(int32_t{}); }
 
-constexpr int64_t LOOKUP_MAX = ((int64_t)1 << 31) - 2;
+constexpr int64_t LOOKUP_MAX = ((int64_t)1 << 31) - 2, LOOKUP_MAX_WIDTH = (int64_t)1 << 21;
 
 static int lookup_check(int64_t n_rows, int64_t width, int id_bytes, int64_t n_ids, int d0, int d1) {
-    if (n_rows < 0 || width < 0 || n_ids < 0 || n_rows > LOOKUP_MAX || n_ids > LOOKUP_MAX || width > ((int64_t)1 << 30)) return PLNLP_E_SHAPE;
+    if (n_rows < 0 || width < 0 || n_ids < 0 || n_rows > LOOKUP_MAX || n_ids > LOOKUP_MAX || width > LOOKUP_MAX_WIDTH) return PLNLP_E_SHAPE;
     if ((id_bytes != 4 && id_bytes != 8) || !is_dtype(d0) || !is_dtype(d1)) return PLNLP_E_UNSUPPORTED;
     return 0;
 }
 
-struct GradWorkspace { int64_t keys[2], pos[2], hist, total, partial, bytes; };
+// ids per counting tile: small tiles until there are four workgroups a CU
+static int sort_rounds(int64_t n) { return n <= ((int64_t)1 << 20) ? 4 : 16; }
+// sorted positions per group of lanes: about 4096 waves of 512 columns, 8 .. 256 positions each
+static int grad_range(int64_t n, int64_t width) {
+    int r = 8;
+    while (r < 256 && (double)n * width > (double)r * 4096 * 512) r *= 2;
+    return r;
+}
+
+struct GradWorkspace { int64_t keys[2], pos[2], hist, total, head, tail, bytes; };
 static GradWorkspace grad_workspace(int64_t n, int64_t width) {
     GradWorkspace w{};
     int64_t at = 0;
     auto take = [&](int64_t bytes) { const int64_t a = at; at += (bytes + 255) / 256 * 256; return a; };
     const bool small = n <= SORT_SMALL;
     for (int i = 0; i < (small ? 1 : 2); ++i) { w.keys[i] = take(4 * n); w.pos[i] = take(4 * n); }
-    const int64_t tiles = (n + SORT_TILE - 1) / SORT_TILE;
+    const int64_t tile = sort_rounds(n) * LOOKUP_THREADS, tiles = (n + tile - 1) / tile;
     w.hist = take(small ? 0 : 4 * tiles << SORT_BITS);
     w.total = take(small ? 0 : 4 << SORT_BITS);
-    w.partial = take(n / SEG * width * 4);
+    const int64_t range = grad_range(n, width), ranges = (n + range - 1) / range;
+    w.head = take(ranges * width * 4);
+    w.tail = take(ranges * width * 4);
     w.bytes = at;
     return w;
 }
@@ -436,7 +474,6 @@ extern "C" int plnlp_embedding_grad(const void* gy, int64_t ldg, int gy_dtype, c
     char* ws = (char*)workspace;
     uint32_t* keys[2] = {(uint32_t*)(ws + w.keys[0]), (uint32_t*)(ws + w.keys[1])};
     int32_t* pos[2] = {(int32_t*)(ws + w.pos[0]), (int32_t*)(ws + w.pos[1])};
-    float* partial = (float*)(ws + w.partial);
     int cur = 0, rc = 0;
     if (n_ids && n_ids <= SORT_SMALL) {
         rc = with_id(id_bytes, [&](auto it) {
@@ -451,24 +488,29 @@ extern "C" int plnlp_embedding_grad(const void* gy, int64_t ldg, int gy_dtype, c
         int bits = 1;
         while (((int64_t)1 << bits) <= n_rows) ++bits;               // keys are 0 .. n_rows
         const int passes = (bits + SORT_BITS - 1) / SORT_BITS, digit = (bits + passes - 1) / passes;
-        const int tiles = (int)((n_ids + SORT_TILE - 1) / SORT_TILE), bins = 1 << digit;
+        const int rounds = sort_rounds(n_ids), tile = rounds * LOOKUP_THREADS, bins = 1 << digit;
+        const int tiles = (int)((n_ids + tile - 1) / tile);
         uint32_t* hist = (uint32_t*)(ws + w.hist);
         uint32_t* total = (uint32_t*)(ws + w.total);
         for (int p = 0; p < passes && !rc; ++p) {
             const int shift = p * digit;
             rc = with_id(id_bytes, [&](auto it) {
                 using I = decltype(it);
-                auto pass = [&](auto first) {
+                auto pass = [&](auto first, auto count) {
                     constexpr bool F = decltype(first)::value;
-                    hipLaunchKernelGGL((sort_count_kernel<I, F>), dim3(tiles), dim3(LOOKUP_THREADS), 4 * bins, s, (const I*)ids, keys[cur],
-                                       n_ids, n_rows, padding_id, shift, bins, tiles, hist);
-                    hipLaunchKernelGGL(sort_offsets_kernel, dim3(bins), dim3(LOOKUP_THREADS), 0, s, hist, tiles, total);
-                    hipLaunchKernelGGL((sort_scatter_kernel<I, F>), dim3(tiles), dim3(LOOKUP_THREADS), 4 * bins * (LOOKUP_THREADS / 64), s,
-                                       (const I*)ids, keys[cur], pos[cur], n_ids, n_rows, padding_id, shift, digit, tiles, hist, total,
+                    constexpr int R = decltype(count)::value;
+                    hipLaunchKernelGGL((sort_count_kernel<I, F, R>), dim3(tiles), dim3(LOOKUP_THREADS), 4 * bins, s, (const I*)ids, keys[cur],
+                                       n_ids, n_rows, padding_id, shift, bins, hist);
+                    hipLaunchKernelGGL(sort_offsets_kernel, dim3((bins + 63) / 64), dim3(1024), 0, s, hist, tiles, bins, total);
+                    hipLaunchKernelGGL((sort_scatter_kernel<I, F, R>), dim3(tiles), dim3(LOOKUP_THREADS), 4 * bins * (LOOKUP_THREADS / 64), s,
+                                       (const I*)ids, keys[cur], pos[cur], n_ids, n_rows, padding_id, shift, digit, hist, total,
                                        keys[cur ^ 1], pos[cur ^ 1]);
                     return launch_status();
                 };
-                return p == 0 ? pass(std::true_type{}) : pass(std::false_type{});
+                auto sized = [&](auto first) {
+                    return rounds == 4 ? pass(first, std::integral_constant<int, 4>{}) : pass(first, std::integral_constant<int, 16>{});
+                };
+                return p == 0 ? sized(std::true_type{}) : sized(std::false_type{});
             });
             cur ^= 1;
         }
@@ -481,13 +523,18 @@ extern "C" int plnlp_embedding_grad(const void* gy, int64_t ldg, int gy_dtype, c
     return with_dtype(gy_dtype, [&](auto gt) { return with_dtype(grad_dtype, [&](auto et) { return with_pack(v, [&](auto vc) {
         using G = decltype(gt); using E = decltype(et);
         constexpr int V = decltype(vc)::value;
-        if (n_ids > 2 * SEG) {
-            hipLaunchKernelGGL((grad_pieces_kernel<G, V>), dim3((unsigned)(n_ids / SEG)), dim3(LOOKUP_THREADS), 0, s, (const G*)gy, ldg,
-                               keys[cur], pos[cur], n_rows, (int)packs, tx, partial);
-            if (int e = launch_status()) return e;
+        const int slabs = (int)((packs + tx - 1) / tx), range = grad_range(n_ids, width), ty = LOOKUP_THREADS / tx;
+        const int64_t ranges = (n_ids + range - 1) / range, run_blocks = (ranges * slabs + ty - 1) / ty;
+        const GradArgs<G, E, V> a{(const G*)gy, ldg, keys[cur], pos[cur], n_ids, n_rows, (int)packs, tx, slabs, range, ranges, run_blocks,
+                                  (float*)(ws + w.head), (float*)(ws + w.tail), scale, (E*)grad, lde};
+        const int64_t clear_blocks = (n_rows + CLEAR_ROWS - 1) / CLEAR_ROWS;
+        if (run_blocks + clear_blocks >= ((int64_t)1 << 31)) return PLNLP_E_SHAPE;
+        hipLaunchKernelGGL((grad_runs_kernel<G, E, V>), dim3((unsigned)(run_blocks + clear_blocks)), dim3(LOOKUP_THREADS), 0, s, a);
+        if (int e = launch_status()) return e;
+        if (ranges > 1) {
+            hipLaunchKernelGGL((grad_joins_kernel<G, E, V>), dim3((unsigned)(ranges - 1), slabs), dim3(LOOKUP_THREADS), 0, s, a);
+            return launch_status();
         }
-        hipLaunchKernelGGL((grad_rows_kernel<G, E, V>), dim3((unsigned)((n_rows + GRAD_ROWS - 1) / GRAD_ROWS)), dim3(LOOKUP_THREADS), 0, s,
-                           (const G*)gy, ldg, keys[cur], pos[cur], n_ids, n_rows, (int)packs, tx, partial, scale, (E*)grad, lde);
-        return launch_status();
+        return 0;
     }); }); });
 }

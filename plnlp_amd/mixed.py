@@ -114,18 +114,19 @@ def embedding_lookup(table: torch.Tensor, ids: torch.Tensor, *, scale: float = 1
 
 # ------------------------------------------------------------------ linear ------
 def _linear_forward(x, weight, bias, residual, act: int, keep: bool):
-    """(y [m, n], z or None) of matrices as _rows gives them; z = x W^T + bias is kept where the backward pass will read it"""
+    """(y [m, n], slope or None) of matrices as _rows gives them; the activation's derivative is kept where the backward pass will
+    read it: int16 [m, n] in steps of 2^-14"""
     lib = L.load()
     m, k = x.shape
     n = weight.shape[0]
     out = torch.empty(m, n, dtype=x.dtype, device=x.device)
-    pre = torch.empty(m, n, dtype=x.dtype, device=x.device) if keep else None
+    slope = torch.empty(m, n, dtype=torch.int16, device=x.device) if keep else None
     n_bytes = lib.plnlp_linear_act_workspace_bytes(m, n, k)
     ws = _workspace(n_bytes, x.device)
     L.check(lib.plnlp_linear_act(x.data_ptr(), _ld(x), weight.data_ptr(), _ld(weight), L.ptr(bias), L.ptr(residual),
-                                 0 if residual is None else _ld(residual), act, m, n, k, L.ptr(pre), n, out.data_ptr(), n,
+                                 0 if residual is None else _ld(residual), act, m, n, k, L.ptr(slope), n, out.data_ptr(), n,
                                  L.DTYPE_CODES[x.dtype], L.ptr(ws), n_bytes, L.stream_ptr()), "plnlp_linear_act")
-    return out, pre
+    return out, slope
 
 
 class LinearActFn(torch.autograd.Function):
@@ -133,16 +134,16 @@ class LinearActFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, weight, bias, residual, act: int):
-        y, pre = _linear_forward(x, weight, bias, residual, act, act != L.ACTIVATIONS["none"])
+        y, slope = _linear_forward(x, weight, bias, residual, act, act != L.ACTIVATIONS["none"])
         ctx.act = act
-        ctx.save_for_backward(x, weight, pre)
+        ctx.save_for_backward(x, weight, slope)
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, gy):
         lib = L.load()
-        x, weight, pre = ctx.saved_tensors
+        x, weight, slope = ctx.saved_tensors
         need = ctx.needs_input_grad
         m, k = x.shape
         n = weight.shape[0]
@@ -154,7 +155,7 @@ class LinearActFn(torch.autograd.Function):
             L.require_device(g, x, weight)
             n_bytes = lib.plnlp_linear_act_backward_workspace_bytes(m, n, k, ctx.act)
             ws = _workspace(n_bytes, x.device)
-            L.check(lib.plnlp_linear_act_backward(g.data_ptr(), _ld(g), L.ptr(pre), n, ctx.act, x.data_ptr(), _ld(x), weight.data_ptr(),
+            L.check(lib.plnlp_linear_act_backward(g.data_ptr(), _ld(g), L.ptr(slope), n, ctx.act, x.data_ptr(), _ld(x), weight.data_ptr(),
                                                   _ld(weight), m, n, k, L.ptr(dx), k, L.ptr(dw), k, L.ptr(db), L.DTYPE_CODES[x.dtype],
                                                   L.ptr(ws), n_bytes, L.stream_ptr()), "plnlp_linear_act_backward")
         return dx, dw, db, gy if need[3] else None, None
@@ -166,8 +167,8 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tenso
 
     x: [..., K]; weight: [N, K] (torch.nn.Linear's layout); bias: [N]; residual: the result's shape [..., N]; all bf16 or all
     fp16.  activation: "none", "relu", "gelu" (z Phi(z)), "gelu_tanh" or "silu".  The product is summed in fp32; bias,
-    activation and residual act on the fp32 sums, which are rounded once.  The backward pass takes the activation's
-    derivative at x W^T + bias rounded to 16 bits (kept by the forward pass where a gradient is wanted).
+    activation and residual act on the fp32 sums, which are rounded once.  The activation's derivative is kept
+    for the backward pass in steps of 2^-14, where a gradient is wanted.
     fp32 matrices are the business of ops.LinearFn."""
     if x.dtype not in _HALF:
         raise TypeError(f"linear_act: x must be bf16 or fp16, not {x.dtype} (ops.LinearFn is the fp32 layer)")

@@ -181,6 +181,7 @@ def act_ref(z, name):
 # |z|^2 / 2 (|z| <= 12 here: 72 * 2^-24 * log2 e) and the reciprocals are good to an ulp: 2e-5 of max(|z|, 1) covers all of them
 ACT_ERR = 2e-5
 SLOPE_LIP = 1.0        # |act''| is at most 0.8 (gelu, gelu_tanh), 0.5 (silu)
+SLOPE_ROUND = 2.0 ** -15       # the slope is kept in steps of 2^-14
 
 
 def linear_case(P, m, n, k, dtype, act, bias, residual, pad=0, seed=0):
@@ -215,8 +216,8 @@ def check_linear(P, x, w, b, r, gy, act, dtype):
     dz = g * slope
     e_dz = torch.zeros_like(dz)
     if act != "none":
-        # the slope is taken at z rounded to the type, dz is rounded to the type
-        e_dz = g.abs() * (SLOPE_LIP * (z.abs() * u + tiny + e_z) + err * z.abs().clamp_min(1)) + dz.abs() * (u + 2 * ADD) + tiny
+        # the slope is taken at z as summed and kept in steps, dz is rounded to the type
+        e_dz = g.abs() * (SLOPE_LIP * e_z + SLOPE_ROUND + err * z.abs().clamp_min(1)) + dz.abs() * (u + 2 * ADD) + tiny
         if act == "relu":
             e_dz = torch.zeros_like(dz)                       # (exact: the inputs are small whole numbers there)
     dx, dw = dz @ wd, dz.t() @ xd
@@ -286,7 +287,7 @@ def test_linear_large_tiles(P, m, n, k, dtype):
     within(y.detach()[rows], y_ref[rows], (1.13 * e_z + ACT_ERR * z.abs().clamp_min(1) + y_ref.abs() * (u + 2 * ADD) + a.abs() * ADD + tiny)[rows])
     gd = gy.double()
     dz = gd * slope
-    e_dz = gd.abs() * (SLOPE_LIP * (z.abs() * u + tiny + e_z) + ACT_ERR * z.abs().clamp_min(1)) + dz.abs() * (u + 2 * ADD) + tiny
+    e_dz = gd.abs() * (SLOPE_LIP * e_z + SLOPE_ROUND + ACT_ERR * z.abs().clamp_min(1)) + dz.abs() * (u + 2 * ADD) + tiny
     ref = dz[rows] @ wd
     within(dx[rows], ref, e_dz[rows] @ wd.abs() + (dz[rows].abs() @ wd.abs()) * (n + 2) * ADD * 1.1 + ref.abs() * u + tiny)
     ref = dz.t() @ xd
