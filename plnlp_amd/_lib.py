@@ -192,9 +192,9 @@ SIGNATURES = {
     "plnlp_linear_act_backward": (C.c_int, [C.c_void_p, c_i64, C.c_void_p, c_i64, C.c_int, C.c_void_p, c_i64, C.c_void_p, c_i64,
                                             c_i64, c_i64, c_i64, C.c_void_p, c_i64, C.c_void_p, c_i64, C.c_void_p, C.c_int,
                                             C.c_void_p, c_i64, C.c_void_p]),
-    "plnlp_grad_norm_workspace_doubles": (c_i64, [C.POINTER(GradTensor), C.c_int]),
-    "plnlp_grad_norm": (C.c_int, [C.POINTER(GradTensor), C.c_int, C.c_int, C.c_void_p, c_i64, C.c_void_p, C.c_void_p]),
-    "plnlp_grad_clip": (C.c_int, [C.POINTER(GradTensor), C.c_int, C.c_int, C.c_double, C.c_void_p, c_i64, C.c_void_p,
+    "plnlp_grad_norm_workspace_doubles": (c_i64, [C.c_void_p, C.c_int]),
+    "plnlp_grad_norm": (C.c_int, [C.c_void_p, C.c_int, C.c_int, C.c_void_p, c_i64, C.c_void_p, C.c_void_p]),
+    "plnlp_grad_clip": (C.c_int, [C.c_void_p, C.c_int, C.c_int, C.c_double, C.c_void_p, c_i64, C.c_void_p,
                                   C.c_void_p]),
 }
 

@@ -127,20 +127,19 @@ template <typename S, typename D> __device__ void clip_chunk(const S* src, D* ds
     for (int64_t i = tid; i < head; i += CLIP_THREADS) dst[i] = (D)((float)src[i] * c);
     src += head; dst += head; n -= head;
     const int64_t nv = n / V;
-    // backwards: what the norm's pass read last is what the Infinity Cache still holds
-    int64_t i = nv - 1 - tid;
-    for (; i - 3 * CLIP_THREADS >= 0; i -= 4 * CLIP_THREADS) {
+    int64_t i = tid;
+    for (; i + 3 * CLIP_THREADS < nv; i += 4 * CLIP_THREADS) {
         float x[4][V];
 #pragma unroll
-        for (int u = 0; u < 4; ++u) load_f32<S, V>(src + (i - u * CLIP_THREADS) * V, x[u]);
+        for (int u = 0; u < 4; ++u) load_f32<S, V>(src + (i + u * CLIP_THREADS) * V, x[u]);
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
 #pragma unroll
             for (int j = 0; j < V; ++j) x[u][j] *= c;
-            store_f32<D, V>(dst + (i - u * CLIP_THREADS) * V, x[u]);
+            store_f32<D, V>(dst + (i + u * CLIP_THREADS) * V, x[u]);
         }
     }
-    for (; i >= 0; i -= CLIP_THREADS) {
+    for (; i < nv; i += CLIP_THREADS) {
         float x[V];
         load_f32<S, V>(src + i * V, x);
 #pragma unroll

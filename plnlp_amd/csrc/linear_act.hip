@@ -34,23 +34,22 @@ template <> struct Mfma<_Float16> {
 };
 
 // ---- activations ------------------------------------------------------------------------------------------
-__device__ __forceinline__ float sigmoid_f(float z) { return __builtin_amdgcn_rcpf(1.f + __expf(-z)); }
+// (these run on every element of a result whose product may take less time than they do: an instruction counts)
+__device__ __forceinline__ float exp2_f(float x) { return __builtin_amdgcn_exp2f(x); }
+constexpr float LOG2E = 1.4426950408889634f;
+__device__ __forceinline__ float sigmoid_f(float z) { return __builtin_amdgcn_rcpf(1.f + exp2_f(-LOG2E * z)); }
 
-// the normal distribution function: Phi(-|z|) = exp(-z^2/2) * P(t) / 2 with t = 1 / (1 + 0.39 |z| / sqrt 2) and P a polynomial fitted
-// to exp(u^2) erfc(u) on [0, 30] in RELATIVE error (2.4e-6; 4e-6 evaluated in f32), so the far negative tail keeps its digits
-__device__ __forceinline__ float gauss_half(float z) {          // exp(-z^2/2)
-    return __expf(-0.5f * z * z);
-}
+// the normal distribution function, g = exp(-z^2/2):  Phi(-|z|) = g * P(t), t = 1 / (1 + 0.45 |z| / sqrt 2), P a polynomial fitted to
+// exp(u^2) erfc(u) / 2 on [0, 30] in RELATIVE error (1.2e-5, a fortieth of half an fp16 step), so the far negative tail keeps its digits
 __device__ __forceinline__ float normal_cdf(float z, float g) {
-    const float t = __builtin_amdgcn_rcpf(fmaf(0.39f * 0.70710678f, fabsf(z), 1.f));
-    float p = -0.10887830704450607f;
-    p = fmaf(p, t, 0.25157830119132996f);
-    p = fmaf(p, t, 0.0152523098513484f);
-    p = fmaf(p, t, 0.20380336046218872f);
-    p = fmaf(p, t, 0.19776275753974915f);
-    p = fmaf(p, t, 0.2204565703868866f);
-    p = fmaf(p, t, 0.22002261877059937f);
-    const float q = 0.5f * p * t * g;
+    const float t = __builtin_amdgcn_rcpf(fmaf(0.45f * 0.70710678f, fabsf(z), 1.f));
+    float p = 0.5f * -0.13489297032356262f;
+    p = fmaf(p, t, 0.5f * 0.28983235359191895f);
+    p = fmaf(p, t, 0.5f * 0.09164738655090332f);
+    p = fmaf(p, t, 0.5f * 0.24759894609451294f);
+    p = fmaf(p, t, 0.5f * 0.2518513798713684f);
+    p = fmaf(p, t, 0.5f * 0.2539602816104889f);
+    const float q = p * t * g;
     return z > 0.f ? 1.f - q : q;
 }
 constexpr float TANH_C = 1.5957691216057308f;                   // 2 sqrt(2 / pi)
@@ -68,20 +67,26 @@ template <int ACT, bool SLOPE> __device__ __forceinline__ float act_of(float z, 
         return z * s;
     }
     if (ACT == PLNLP_ACT_GELU) {
-        const float g = gauss_half(z), c = normal_cdf(z, g);
+        const float g = exp2_f((-0.5f * LOG2E * z) * z), c = normal_cdf(z, g);
         if (SLOPE) slope = fmaf(z * 0.3989422804014327f, g, c);
         return z * c;
     }
     if (ACT == PLNLP_ACT_GELU_TANH) {
-        const float s = sigmoid_f(TANH_C * fmaf(TANH_A * z * z, z, z));
-        if (SLOPE) slope = fmaf(z * s * (1.f - s), TANH_C * fmaf(3.f * TANH_A * z, z, 1.f), s);
-        return z * s;
+        const float z2 = z * z, s = __builtin_amdgcn_rcpf(1.f + exp2_f(z * fmaf(-LOG2E * TANH_C * TANH_A, z2, -LOG2E * TANH_C)));
+        const float y = z * s;
+        // (z2 may be infinite where 1 - s is 0)
+        if (SLOPE) slope = fmaf(fmaf(-y, s, y), fmaf(3.f * TANH_C * TANH_A, fminf(z2, 1e30f), TANH_C), s);
+        return y;
     }
     return z;
 }
+// the slope in steps of 2^-14: adding 1.5 * 2^23 rounds to a whole number and leaves it in the low bits; a NaN becomes SLOPE_NAN, which
+// no slope reaches (the smaller of a NaN and a number is the number)
 constexpr float SLOPE_STEP = 1.f / 16384.f;
-constexpr int SLOPE_NAN = -32768;
-__device__ __forceinline__ int16_t pack_slope(float s) { return s == s ? (int16_t)__float2int_rn(s * 16384.f) : (int16_t)SLOPE_NAN; }
+constexpr int SLOPE_NAN = 20000;
+__device__ __forceinline__ int16_t pack_slope(float s) {
+    return (int16_t)__float_as_uint(fminf(fmaf(s, 16384.f, 12582912.f), 12582912.f + SLOPE_NAN));
+}
 __device__ __forceinline__ float unpack_slope(int16_t q) { return q == SLOPE_NAN ? __builtin_nanf("") : (float)q * SLOPE_STEP; }
 // f(std::integral_constant<int, ACT>{}) of a run-time activation
 template <typename F> __host__ __device__ __forceinline__ int with_act(int act, F&& f) {
@@ -218,35 +223,37 @@ template <int R, int THREADS> __device__ __forceinline__ void store_cols(const S
 }
 
 template <typename T, int BM, int BN, int WM, int WN, bool PT, bool QT, bool VEC, int ACT>
-__global__ __launch_bounds__(WM * WN * 64) void tile_kernel(TileArgs<T> a) {
+__global__ __launch_bounds__(WM * WN * 64, 2) void tile_kernel(TileArgs<T> a) {
     constexpr int THREADS = WM * WN * 64, TM = BM / WM / 16;         // 16-row pieces of a wave's part; it is 64 columns wide
     static_assert(BN / WN == 64, "a wave covers 64 columns");
     typedef typename Mfma<T>::frag frag;
     extern __shared__ __attribute__((aligned(16))) char lds[];       // two buffers of P rows, then Q rows
     constexpr int BUF = (BM + BN) * 128;
 
-    // Workgroups are dealt to the eight XCDs in turn: each XCD gets a contiguous run of tiles, so that its L2 holds the panels they share
+    // A workgroup takes tiles blockIdx.x, + gridDim.x, ... (a multiple of 8): the first loads of its next tile are under way while it
+    // finishes one.  Workgroups are dealt to the eight XCDs in turn: each XCD gets a contiguous run of tiles, so that its L2 holds the
+    // panels they share, and walks groups of 8 row panels column by column.
     const int tiles = a.tiles_m * a.tiles_n, total = tiles * a.slices;
-    const int per = total >> 3, extra = total & 7, xcd = blockIdx.x & 7, nth = blockIdx.x >> 3;
-    const int id = xcd * per + min(xcd, extra) + nth;
-    const int slice = id / tiles, tile = id % tiles;
-    // and walks groups of 8 row panels column by column
-    constexpr int GROUP = 8;
-    const int group = tile / (GROUP * a.tiles_n), in_group = tile % (GROUP * a.tiles_n);
-    const int g_rows = min(GROUP, a.tiles_m - group * GROUP);
-    const int64_t m0 = (int64_t)(group * GROUP + in_group % g_rows) * BM, n0 = (int64_t)(in_group / g_rows) * BN;
+    const int term_steps = (int)((a.k + BK - 1) / BK);
+    int64_t m0, n0;
+    int slice, first, steps;
+    auto locate = [&](int at) {
+        const int per = total >> 3, extra = total & 7, xcd = at & 7;
+        const int id = xcd * per + min(xcd, extra) + (at >> 3);
+        const int tile = id % tiles;
+        slice = id / tiles;
+        constexpr int GROUP = 8;
+        const int group = tile / (GROUP * a.tiles_n), in_group = tile % (GROUP * a.tiles_n);
+        const int g_rows = min(GROUP, a.tiles_m - group * GROUP);
+        m0 = (int64_t)(group * GROUP + in_group % g_rows) * BM;
+        n0 = (int64_t)(in_group / g_rows) * BN;
+        first = slice * a.steps;
+        steps = min(a.steps, term_steps * a.terms - first);
+    };
+    locate(blockIdx.x);
 
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
     const int wm = (wave / WN) * (BM / WM), wn = (wave % WN) * 64;
-    const int term_steps = (int)((a.k + BK - 1) / BK), first = slice * a.steps;
-    const int steps = min(a.steps, term_steps * a.terms - first);
-    const int rows_p = (int)min((int64_t)BM, a.m - m0), rows_q = (int)min((int64_t)BN, a.n - n0);
-
-    f32x4 acc[TM][4];
-#pragma unroll
-    for (int i = 0; i < TM; ++i)
-#pragma unroll
-        for (int t = 0; t < 4; ++t) acc[i][t] = f32x4{0.f, 0.f, 0.f, 0.f};
 
     Stage<BM, THREADS> sp;
     Stage<BN, THREADS> sq;
@@ -254,6 +261,7 @@ __global__ __launch_bounds__(WM * WN * 64) void tile_kernel(TileArgs<T> a) {
         const int at = first + step, term = at >= term_steps;
         const int64_t k = (int64_t)(at - (term ? term_steps : 0)) * BK, left = a.k - k;
         const T* p = a.p + (term ? a.plane : 0);
+        const int rows_p = (int)min((int64_t)BM, a.m - m0), rows_q = (int)min((int64_t)BN, a.n - n0);
         if (PT) fetch_cols<T, BM, THREADS, VEC>(sp, p + k * a.ldp + m0, a.ldp, rows_p, left);
         else fetch_rows<T, BM, THREADS, VEC>(sp, p + m0 * a.ldp + k, a.ldp, rows_p, left);
         if (QT) fetch_cols<T, BN, THREADS, VEC>(sq, a.q + k * a.ldq + n0, a.ldq, rows_q, left);
@@ -264,76 +272,90 @@ __global__ __launch_bounds__(WM * WN * 64) void tile_kernel(TileArgs<T> a) {
         if (PT) store_cols<BM, THREADS>(sp, b); else store_rows<BM, THREADS>(sp, b);
         if (QT) store_cols<BN, THREADS>(sq, b + BM * 128); else store_rows<BN, THREADS>(sq, b + BM * 128);
     };
-    if (steps > 0) {
-        fetch(0);
-        stage(0);
-        if (steps > 1) fetch(1);
-        __syncthreads();
-    }
-    for (int step = 0; step < steps; ++step) {
-        const char* b = lds + (step & 1) * BUF;
-        if (step + 1 < steps) stage((step + 1) & 1);      // the other buffer was read before the barrier that ended the last step
-        if (step + 2 < steps) fetch(step + 2);            // a whole step to arrive in
+    if (steps > 0) fetch(0);
+    for (int at = blockIdx.x;;) {
+        f32x4 acc[TM][4];
 #pragma unroll
-        for (int ks = 0; ks < BK / 32; ++ks) {
-            frag q[4];
+        for (int i = 0; i < TM; ++i)
 #pragma unroll
-            for (int t = 0; t < 4; ++t) {
-                const int row = wn + q_row(t, r);
-                q[t] = *reinterpret_cast<const frag*>(b + (BM + row) * 128 + (((ks * 4 + g) ^ swz(row)) << 4));
-            }
-#pragma unroll
-            for (int i = 0; i < TM; ++i) {
-                const int row = wm + i * 16 + r;
-                const frag p = *reinterpret_cast<const frag*>(b + row * 128 + (((ks * 4 + g) ^ swz(row)) << 4));
-#pragma unroll
-                for (int t = 0; t < 4; ++t) acc[i][t] = Mfma<T>::go(q[t], p, acc[i][t]);
-            }
+            for (int t = 0; t < 4; ++t) acc[i][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+        if (steps > 0) {
+            stage(0);
+            if (steps > 1) fetch(1);
+            __syncthreads();
         }
-        __syncthreads();
-    }
-
-    // lane (r, g) holds columns n + 32 h + 0..7 (h = 0, 1) of rows wm + 16 i + r
-    const int64_t n = n0 + wn + 8 * g;
-    int cols[2];
+        for (int step = 0; step < steps; ++step) {
+            const char* b = lds + (step & 1) * BUF;
+            if (step + 1 < steps) stage((step + 1) & 1);      // the other buffer was read before the barrier that ended the last step
+            if (step + 2 < steps) fetch(step + 2);            // a whole step to arrive in
 #pragma unroll
-    for (int h = 0; h < 2; ++h) cols[h] = (int)max(min((int64_t)8, a.n - n - 32 * h), (int64_t)0);
-    float bias[2][8];
+            for (int ks = 0; ks < BK / 32; ++ks) {
+                frag q[4];
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) bias[h][j] = (ACT != PARTIAL && a.fin.bias && j < cols[h]) ? (float)a.fin.bias[n + 32 * h + j] : 0.f;
-#pragma unroll
-    for (int i = 0; i < TM; ++i) {
-        const int64_t m = m0 + wm + i * 16 + r;
-        if (m >= a.m) continue;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int64_t col = n + 32 * h;
-            if (cols[h] <= 0) continue;
-            if constexpr (ACT == PARTIAL) {
-                float* o = a.partial + ((int64_t)slice * a.m + m) * a.n + col;
-#pragma unroll
-                for (int t = 0; t < 2; ++t) {
-                    if (VEC) *reinterpret_cast<f32x4*>(o + 4 * t) = acc[i][2 * h + t];      // (n is whole groups of eight)
-                    else
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) if (4 * t + j < cols[h]) o[4 * t + j] = acc[i][2 * h + t][j];
+                for (int t = 0; t < 4; ++t) {
+                    const int row = wn + q_row(t, r);
+                    q[t] = *reinterpret_cast<const frag*>(b + (BM + row) * 128 + (((ks * 4 + g) ^ swz(row)) << 4));
                 }
-            } else if constexpr (VEC) {
-                float v[8];
 #pragma unroll
-                for (int j = 0; j < 8; ++j) v[j] = acc[i][2 * h + (j >> 2)][j & 3];
-                finish_cols<ACT, T, 8>(a.fin, v, bias[h], m, col);
-            } else {
+                for (int i = 0; i < TM; ++i) {
+                    const int row = wm + i * 16 + r;
+                    const frag p = *reinterpret_cast<const frag*>(b + row * 128 + (((ks * 4 + g) ^ swz(row)) << 4));
 #pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    if (j < cols[h]) {
-                        float v[1] = {acc[i][2 * h + (j >> 2)][j & 3]}, b[1] = {bias[h][j]};
-                        finish_cols<ACT, T, 1>(a.fin, v, b, m, col + j);
+                    for (int t = 0; t < 4; ++t) acc[i][t] = Mfma<T>::go(q[t], p, acc[i][t]);
+                }
+            }
+            __syncthreads();
+        }
+
+        // lane (r, g) holds columns n + 32 h + 0..7 (h = 0, 1) of rows mr + 16 i
+        const int64_t n = n0 + wn + 8 * g, mr = m0 + wm + r;
+        const int part = slice;
+        at += gridDim.x;
+        if (at < total) {
+            locate(at);
+            if (steps > 0) fetch(0);
+        }
+        int cols[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) cols[h] = (int)max(min((int64_t)8, a.n - n - 32 * h), (int64_t)0);
+        float bias[2][8];
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) bias[h][j] = (ACT != PARTIAL && a.fin.bias && j < cols[h]) ? (float)a.fin.bias[n + 32 * h + j] : 0.f;
+#pragma unroll
+        for (int i = 0; i < TM; ++i) {
+            const int64_t m = mr + i * 16;
+            if (m >= a.m) continue;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int64_t col = n + 32 * h;
+                if (cols[h] <= 0) continue;
+                if constexpr (ACT == PARTIAL) {
+                    float* o = a.partial + ((int64_t)part * a.m + m) * a.n + col;
+#pragma unroll
+                    for (int t = 0; t < 2; ++t) {
+                        if (VEC) *reinterpret_cast<f32x4*>(o + 4 * t) = acc[i][2 * h + t];      // (n is whole groups of eight)
+                        else
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) if (4 * t + j < cols[h]) o[4 * t + j] = acc[i][2 * h + t][j];
                     }
+                } else if constexpr (VEC) {
+                    float v[8];
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) v[j] = acc[i][2 * h + (j >> 2)][j & 3];
+                    finish_cols<ACT, T, 8>(a.fin, v, bias[h], m, col);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        if (j < cols[h]) {
+                            float v[1] = {acc[i][2 * h + (j >> 2)][j & 3]}, b[1] = {bias[h][j]};
+                            finish_cols<ACT, T, 1>(a.fin, v, b, m, col + j);
+                        }
+                }
             }
         }
+        if (at >= total) return;
     }
 }
 
@@ -544,7 +566,9 @@ static int launch_tile(const TileArgs<T>& a, hipStream_t s) {
         const hipError_t e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
         if (e != hipSuccess) return (int)e;
     }
-    hipLaunchKernelGGL(kernel, dim3((unsigned)(a.tiles_m * a.tiles_n * a.slices)), dim3(WM * WN * 64), LDS, s, a);
+    const int per_cu = LDS > 81920 ? 1 : 2;               // workgroups whose LDS (and registers) a CU holds
+    const unsigned blocks = (unsigned)std::min(a.tiles_m * a.tiles_n * a.slices, 256 * per_cu);
+    hipLaunchKernelGGL(kernel, dim3(blocks), dim3(WM * WN * 64), LDS, s, a);
     return launch_status();
 }
 

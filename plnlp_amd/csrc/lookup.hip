@@ -67,7 +67,7 @@ template <typename I> __device__ __forceinline__ uint32_t sort_key(const I* ids,
 
 template <typename I, int N>
 __global__ __launch_bounds__(1024) void sort_small_kernel(const I* __restrict__ ids, int n, int64_t n_rows, int64_t padding,
-                                                          uint32_t* __restrict__ keys, int32_t* __restrict__ pos) {
+                                                          uint2* __restrict__ sorted) {
     __shared__ uint64_t k[N];
     for (int i = threadIdx.x; i < N; i += 1024)
         k[i] = i < n ? ((uint64_t)sort_key(ids, i, n_rows, padding) << 32) | (uint32_t)i : ~0ull;
@@ -81,16 +81,13 @@ __global__ __launch_bounds__(1024) void sort_small_kernel(const I* __restrict__ 
             }
             __syncthreads();
         }
-    for (int i = threadIdx.x; i < n; i += 1024) {
-        keys[i] = (uint32_t)(k[i] >> 32);
-        pos[i] = (int32_t)(uint32_t)k[i];
-    }
+    for (int i = threadIdx.x; i < n; i += 1024) sorted[i] = make_uint2((uint32_t)(k[i] >> 32), (uint32_t)k[i]);
 }
 
 // One counting pass sorts by the digit (key >> shift) & (bins - 1).  A tile is 256 * ROUNDS ids; hist[tile][digit].
 // FIRST: the keys come from the ids, the positions are 0 .. n-1.
 template <typename I, bool FIRST, int ROUNDS>
-__global__ __launch_bounds__(LOOKUP_THREADS) void sort_count_kernel(const I* __restrict__ ids, const uint32_t* __restrict__ keys, int64_t n,
+__global__ __launch_bounds__(LOOKUP_THREADS) void sort_count_kernel(const I* __restrict__ ids, const uint2* __restrict__ in, int64_t n,
                                                                     int64_t n_rows, int64_t padding, int shift, int bins,
                                                                     uint32_t* __restrict__ hist) {
     extern __shared__ uint32_t cnt[];
@@ -99,7 +96,7 @@ __global__ __launch_bounds__(LOOKUP_THREADS) void sort_count_kernel(const I* __r
 #pragma unroll
     for (int u = 0; u < ROUNDS; ++u) {
         const int64_t i = lo + u * LOOKUP_THREADS;
-        key[u] = i >= n ? 0 : FIRST ? sort_key(ids, i, n_rows, padding) : keys[i];
+        key[u] = i >= n ? 0 : FIRST ? sort_key(ids, i, n_rows, padding) : in[i].x;
     }
     for (int d = threadIdx.x; d < bins; d += LOOKUP_THREADS) cnt[d] = 0;
     __syncthreads();
@@ -143,42 +140,37 @@ __device__ __forceinline__ uint32_t wave_scan(uint32_t v) {     // inclusive
 }
 
 template <typename I, bool FIRST, int ROUNDS>
-__global__ __launch_bounds__(LOOKUP_THREADS) void sort_scatter_kernel(const I* __restrict__ ids, const uint32_t* __restrict__ keys,
-                                                                      const int32_t* __restrict__ pos, int64_t n, int64_t n_rows,
-                                                                      int64_t padding, int shift, int bits,
+__global__ __launch_bounds__(LOOKUP_THREADS) void sort_scatter_kernel(const I* __restrict__ ids, const uint2* __restrict__ in, int64_t n,
+                                                                      int64_t n_rows, int64_t padding, int shift, int bits,
                                                                       const uint32_t* __restrict__ hist, const uint32_t* __restrict__ total,
-                                                                      uint32_t* __restrict__ keys_out, int32_t* __restrict__ pos_out) {
+                                                                      uint2* __restrict__ out) {
     constexpr int WAVES = LOOKUP_THREADS / 64;
     extern __shared__ uint32_t lds[];                  // cnt[WAVES][bins]
     __shared__ uint32_t part[WAVES];
     const int bins = 1 << bits, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     // ranks within the wave's own run of 64 * ROUNDS ids, in order: lanes of the same digit find each other by one ballot a bit
-    uint32_t key[ROUNDS], rank[ROUNDS];
-    int32_t p[ROUNDS];
+    uint2 pair[ROUNDS];
+    uint32_t rank[ROUNDS];
     uint32_t* cnt = lds + wave * bins;
     const int64_t lo = ((int64_t)blockIdx.x * WAVES + wave) * 64 * ROUNDS + lane;
 #pragma unroll
     for (int u = 0; u < ROUNDS; ++u) {
         const int64_t i = lo + u * 64;
-        key[u] = 0; p[u] = 0;
-        if (i < n) {
-            key[u] = FIRST ? sort_key(ids, i, n_rows, padding) : keys[i];
-            p[u] = FIRST ? (int32_t)i : pos[i];
-        }
+        pair[u] = i >= n ? make_uint2(0, 0) : FIRST ? make_uint2(sort_key(ids, i, n_rows, padding), (uint32_t)i) : in[i];
     }
     for (int d = threadIdx.x; d < WAVES * bins; d += LOOKUP_THREADS) lds[d] = 0;
     __syncthreads();
 #pragma unroll
     for (int u = 0; u < ROUNDS; ++u) {
-        const bool in = lo + u * 64 < n;
-        const uint32_t d = (key[u] >> shift) & (bins - 1);
-        uint64_t same = __ballot(in);
+        const bool real = lo + u * 64 < n;
+        const uint32_t d = (pair[u].x >> shift) & (bins - 1);
+        uint64_t same = __ballot(real);
         for (int b = 0; b < bits; ++b) {
             const uint64_t m = __ballot((d >> b) & 1);
             same &= ((d >> b) & 1) ? m : ~m;
         }
         rank[u] = 0;
-        if (in) {
+        if (real) {
             const int leader = __ffsll((unsigned long long)same) - 1;
             uint32_t before = 0;
             if (lane == leader) before = atomicAdd(&cnt[d], (uint32_t)__popcll(same));
@@ -212,28 +204,25 @@ __global__ __launch_bounds__(LOOKUP_THREADS) void sort_scatter_kernel(const I* _
 #pragma unroll
     for (int u = 0; u < ROUNDS; ++u) {
         if (lo + u * 64 >= n) continue;
-        const uint32_t at = cnt[(key[u] >> shift) & (bins - 1)] + rank[u];
-        keys_out[at] = key[u];
-        pos_out[at] = p[u];
+        out[cnt[(pair[u].x >> shift) & (bins - 1)] + rank[u]] = pair[u];
     }
 }
 
 // ---- gradient -----------------------------------------------------------------------------------------
 constexpr int CLEAR_ROWS = LOOKUP_THREADS;      // rows of dE a clearing workgroup looks up, one a thread
 
-// [b, e) of sorted positions: the first position whose key is >= want
-__device__ __forceinline__ int64_t lower_bound(const uint32_t* __restrict__ keys, int64_t n, uint32_t want) {
-    int64_t lo = 0, hi = n;
+// the first sorted position in [lo, hi) whose key is >= want, hi if there is none
+__device__ __forceinline__ int64_t lower_bound(const uint2* __restrict__ sorted, int64_t lo, int64_t hi, uint32_t want) {
     while (lo < hi) {
         const int64_t mid = (lo + hi) >> 1;
-        if (keys[mid] < want) lo = mid + 1; else hi = mid;
+        if (sorted[mid].x < want) lo = mid + 1; else hi = mid;
     }
     return lo;
 }
 
 template <typename G, typename E, int V> struct GradArgs {
     const G* gy; int64_t ldg;
-    const uint32_t* keys; const int32_t* pos;
+    const uint2* sorted;              // (key, position), by key and then by position
     int64_t n, n_rows;
     int packs, tx, slabs;             // a row is `packs` packs of V; a group of tx lanes takes one slab of tx packs
     int range;                        // sorted positions per group
@@ -250,8 +239,8 @@ template <typename G, typename E, int V> __global__ __launch_bounds__(LOOKUP_THR
         const int64_t row0 = ((int64_t)blockIdx.x - a.run_blocks) * CLEAR_ROWS, row = row0 + threadIdx.x;
         bool empty = row < a.n_rows;
         if (empty && a.n > 0) {
-            const int64_t at = lower_bound(a.keys, a.n, (uint32_t)row);
-            empty = at == a.n || a.keys[at] != (uint32_t)row;
+            const int64_t at = lower_bound(a.sorted, 0, a.n, (uint32_t)row);
+            empty = at == a.n || a.sorted[at].x != (uint32_t)row;
         }
         none[threadIdx.x] = empty;
         __syncthreads();
@@ -266,8 +255,8 @@ template <typename G, typename E, int V> __global__ __launch_bounds__(LOOKUP_THR
     if (range >= a.n_ranges || c >= a.packs) return;
     const int64_t b = range * a.range, e = min(b + a.range, a.n), col = (int64_t)c * V;
     const uint32_t end = (uint32_t)a.n_rows;
-    uint32_t cur = a.keys[b];
-    bool entered = b > 0 && a.keys[b - 1] == cur;          // the current run began in an earlier range
+    uint32_t cur = a.sorted[b].x;
+    bool entered = b > 0 && a.sorted[b - 1].x == cur;          // the current run began in an earlier range
     float s[V] = {};
     auto put = [&](bool leaves) {
         if (cur >= end) return;
@@ -282,25 +271,20 @@ template <typename G, typename E, int V> __global__ __launch_bounds__(LOOKUP_THR
         }
     };
     constexpr int U = 8;
-    uint32_t k[U];
-    int32_t p[U];
+    uint2 next[U];
     auto ask = [&](int64_t i) {
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int64_t at = min(i + u, e - 1);
-            k[u] = a.keys[at];
-            p[u] = a.pos[at];
-        }
+        for (int u = 0; u < U; ++u) next[u] = a.sorted[min(i + u, e - 1)];
     };
     ask(b);
     for (int64_t i = b; i < e; i += U) {
-        if (k[0] >= end) { if (cur < end) put(false); cur = end; break; }      // only ids without a gradient follow
+        if (next[0].x >= end) { if (cur < end) put(false); cur = end; break; }      // only ids without a gradient follow
         Pack<G, V> row[U];
         uint32_t key[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            key[u] = k[u];
-            row[u] = *reinterpret_cast<const Pack<G, V>*>(a.gy + (int64_t)p[u] * a.ldg + col);
+            key[u] = next[u].x;
+            row[u] = *reinterpret_cast<const Pack<G, V>*>(a.gy + (int64_t)next[u].y * a.ldg + col);
         }
         if (i + U < e) ask(i + U);
 #pragma unroll
@@ -317,7 +301,7 @@ template <typename G, typename E, int V> __global__ __launch_bounds__(LOOKUP_THR
             for (int j = 0; j < V; ++j) s[j] += (float)row[u].v[j];
         }
     }
-    put(e < a.n && a.keys[e] == cur);
+    put(e < a.n && a.sorted[e].x == cur);
 }
 
 // the range in which a run begins that leaves it: its tail + the heads of the ranges the run enters, in order of the groups of lanes
@@ -325,9 +309,12 @@ template <typename G, typename E, int V> __global__ __launch_bounds__(LOOKUP_THR
 template <typename G, typename E, int V> __global__ __launch_bounds__(LOOKUP_THREADS) void grad_joins_kernel(GradArgs<G, E, V> a) {
     __shared__ float lds[LOOKUP_THREADS * V];
     const int64_t range = blockIdx.x, b = range * a.range, e = b + a.range;      // (not the last range: e < n)
-    const uint32_t key = a.keys[e - 1];
-    if (key >= (uint32_t)a.n_rows || a.keys[e] != key || (b > 0 && a.keys[b - 1] == key)) return;
-    const int64_t last = (lower_bound(a.keys, a.n, key + 1) - 1) / a.range;
+    const uint32_t key = a.sorted[e - 1].x;
+    if (key >= (uint32_t)a.n_rows || a.sorted[e].x != key || (b > 0 && a.sorted[b - 1].x == key)) return;
+    // the range the run ends in: mostly the next one
+    const int64_t next_end = min(e + a.range, a.n);
+    const int64_t last = (next_end == a.n || a.sorted[next_end].x != key) ? range + 1
+                                                                           : (lower_bound(a.sorted, next_end, a.n, key + 1) - 1) / a.range;
     const int x = threadIdx.x & (a.tx - 1), y = threadIdx.x / a.tx, ty = LOOKUP_THREADS / a.tx;
     const int c = blockIdx.y * a.tx + x;
     const int64_t width = (int64_t)a.packs * V, col = (int64_t)c * V;
@@ -409,13 +396,13 @@ static int grad_range(int64_t n, int64_t width) {
     return r;
 }
 
-struct GradWorkspace { int64_t keys[2], pos[2], hist, total, head, tail, bytes; };
+struct GradWorkspace { int64_t sorted[2], hist, total, head, tail, bytes; };
 static GradWorkspace grad_workspace(int64_t n, int64_t width) {
     GradWorkspace w{};
     int64_t at = 0;
     auto take = [&](int64_t bytes) { const int64_t a = at; at += (bytes + 255) / 256 * 256; return a; };
     const bool small = n <= SORT_SMALL;
-    for (int i = 0; i < (small ? 1 : 2); ++i) { w.keys[i] = take(4 * n); w.pos[i] = take(4 * n); }
+    for (int i = 0; i < (small ? 1 : 2); ++i) w.sorted[i] = take(8 * n);
     const int64_t tile = sort_rounds(n) * LOOKUP_THREADS, tiles = (n + tile - 1) / tile;
     w.hist = take(small ? 0 : 4 * tiles << SORT_BITS);
     w.total = take(small ? 0 : 4 << SORT_BITS);
@@ -472,14 +459,13 @@ extern "C" int plnlp_embedding_grad(const void* gy, int64_t ldg, int gy_dtype, c
     if ((uintptr_t)workspace % 16) return PLNLP_E_ALIGN;
     hipStream_t s = (hipStream_t)stream;
     char* ws = (char*)workspace;
-    uint32_t* keys[2] = {(uint32_t*)(ws + w.keys[0]), (uint32_t*)(ws + w.keys[1])};
-    int32_t* pos[2] = {(int32_t*)(ws + w.pos[0]), (int32_t*)(ws + w.pos[1])};
+    uint2* sorted[2] = {(uint2*)(ws + w.sorted[0]), (uint2*)(ws + w.sorted[1])};
     int cur = 0, rc = 0;
     if (n_ids && n_ids <= SORT_SMALL) {
         rc = with_id(id_bytes, [&](auto it) {
             using I = decltype(it);
             auto run = [&](auto kernel) {
-                hipLaunchKernelGGL(kernel, dim3(1), dim3(1024), 0, s, (const I*)ids, (int)n_ids, n_rows, padding_id, keys[0], pos[0]);
+                hipLaunchKernelGGL(kernel, dim3(1), dim3(1024), 0, s, (const I*)ids, (int)n_ids, n_rows, padding_id, sorted[0]);
                 return launch_status();
             };
             return n_ids <= 256 ? run(sort_small_kernel<I, 256>) : n_ids <= 1024 ? run(sort_small_kernel<I, 1024>) : run(sort_small_kernel<I, SORT_SMALL>);
@@ -499,12 +485,11 @@ extern "C" int plnlp_embedding_grad(const void* gy, int64_t ldg, int gy_dtype, c
                 auto pass = [&](auto first, auto count) {
                     constexpr bool F = decltype(first)::value;
                     constexpr int R = decltype(count)::value;
-                    hipLaunchKernelGGL((sort_count_kernel<I, F, R>), dim3(tiles), dim3(LOOKUP_THREADS), 4 * bins, s, (const I*)ids, keys[cur],
-                                       n_ids, n_rows, padding_id, shift, bins, hist);
+                    hipLaunchKernelGGL((sort_count_kernel<I, F, R>), dim3(tiles), dim3(LOOKUP_THREADS), 4 * bins, s, (const I*)ids,
+                                       sorted[cur], n_ids, n_rows, padding_id, shift, bins, hist);
                     hipLaunchKernelGGL(sort_offsets_kernel, dim3((bins + 63) / 64), dim3(1024), 0, s, hist, tiles, bins, total);
                     hipLaunchKernelGGL((sort_scatter_kernel<I, F, R>), dim3(tiles), dim3(LOOKUP_THREADS), 4 * bins * (LOOKUP_THREADS / 64), s,
-                                       (const I*)ids, keys[cur], pos[cur], n_ids, n_rows, padding_id, shift, digit, hist, total,
-                                       keys[cur ^ 1], pos[cur ^ 1]);
+                                       (const I*)ids, sorted[cur], n_ids, n_rows, padding_id, shift, digit, hist, total, sorted[cur ^ 1]);
                     return launch_status();
                 };
                 auto sized = [&](auto first) {
@@ -525,7 +510,7 @@ extern "C" int plnlp_embedding_grad(const void* gy, int64_t ldg, int gy_dtype, c
         constexpr int V = decltype(vc)::value;
         const int slabs = (int)((packs + tx - 1) / tx), range = grad_range(n_ids, width), ty = LOOKUP_THREADS / tx;
         const int64_t ranges = (n_ids + range - 1) / range, run_blocks = (ranges * slabs + ty - 1) / ty;
-        const GradArgs<G, E, V> a{(const G*)gy, ldg, keys[cur], pos[cur], n_ids, n_rows, (int)packs, tx, slabs, range, ranges, run_blocks,
+        const GradArgs<G, E, V> a{(const G*)gy, ldg, sorted[cur], n_ids, n_rows, (int)packs, tx, slabs, range, ranges, run_blocks,
                                   (float*)(ws + w.head), (float*)(ws + w.tail), scale, (E*)grad, lde};
         const int64_t clear_blocks = (n_rows + CLEAR_ROWS - 1) / CLEAR_ROWS;
         if (run_blocks + clear_blocks >= ((int64_t)1 << 31)) return PLNLP_E_SHAPE;

@@ -11,7 +11,6 @@ stream of the current device, on which every tensor has to be; nothing waits for
 Like the rest of the package there is no CPU path."""
 from __future__ import annotations
 
-import ctypes as C
 import math
 from typing import List, Optional, Sequence
 
@@ -24,18 +23,33 @@ from . import _lib as L
 _HALF = (torch.bfloat16, torch.float16)
 
 
+def _stream(*tensors: Optional[torch.Tensor]) -> int:
+    """the current stream, once every tensor is known to be on its device (L.require_device says what is wrong if one is not)"""
+    device = tensors[0].get_device()
+    if device < 0 or device != torch.cuda.current_device():
+        L.require_device(*tensors)
+    for t in tensors:
+        if t is not None and t.get_device() != device:
+            L.require_device(*tensors)
+    return L.stream_ptr()
+
+
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """a matrix with consecutive elements along its rows and rows that do not overlap: t itself, or a contiguous copy"""
-    if t.shape[0] == 0 or t.shape[1] == 0:
+    if t.is_contiguous():
         return t
-    if (t.shape[1] > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
+    rows, cols = t.shape
+    if rows == 0 or cols == 0:
+        return t
+    if (cols > 1 and t.stride(1) != 1) or (rows > 1 and t.stride(0) < cols):
         return t.contiguous()
     return t
 
 
 def _ld(t: torch.Tensor) -> int:
     """elements between the rows of a matrix as _rows gives it (a single row: any; then its width)"""
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+    rows, cols = t.shape
+    return t.stride(0) if rows > 1 else cols
 
 
 def _workspace(n_bytes: int, device) -> Optional[torch.Tensor]:
@@ -44,28 +58,28 @@ def _workspace(n_bytes: int, device) -> Optional[torch.Tensor]:
 
 # ------------------------------------------------------------------ lookup ------
 def _lookup_rows(table: torch.Tensor, ids: torch.Tensor, scale: float, out_dtype: torch.dtype) -> torch.Tensor:
-    table = _rows(table)
-    out = torch.empty(*ids.shape, table.shape[1], dtype=out_dtype, device=table.device)
-    flat = ids.contiguous()
-    L.check(L.load().plnlp_embedding_lookup(table.data_ptr(), _ld(table), L.DTYPE_CODES[table.dtype], table.shape[0], table.shape[1],
-                                            flat.data_ptr(), flat.element_size(), flat.numel(), scale, out.data_ptr(),
-                                            max(table.shape[1], 1), L.DTYPE_CODES[out_dtype], L.stream_ptr()),
-            "plnlp_embedding_lookup")
+    stream = _stream(table, ids)
+    table, flat = _rows(table), ids.contiguous()
+    rows, width = table.shape
+    out = table.new_empty((*ids.shape, width), dtype=out_dtype)
+    L.check(L.load().plnlp_embedding_lookup(table.data_ptr(), _ld(table), L.DTYPE_CODES[table.dtype], rows, width, flat.data_ptr(),
+                                            flat.element_size(), flat.numel(), scale, out.data_ptr(), max(width, 1),
+                                            L.DTYPE_CODES[out_dtype], stream), "plnlp_embedding_lookup")
     return out
 
 
 def _lookup_grad(gy: torch.Tensor, ids: torch.Tensor, n_rows: int, padding: int, scale: float, dtype: torch.dtype) -> torch.Tensor:
     lib = L.load()
     width = gy.shape[-1]
+    stream = _stream(gy, ids)
     gy = _rows(gy.reshape(ids.numel(), width))
     flat = ids.contiguous()
-    L.require_device(gy, flat)
     grad = torch.empty(n_rows, width, dtype=dtype, device=gy.device)
     n_bytes = lib.plnlp_embedding_grad_workspace_bytes(flat.numel(), width)
     ws = _workspace(n_bytes, gy.device)
     L.check(lib.plnlp_embedding_grad(gy.data_ptr(), max(_ld(gy), width), L.DTYPE_CODES[gy.dtype], flat.data_ptr(), flat.element_size(),
                                      flat.numel(), padding, scale, grad.data_ptr(), max(width, 1), L.DTYPE_CODES[dtype], n_rows, width,
-                                     L.ptr(ws), n_bytes, L.stream_ptr()), "plnlp_embedding_grad")
+                                     L.ptr(ws), n_bytes, stream), "plnlp_embedding_grad")
     return grad
 
 
@@ -106,7 +120,6 @@ def embedding_lookup(table: torch.Tensor, ids: torch.Tensor, *, scale: float = 1
         if not -table.shape[0] <= padding_idx < table.shape[0]:
             raise ValueError(f"embedding_lookup: padding_idx {padding_idx} is no row of a table of {table.shape[0]}")
         padding = padding_idx % table.shape[0]
-    L.require_device(table, ids)
     if torch.is_grad_enabled() and table.requires_grad:
         return EmbeddingLookupFn.apply(table, ids, float(scale), padding, out_dtype)
     return _lookup_rows(table, ids, float(scale), out_dtype)
@@ -116,16 +129,17 @@ def embedding_lookup(table: torch.Tensor, ids: torch.Tensor, *, scale: float = 1
 def _linear_forward(x, weight, bias, residual, act: int, keep: bool):
     """(y [m, n], slope or None) of matrices as _rows gives them; the activation's derivative is kept where the backward pass will
     read it: int16 [m, n] in steps of 2^-14"""
+    stream = _stream(x, weight, bias, residual)
     lib = L.load()
     m, k = x.shape
     n = weight.shape[0]
-    out = torch.empty(m, n, dtype=x.dtype, device=x.device)
-    slope = torch.empty(m, n, dtype=torch.int16, device=x.device) if keep else None
+    out = x.new_empty((m, n))
+    slope = x.new_empty((m, n), dtype=torch.int16) if keep else None
     n_bytes = lib.plnlp_linear_act_workspace_bytes(m, n, k)
     ws = _workspace(n_bytes, x.device)
     L.check(lib.plnlp_linear_act(x.data_ptr(), _ld(x), weight.data_ptr(), _ld(weight), L.ptr(bias), L.ptr(residual),
                                  0 if residual is None else _ld(residual), act, m, n, k, L.ptr(slope), n, out.data_ptr(), n,
-                                 L.DTYPE_CODES[x.dtype], L.ptr(ws), n_bytes, L.stream_ptr()), "plnlp_linear_act")
+                                 L.DTYPE_CODES[x.dtype], L.ptr(ws), n_bytes, stream), "plnlp_linear_act")
     return out, slope
 
 
@@ -151,13 +165,13 @@ class LinearActFn(torch.autograd.Function):
         dw = torch.empty(n, k, dtype=x.dtype, device=x.device) if need[1] else None
         db = torch.empty(n, dtype=x.dtype, device=x.device) if need[2] else None
         if need[0] or need[1] or need[2]:
+            stream = _stream(gy, x, weight)
             g = _rows(gy)
-            L.require_device(g, x, weight)
             n_bytes = lib.plnlp_linear_act_backward_workspace_bytes(m, n, k, ctx.act)
             ws = _workspace(n_bytes, x.device)
             L.check(lib.plnlp_linear_act_backward(g.data_ptr(), _ld(g), L.ptr(slope), n, ctx.act, x.data_ptr(), _ld(x), weight.data_ptr(),
                                                   _ld(weight), m, n, k, L.ptr(dx), k, L.ptr(dw), k, L.ptr(db), L.DTYPE_CODES[x.dtype],
-                                                  L.ptr(ws), n_bytes, L.stream_ptr()), "plnlp_linear_act_backward")
+                                                  L.ptr(ws), n_bytes, stream), "plnlp_linear_act_backward")
         return dx, dw, db, gy if need[3] else None, None
 
 
@@ -170,38 +184,49 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tenso
     activation and residual act on the fp32 sums, which are rounded once.  The activation's derivative is kept
     for the backward pass in steps of 2^-14, where a gradient is wanted.
     fp32 matrices are the business of ops.LinearFn."""
-    if x.dtype not in _HALF:
-        raise TypeError(f"linear_act: x must be bf16 or fp16, not {x.dtype} (ops.LinearFn is the fp32 layer)")
-    if activation not in L.ACTIVATIONS:
+    dtype = x.dtype
+    if dtype not in _HALF:
+        raise TypeError(f"linear_act: x must be bf16 or fp16, not {dtype} (ops.LinearFn is the fp32 layer)")
+    act = L.ACTIVATIONS.get(activation)
+    if act is None:
         raise ValueError(f"linear_act: activation must be one of {', '.join(L.ACTIVATIONS)}, not {activation!r}")
-    if x.dim() < 1 or weight.dim() != 2 or weight.shape[1] != x.shape[-1]:
-        raise ValueError(f"linear_act: x {tuple(x.shape)} and weight {tuple(weight.shape)} do not match ([..., K] and [N, K])")
+    shape = x.shape
+    if len(shape) < 1 or weight.dim() != 2 or weight.shape[1] != shape[-1]:
+        raise ValueError(f"linear_act: x {tuple(shape)} and weight {tuple(weight.shape)} do not match ([..., K] and [N, K])")
     n = weight.shape[0]
-    shape = (*x.shape[:-1], n)
-    if bias is not None and tuple(bias.shape) != (n,):
-        raise ValueError(f"linear_act: bias must have shape ({n},), not {tuple(bias.shape)}")
-    if residual is not None and tuple(residual.shape) != shape:
-        raise ValueError(f"linear_act: residual must have the result's shape {shape}, not {tuple(residual.shape)}")
-    for t in (weight, bias, residual):
-        if t is not None and t.dtype != x.dtype:
-            raise TypeError(f"linear_act: all operands must have x's type {x.dtype}, not {t.dtype}")
-    L.require_device(x, weight, bias, residual)
-    rows = math.prod(x.shape[:-1])
-    x2 = _rows(x.reshape(rows, x.shape[-1]))
-    w2 = _rows(weight)
-    b2 = bias if bias is None or bias.stride(0) == 1 or n <= 1 else bias.contiguous()
-    r2 = None if residual is None else _rows(residual.reshape(rows, n))
-    act = L.ACTIVATIONS[activation]
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x2, w2, b2, r2)):
-        y = LinearActFn.apply(x2, w2, b2, r2, act)
+    out_shape = (*shape[:-1], n)
+    grad = x.requires_grad or weight.requires_grad
+    if weight.dtype != dtype:
+        raise TypeError(f"linear_act: all operands must have x's type {dtype}; weight is {weight.dtype}")
+    if bias is not None:
+        if bias.shape != (n,):
+            raise ValueError(f"linear_act: bias must have shape ({n},), not {tuple(bias.shape)}")
+        if bias.dtype != dtype:
+            raise TypeError(f"linear_act: all operands must have x's type {dtype}; bias is {bias.dtype}")
+        grad = grad or bias.requires_grad
+        bias = bias.contiguous()
+    if residual is not None:
+        if residual.shape != out_shape:
+            raise ValueError(f"linear_act: residual must have the result's shape {out_shape}, not {tuple(residual.shape)}")
+        if residual.dtype != dtype:
+            raise TypeError(f"linear_act: all operands must have x's type {dtype}; residual is {residual.dtype}")
+        grad = grad or residual.requires_grad
+    if len(shape) != 2:
+        rows = math.prod(shape[:-1])
+        x = x.reshape(rows, shape[-1])
+        residual = None if residual is None else residual.reshape(rows, n)
+    x, weight = _rows(x), _rows(weight)
+    residual = None if residual is None else _rows(residual)
+    if grad and torch.is_grad_enabled():
+        y = LinearActFn.apply(x, weight, bias, residual, act)
     else:
-        y = _linear_forward(x2, w2, b2, r2, act, False)[0]
-    return y.view(shape)
+        y = _linear_forward(x, weight, bias, residual, act, False)[0]
+    return y if len(shape) == 2 else y.view(out_shape)
 
 
 # ------------------------------------------------------------------ clipping ----
-_GRAD_ROW = np.dtype([("src", np.uint64), ("dst", np.uint64), ("n", np.int64), ("src_dtype", np.int32), ("dst_dtype", np.int32)])
-assert _GRAD_ROW.itemsize == C.sizeof(L.GradTensor)
+_DST_CODES = {t: c << 32 for t, c in L.DTYPE_CODES.items()}
+_SIZES = np.array([4, 2, 2], dtype=np.int64)
 
 
 def _norm_kind(norm_type) -> int:
@@ -215,49 +240,54 @@ def _norm_kind(norm_type) -> int:
     raise ValueError(f"norm_type must be 1, 2 or inf, not {norm_type!r}")
 
 
-def _check_list(tensors: Sequence[torch.Tensor], what: str) -> None:
-    device = torch.cuda.current_device() if tensors and torch.cuda.is_available() else -1
-    for t in tensors:
-        if t.dtype not in L.DTYPE_CODES or t.layout is not torch.strided:
-            raise TypeError(f"{what} must be dense bf16, fp16 or fp32 tensors, not {t.dtype}, {t.layout}")
-        if t.get_device() != device or device < 0:
-            L.require_device(t)
+def _pointers(tensors: Sequence[torch.Tensor], what: str):
+    """(addresses, sizes, types) of a list of dense tensors of the three types on the current device"""
+    try:
+        ptrs = list(map(torch.Tensor.data_ptr, tensors))
+    except RuntimeError:
+        raise TypeError(f"{what} must be dense tensors") from None
+    types = [t.dtype for t in tensors]
+    for t in set(types):
+        if t not in L.DTYPE_CODES:
+            raise TypeError(f"{what} must be bf16, fp16 or fp32, not {t}")
+    on = set(map(torch.Tensor.get_device, tensors))
+    if on and (len(on) > 1 or -1 in on or torch.cuda.current_device() not in on):
+        L.require_device(*tensors)
+    return ptrs, list(map(torch.Tensor.numel, tensors)), types
 
 
-def _table(src: Sequence[torch.Tensor], dst: Optional[Sequence[torch.Tensor]]):
-    rows = np.zeros(len(src), dtype=_GRAD_ROW)
-    codes = L.DTYPE_CODES
-    rows["src"] = [t.data_ptr() for t in src]
-    rows["n"] = [t.numel() for t in src]
-    rows["src_dtype"] = [codes[t.dtype] for t in src]
-    if dst is not None:
-        rows["dst"] = [t.data_ptr() for t in dst] if dst is not src else rows["src"]
-        rows["dst_dtype"] = [codes[t.dtype] for t in dst] if dst is not src else rows["src_dtype"]
-    return rows
+def _codes(types, codes) -> list:
+    return list(map(codes.__getitem__, types))
 
 
-def _refuse_overlaps(rows) -> None:
-    """a written range that another entry reads or writes would be scaled twice, or read half scaled"""
-    rows = rows[rows["n"] > 0]
-    size = np.array([4, 2, 2])
-    s0 = rows["src"].astype(np.int64)
-    s1 = s0 + rows["n"] * size[rows["src_dtype"]]
-    d0 = rows["dst"].astype(np.int64)
-    d1 = d0 + rows["n"] * size[rows["dst_dtype"]]
-    order = np.argsort(d0, kind="stable")
-    bad = bool((d1[order][:-1] > d0[order][1:]).any())
-    if not bad:
-        same = s0 == d0
-        # each source against the written ranges around its beginning (they do not overlap one another): the last that begins at or
-        # before it and the next one; its own is meant to be there where it is clipped in place
-        at = np.searchsorted(d0[order], s0, side="right")
-        before, after = np.maximum(at - 1, 0), np.minimum(at, len(order) - 1)
-        own = np.arange(len(rows))
-        hit = (at > 0) & (d1[order][before] > s0) & ~(same & (order[before] == own))
-        hit |= (at < len(order)) & (d0[order][after] < s1)
-        bad = bool(hit.any())
-    if bad:
-        raise ValueError("clip_grads: the memory of a clipped tensor overlaps another tensor of the call (a gradient listed twice?)")
+def _contiguous(tensors: List[torch.Tensor], fresh: bool = False) -> List[torch.Tensor]:
+    """the list itself where all are contiguous, else with copies (fresh: uninitialised ones) in the place of those that are not"""
+    if all(map(torch.Tensor.is_contiguous, tensors)):
+        return tensors
+    return [t if t.is_contiguous() else torch.empty_like(t, memory_format=torch.contiguous_format) if fresh else t.contiguous()
+            for t in tensors]
+
+
+def _overlap(src, dst, n, src_types, dst_types) -> bool:
+    """whether a written range [dst, dst + n) meets another written range, or a read range [src, src + n) other than the one that is
+    clipped in place (arrays of addresses, elements and type codes)"""
+    some = n > 0
+    if not some.all():
+        src, dst, n, src_types, dst_types = src[some], dst[some], n[some], src_types[some], dst_types[some]
+    end = dst + n * _SIZES[dst_types]
+    order = np.argsort(dst)
+    first, last = dst[order], end[order]
+    if (last[:-1] > first[1:]).any():
+        return True
+    if src is dst or len(src) == 0 or (src == dst).all():
+        return False
+    # each read range against the written ones around its beginning, which do not overlap one another: the last that begins at or
+    # before it and the next one; its own is meant to be there where it is clipped in place
+    src_end = src + n * _SIZES[src_types]
+    at = np.searchsorted(first, src, side="right")
+    before, after = np.maximum(at - 1, 0), np.minimum(at, len(order) - 1)
+    mine = (src == dst) & (order[before] == np.arange(len(src)))
+    return bool(((at > 0) & (last[before] > src) & ~mine).any() or ((at < len(order)) & (first[after] < src_end)).any())
 
 
 def grad_norm(grads: Sequence[torch.Tensor], *, norm_type: float = 2.0) -> torch.Tensor:
@@ -266,19 +296,34 @@ def grad_norm(grads: Sequence[torch.Tensor], *, norm_type: float = 2.0) -> torch
     neither large nor tiny elements leave the range.  Tensors that are not contiguous are read through a copy."""
     kind = _norm_kind(norm_type)
     grads = list(grads)
-    _check_list(grads, "grad_norm: gradients")
-    return _norm(grads, kind)
+    ptrs, sizes, types = _pointers(grads, "grad_norm: gradients")
+    flat = _contiguous(grads)
+    if flat is not grads:
+        ptrs = list(map(torch.Tensor.data_ptr, flat))
+    return _run_clip(ptrs, ptrs, sizes, _codes(types, L.DTYPE_CODES), None, kind, None)
 
 
-def _norm(grads, kind: int) -> torch.Tensor:
+def _run_clip(src, dst, sizes, src_codes, dst_codes, kind: int, max_norm: Optional[float]) -> torch.Tensor:
+    """grad_norm (max_norm None) or clip_grads on lists of addresses"""
     lib = L.load()
-    grads = [t if t.is_contiguous() else t.contiguous() for t in grads]
-    norm = torch.empty((), dtype=torch.float32, device="cuda")
-    rows = _table(grads, None)
-    arr = rows.ctypes.data_as(C.POINTER(L.GradTensor))
-    need = lib.plnlp_grad_norm_workspace_doubles(arr, len(grads))
-    ws = torch.empty(need, dtype=torch.float64, device="cuda")
-    L.check(lib.plnlp_grad_norm(arr, len(grads), kind, ws.data_ptr(), need, norm.data_ptr(), L.stream_ptr()), "plnlp_grad_norm")
+    n = len(src)
+    types = src_codes if dst_codes is None else list(map(int.__or__, src_codes, dst_codes))
+    # the rows of plnlp_grad_tensor: two addresses, a size, two 32-bit type codes
+    rows = np.array([src, dst, sizes, types], dtype=np.int64)
+    if max_norm is not None and (n > 1 or src is not dst):
+        to = rows[3] >> 32
+        if _overlap(rows[0], rows[0] if src is dst else rows[1], rows[2], rows[3] & 3, to):
+            raise ValueError("clip_grads: the memory of a clipped tensor overlaps another tensor of the call (a gradient listed twice?)")
+    rows = np.ascontiguousarray(rows.T)
+    at = rows.ctypes.data
+    need = lib.plnlp_grad_norm_workspace_doubles(at, n)
+    device = torch.cuda.current_device()
+    norm = torch.empty((), dtype=torch.float32, device=device)
+    ws = torch.empty(need, dtype=torch.float64, device=device)
+    if max_norm is None:
+        L.check(lib.plnlp_grad_norm(at, n, kind, ws.data_ptr(), need, norm.data_ptr(), L.stream_ptr()), "plnlp_grad_norm")
+    else:
+        L.check(lib.plnlp_grad_clip(at, n, kind, max_norm, ws.data_ptr(), need, norm.data_ptr(), L.stream_ptr()), "plnlp_grad_clip")
     return norm
 
 
@@ -287,37 +332,34 @@ def clip_grads(grads: Sequence[torch.Tensor], max_norm: float, *, norm_type: flo
     """Scales all gradients by min(1, max_norm / (norm + 1e-6)), norm = grad_norm(grads), and returns that norm (a 0-d fp32
     tensor on the device; nothing is read back by the host).
 
-    out: where the scaled gradients go -- tensors of the same shapes, of any of the three types: 16-bit gradients into the fp32
-    ones an optimiser of fp32 parameters reads; None: in place.  As torch.nn.utils.clip_grad_norm_ has it, a NaN norm makes
-    every gradient NaN and an infinite one makes the finite elements zero.  A tensor listed twice, or one whose memory another
-    one's result would overwrite, is refused.  Tensors that are not contiguous are handled through copies."""
+    out: where the scaled gradients go -- one tensor of as many elements for each, of any of the three types: 16-bit gradients
+    into the fp32 ones an optimiser of fp32 parameters reads; None: in place.  As torch.nn.utils.clip_grad_norm_ has it, a NaN
+    norm makes every gradient NaN and an infinite one makes the finite elements zero.  A tensor listed twice, or one whose
+    memory another one's result would overwrite, is refused.  Tensors that are not contiguous are handled through copies."""
     kind = _norm_kind(norm_type)
     max_norm = float(max_norm)
     if not max_norm >= 0.0:
         raise ValueError(f"clip_grads: max_norm must be 0 or more, not {max_norm}")
     grads = list(grads)
-    _check_list(grads, "clip_grads: gradients")
-    lib = L.load()
-    src = [t if t.is_contiguous() else t.contiguous() for t in grads]
-    back = []
+    src, sizes, types = _pointers(grads, "clip_grads: gradients")
     if out is None:
-        dst = src
-        back = [(t, c) for t, c in zip(grads, src) if c is not t]
+        to, dst, to_types = grads, src, types
     else:
-        out = list(out)
-        _check_list(out, "clip_grads: out")
-        if len(out) != len(grads) or any(o.shape != g.shape for o, g in zip(out, grads)):
-            raise ValueError("clip_grads: out must hold one tensor of the same shape for each gradient")
-        dst = [t if t.is_contiguous() else torch.empty_like(t, memory_format=torch.contiguous_format) for t in out]
-        back = [(t, c) for t, c in zip(out, dst) if c is not t]
-    rows = _table(src, dst)
-    if len(rows) > 1 or out is not None:
-        _refuse_overlaps(rows)
-    arr = rows.ctypes.data_as(C.POINTER(L.GradTensor))
-    need = lib.plnlp_grad_norm_workspace_doubles(arr, len(src))
-    norm = torch.empty((), dtype=torch.float32, device="cuda")
-    ws = torch.empty(need, dtype=torch.float64, device="cuda")
-    L.check(lib.plnlp_grad_clip(arr, len(src), kind, max_norm, ws.data_ptr(), need, norm.data_ptr(), L.stream_ptr()), "plnlp_grad_clip")
-    for t, c in back:
-        t.copy_(c)
+        to = list(out)
+        dst, to_sizes, to_types = _pointers(to, "clip_grads: out")
+        if to_sizes != sizes:
+            raise ValueError("clip_grads: out must hold one tensor of as many elements for each gradient")
+    flat = _contiguous(grads)
+    flat_to = flat if out is None else _contiguous(to, fresh=True)
+    if flat is not grads:
+        src = list(map(torch.Tensor.data_ptr, flat))
+    if flat_to is not to:
+        dst = src if out is None else list(map(torch.Tensor.data_ptr, flat_to))
+    norm = _run_clip(src, dst, sizes, _codes(types, L.DTYPE_CODES), _codes(to_types, _DST_CODES), kind, max_norm)
+    torch.autograd.graph.increment_version(to)       # (written behind autograd's back)
+    if flat_to is not to:
+        with torch.no_grad():
+            for t, c in zip(to, flat_to):
+                if c is not t:
+                    t.copy_(c)
     return norm

@@ -628,24 +628,20 @@ def test_overlaps_are_found():
     import numpy as np
     from plnlp_amd import mixed
 
-    def rows(*entries):
-        return np.array([(s, d, n, st, dt) for s, d, n, st, dt in entries], dtype=mixed._GRAD_ROW)
-    ok = [rows((1000, 1000, 10, 0, 0), (1040, 1040, 10, 0, 0)),              # in place, side by side
-          rows((1000, 2000, 10, 1, 0), (1010, 2040, 10, 1, 0)),              # sources may overlap: they are only read
-          rows((1000, 1000, 10, 0, 0), (1000, 1000, 0, 0, 0)),               # nothing in an empty one
-          rows((1000, 3000, 10, 1, 0), (5000, 5000, 4, 0, 0)), rows()]
-    bad = [rows((1000, 1000, 10, 0, 0), (1000, 1000, 10, 0, 0)),             # listed twice
-           rows((1000, 1000, 10, 0, 0), (1036, 1036, 10, 0, 0)),
-           rows((1000, 2000, 10, 0, 0), (1100, 2039, 10, 0, 0)),             # written ranges overlap
-           rows((1000, 1020, 10, 0, 0)),                                     # its own source, shifted
-           rows((1020, 1000, 10, 0, 0)),
-           rows((1000, 2000, 10, 0, 0), (2000, 3000, 10, 0, 0)),             # one's result over another's source
-           rows((2036, 3000, 10, 0, 0), (1000, 2000, 10, 0, 0))]
-    for r in ok:
-        mixed._refuse_overlaps(r)
-    for r in bad:
-        with pytest.raises(ValueError):
-            mixed._refuse_overlaps(r)
+    def check(*entries):
+        src, dst, n, st, dt = (np.array([e[i] for e in entries], dtype=np.int64) for i in range(5))
+        return mixed._overlap(src, dst, n, st, dt)
+    F, H = 0, 1                                                              # four bytes, two bytes
+    assert not check() and not check((1000, 1000, 10, F, F), (1040, 1040, 10, F, F))          # in place, side by side
+    assert not check((1000, 2000, 10, H, F), (1010, 2040, 10, H, F))         # sources may overlap: they are only read
+    assert not check((1000, 1000, 10, F, F), (1000, 1000, 0, F, F))          # nothing in an empty one
+    assert not check((1000, 3000, 10, H, F), (5000, 5000, 4, F, F))
+    assert check((1000, 1000, 10, F, F), (1000, 1000, 10, F, F))             # listed twice
+    assert check((1000, 1000, 10, F, F), (1036, 1036, 10, F, F))
+    assert check((1000, 2000, 10, F, F), (1100, 2039, 10, F, F))             # written ranges overlap
+    assert check((1000, 1020, 10, F, F)) and check((1020, 1000, 10, F, F))   # its own source, shifted
+    assert check((1000, 2000, 10, F, F), (2000, 3000, 10, F, F))             # one's result over another's source
+    assert check((2036, 3000, 10, F, F), (1000, 2000, 10, F, F))
 
 
 def test_argument_checks_of_the_library():
