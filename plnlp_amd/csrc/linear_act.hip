@@ -110,8 +110,9 @@ template <typename T> struct Finish {
 };
 constexpr int PARTIAL = -1; // in the place of an activation: the sum is one K slice's, stored as it is
 
-// V consecutive columns of row m from column n on (all inside the matrix); b = the bias there
-template <int ACT, typename T, int V> __device__ __forceinline__ void finish_cols(const Finish<T>& f, float (&v)[V], const float (&b)[V], int64_t m, int64_t n) {
+// V consecutive columns of row m from column n on (all inside the matrix); b = the bias there, res = the residual there (if f.res)
+template <int ACT, typename T, int V>
+__device__ __forceinline__ void finish_with(const Finish<T>& f, float (&v)[V], const float (&b)[V], const Pack<T, V>& res, int64_t m, int64_t n) {
 #pragma unroll
     for (int j = 0; j < V; ++j) v[j] += b[j];
     float s[V];
@@ -123,13 +124,16 @@ template <int ACT, typename T, int V> __device__ __forceinline__ void finish_col
     } else
 #pragma unroll
         for (int j = 0; j < V; ++j) v[j] = act_of<ACT, false>(v[j], s[j]);
-    if (f.res) {
-        float r[V];
-        load_f32<T, V>(f.res + m * f.ldr + n, r);
+    if (f.res)
 #pragma unroll
-        for (int j = 0; j < V; ++j) v[j] += r[j];
-    }
+        for (int j = 0; j < V; ++j) v[j] += (float)res.v[j];
     store_f32<T, V>(f.out + m * f.ldo + n, v);
+}
+template <int ACT, typename T, int V>
+__device__ __forceinline__ void finish_cols(const Finish<T>& f, float (&v)[V], const float (&b)[V], int64_t m, int64_t n) {
+    Pack<T, V> res;
+    if (f.res) res = *reinterpret_cast<const Pack<T, V>*>(f.res + m * f.ldr + n);
+    finish_with<ACT, T, V>(f, v, b, res, m, n);
 }
 
 // ---- the tile kernel --------------------------------------------------------------------------------------------
@@ -140,13 +144,15 @@ template <typename T> struct TileArgs {
     int64_t  plane;                                // P's second term lies this many elements behind its first
     int      terms;                                // 1, or 2: C = (P + P2) Q^T as one sum over twice as many steps
     int      tiles_m, tiles_n, slices, steps;      // steps: BK-steps per slice
+    float*   sums;                                 // nullable [slices, m]: sum_k P(m, k) of each slice (PT)
     float*   partial;                              // slices > 1: [slices, m, n]
     Finish<T> fin;
 };
 
-// which 16-byte unit of LDS row r holds unit 0 (unit u sits at u ^ swz): eight lanes that read rows 0..7, or the permuted Q rows
-// {0..3, 8..11}, or that store a transposed block's rows 4 apart, touch eight different units
-__device__ __forceinline__ int swz(int r) { return (r & 7) ^ (((r >> 3) & 1) * 6) ^ ((r >> 4) & 1); }
+// Unit u of LDS row r sits at u ^ swz(r).  A 16-byte read serves 16 lanes a clock from 64 banks, two rows of 128 bytes: of the rows
+// 0..15 of a fragment, of the dealt Q rows (q_row) and of a transposed block's rows 4 apart, those of one parity sit in eight
+// different units.
+__device__ __forceinline__ int swz(int r) { return ((r >> 1) & 1) ^ (((r >> 3) & 1) << 1) ^ (((r >> 2) & 1) << 2) ^ (((r >> 4) & 1) * 5); }
 
 // Q row (column of C) behind row r of the MFMA's tile t: lane group g = r >> 2 gets columns 32 (t / 2) + 8 g + 4 (t & 1) + 0..3, so its
 // tiles 2h and 2h + 1 are eight consecutive columns, and the four groups' stores 64 consecutive bytes
@@ -206,20 +212,21 @@ __device__ __forceinline__ void fetch_cols(Stage<R, THREADS>& s, const T* base, 
         }
     }
 }
+// column j of an 8 k x 4 columns block held as eight rows of two words: its eight k
+__device__ __forceinline__ u32x4 block_column(const uint32_t* d, int j) {
+    u32x4 o;
+#pragma unroll
+    for (int h = 0; h < 4; ++h) {
+        const uint32_t a = d[(2 * h) * 2 + (j >> 1)], b = d[(2 * h + 1) * 2 + (j >> 1)];
+        o[h] = __builtin_amdgcn_perm(b, a, (j & 1) ? 0x07060302u : 0x05040100u);
+    }
+    return o;
+}
 template <int R, int THREADS> __device__ __forceinline__ void store_cols(const Stage<R, THREADS>& s, char* lds) {
     const int c = (threadIdx.x % (R / 4)) * 4, g = threadIdx.x / (R / 4);
     const uint32_t* d = reinterpret_cast<const uint32_t*>(s.r);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        u32x4 o;
-#pragma unroll
-        for (int h = 0; h < 4; ++h) {
-            const uint32_t a = d[(2 * h) * 2 + (j >> 1)], b = d[(2 * h + 1) * 2 + (j >> 1)];
-            o[h] = __builtin_amdgcn_perm(b, a, (j & 1) ? 0x07060302u : 0x05040100u);
-        }
-        const int row = c + j;
-        *reinterpret_cast<u32x4*>(lds + row * 128 + ((g ^ swz(row)) << 4)) = o;
-    }
+    for (int j = 0; j < 4; ++j) *reinterpret_cast<u32x4*>(lds + (c + j) * 128 + ((g ^ swz(c + j)) << 4)) = block_column(d, j);
 }
 
 template <typename T, int BM, int BN, int WM, int WN, bool PT, bool QT, bool VEC, int ACT>
@@ -230,30 +237,38 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void tile_kernel(TileArgs<T> a) {
     extern __shared__ __attribute__((aligned(16))) char lds[];       // two buffers of P rows, then Q rows
     constexpr int BUF = (BM + BN) * 128;
 
-    // A workgroup takes tiles blockIdx.x, + gridDim.x, ... (a multiple of 8): the first loads of its next tile are under way while it
-    // finishes one.  Workgroups are dealt to the eight XCDs in turn: each XCD gets a contiguous run of tiles, so that its L2 holds the
-    // panels they share, and walks groups of 8 row panels column by column.
+    // Workgroups are dealt to the eight XCDs in turn: each XCD gets a contiguous run of tiles, so that its L2 holds the panels they share
     const int tiles = a.tiles_m * a.tiles_n, total = tiles * a.slices;
-    const int term_steps = (int)((a.k + BK - 1) / BK);
-    int64_t m0, n0;
-    int slice, first, steps;
-    auto locate = [&](int at) {
-        const int per = total >> 3, extra = total & 7, xcd = at & 7;
-        const int id = xcd * per + min(xcd, extra) + (at >> 3);
-        const int tile = id % tiles;
-        slice = id / tiles;
-        constexpr int GROUP = 8;
-        const int group = tile / (GROUP * a.tiles_n), in_group = tile % (GROUP * a.tiles_n);
-        const int g_rows = min(GROUP, a.tiles_m - group * GROUP);
-        m0 = (int64_t)(group * GROUP + in_group % g_rows) * BM;
-        n0 = (int64_t)(in_group / g_rows) * BN;
-        first = slice * a.steps;
-        steps = min(a.steps, term_steps * a.terms - first);
-    };
-    locate(blockIdx.x);
+    const int per = total >> 3, extra = total & 7, xcd = blockIdx.x & 7, nth = blockIdx.x >> 3;
+    const int id = xcd * per + min(xcd, extra) + nth;
+    const int slice = id / tiles, tile = id % tiles;
+    // and walks groups of 8 row panels column by column
+    constexpr int GROUP = 8;
+    const int group = tile / (GROUP * a.tiles_n), in_group = tile % (GROUP * a.tiles_n);
+    const int g_rows = min(GROUP, a.tiles_m - group * GROUP);
+    const int64_t m0 = (int64_t)(group * GROUP + in_group % g_rows) * BM, n0 = (int64_t)(in_group / g_rows) * BN;
 
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
     const int wm = (wave / WN) * (BM / WM), wn = (wave % WN) * 64;
+    const int term_steps = (int)((a.k + BK - 1) / BK), first = slice * a.steps;
+    const int steps = min(a.steps, term_steps * a.terms - first);
+    const int rows_p = (int)min((int64_t)BM, a.m - m0), rows_q = (int)min((int64_t)BN, a.n - n0);
+
+    f32x4 acc[TM][4];
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int t = 0; t < 4; ++t) acc[i][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+    // sums over k of P, the bias gradient where P is dz: one more product, with a Q of ones, in the waves of the first column tile
+    constexpr bool SUMS = PT && BM == 128;      // (a result large enough for 256 x 256 tiles comes with its dz summed already)
+    const bool sum_p = SUMS && a.sums && n0 == 0 && wn == 0;
+    f32x4 psum[SUMS ? TM : 1];
+    frag ones;
+#pragma unroll
+    for (int i = 0; i < (SUMS ? TM : 1); ++i) psum[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int j = 0; j < 8; ++j) ones[j] = (T)1.f;
 
     Stage<BM, THREADS> sp;
     Stage<BN, THREADS> sq;
@@ -261,7 +276,6 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void tile_kernel(TileArgs<T> a) {
         const int at = first + step, term = at >= term_steps;
         const int64_t k = (int64_t)(at - (term ? term_steps : 0)) * BK, left = a.k - k;
         const T* p = a.p + (term ? a.plane : 0);
-        const int rows_p = (int)min((int64_t)BM, a.m - m0), rows_q = (int)min((int64_t)BN, a.n - n0);
         if (PT) fetch_cols<T, BM, THREADS, VEC>(sp, p + k * a.ldp + m0, a.ldp, rows_p, left);
         else fetch_rows<T, BM, THREADS, VEC>(sp, p + m0 * a.ldp + k, a.ldp, rows_p, left);
         if (QT) fetch_cols<T, BN, THREADS, VEC>(sq, a.q + k * a.ldq + n0, a.ldq, rows_q, left);
@@ -272,90 +286,84 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void tile_kernel(TileArgs<T> a) {
         if (PT) store_cols<BM, THREADS>(sp, b); else store_rows<BM, THREADS>(sp, b);
         if (QT) store_cols<BN, THREADS>(sq, b + BM * 128); else store_rows<BN, THREADS>(sq, b + BM * 128);
     };
-    if (steps > 0) fetch(0);
-    for (int at = blockIdx.x;;) {
-        f32x4 acc[TM][4];
+    if (steps > 0) {
+        fetch(0);
+        stage(0);
+        if (steps > 1) fetch(1);
+        __syncthreads();
+    }
+    for (int step = 0; step < steps; ++step) {
+        const char* b = lds + (step & 1) * BUF;
+        if (step + 1 < steps) stage((step + 1) & 1);      // the other buffer was read before the barrier that ended the last step
+        if (step + 2 < steps) fetch(step + 2);            // a whole step to arrive in
 #pragma unroll
-        for (int i = 0; i < TM; ++i)
+        for (int ks = 0; ks < BK / 32; ++ks) {
+            frag q[4];
 #pragma unroll
-            for (int t = 0; t < 4; ++t) acc[i][t] = f32x4{0.f, 0.f, 0.f, 0.f};
-        if (steps > 0) {
-            stage(0);
-            if (steps > 1) fetch(1);
-            __syncthreads();
-        }
-        for (int step = 0; step < steps; ++step) {
-            const char* b = lds + (step & 1) * BUF;
-            if (step + 1 < steps) stage((step + 1) & 1);      // the other buffer was read before the barrier that ended the last step
-            if (step + 2 < steps) fetch(step + 2);            // a whole step to arrive in
-#pragma unroll
-            for (int ks = 0; ks < BK / 32; ++ks) {
-                frag q[4];
-#pragma unroll
-                for (int t = 0; t < 4; ++t) {
-                    const int row = wn + q_row(t, r);
-                    q[t] = *reinterpret_cast<const frag*>(b + (BM + row) * 128 + (((ks * 4 + g) ^ swz(row)) << 4));
-                }
-#pragma unroll
-                for (int i = 0; i < TM; ++i) {
-                    const int row = wm + i * 16 + r;
-                    const frag p = *reinterpret_cast<const frag*>(b + row * 128 + (((ks * 4 + g) ^ swz(row)) << 4));
-#pragma unroll
-                    for (int t = 0; t < 4; ++t) acc[i][t] = Mfma<T>::go(q[t], p, acc[i][t]);
-                }
+            for (int t = 0; t < 4; ++t) {
+                const int row = wn + q_row(t, r);
+                q[t] = *reinterpret_cast<const frag*>(b + (BM + row) * 128 + (((ks * 4 + g) ^ swz(row)) << 4));
             }
-            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < TM; ++i) {
+                const int row = wm + i * 16 + r;
+                const frag p = *reinterpret_cast<const frag*>(b + row * 128 + (((ks * 4 + g) ^ swz(row)) << 4));
+#pragma unroll
+                for (int t = 0; t < 4; ++t) acc[i][t] = Mfma<T>::go(q[t], p, acc[i][t]);
+                if (SUMS) if (sum_p) psum[SUMS ? i : 0] = Mfma<T>::go(ones, p, psum[SUMS ? i : 0]);
+            }
         }
+        __syncthreads();
+    }
 
-        // lane (r, g) holds columns n + 32 h + 0..7 (h = 0, 1) of rows mr + 16 i
-        const int64_t n = n0 + wn + 8 * g, mr = m0 + wm + r;
-        const int part = slice;
-        at += gridDim.x;
-        if (at < total) {
-            locate(at);
-            if (steps > 0) fetch(0);
+    if (SUMS && sum_p && g == 0) {
+#pragma unroll
+        for (int i = 0; i < (SUMS ? TM : 1); ++i) {
+            const int64_t m = m0 + wm + i * 16 + r;
+            if (m < a.m) a.sums[(int64_t)slice * a.m + m] = psum[i][0];
         }
-        int cols[2];
+    }
+    // lane (r, g) holds columns n + 32 h + 0..7 (h = 0, 1) of rows wm + 16 i + r
+    const int64_t n = n0 + wn + 8 * g;
+    int cols[2];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) cols[h] = (int)max(min((int64_t)8, a.n - n - 32 * h), (int64_t)0);
-        float bias[2][8];
+    for (int h = 0; h < 2; ++h) cols[h] = (int)max(min((int64_t)8, a.n - n - 32 * h), (int64_t)0);
+    float bias[2][8];
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
+    for (int h = 0; h < 2; ++h)
 #pragma unroll
-            for (int j = 0; j < 8; ++j) bias[h][j] = (ACT != PARTIAL && a.fin.bias && j < cols[h]) ? (float)a.fin.bias[n + 32 * h + j] : 0.f;
+        for (int j = 0; j < 8; ++j) bias[h][j] = (ACT != PARTIAL && a.fin.bias && j < cols[h]) ? (float)a.fin.bias[n + 32 * h + j] : 0.f;
 #pragma unroll
-        for (int i = 0; i < TM; ++i) {
-            const int64_t m = mr + i * 16;
-            if (m >= a.m) continue;
+    for (int i = 0; i < TM; ++i) {
+        const int64_t m = m0 + wm + i * 16 + r;
+        if (m >= a.m) continue;
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int64_t col = n + 32 * h;
-                if (cols[h] <= 0) continue;
-                if constexpr (ACT == PARTIAL) {
-                    float* o = a.partial + ((int64_t)part * a.m + m) * a.n + col;
+        for (int h = 0; h < 2; ++h) {
+            const int64_t col = n + 32 * h;
+            if (cols[h] <= 0) continue;
+            if constexpr (ACT == PARTIAL) {
+                float* o = a.partial + ((int64_t)slice * a.m + m) * a.n + col;
 #pragma unroll
-                    for (int t = 0; t < 2; ++t) {
-                        if (VEC) *reinterpret_cast<f32x4*>(o + 4 * t) = acc[i][2 * h + t];      // (n is whole groups of eight)
-                        else
+                for (int t = 0; t < 2; ++t) {
+                    if (VEC) *reinterpret_cast<f32x4*>(o + 4 * t) = acc[i][2 * h + t];      // (n is whole groups of eight)
+                    else
 #pragma unroll
-                            for (int j = 0; j < 4; ++j) if (4 * t + j < cols[h]) o[4 * t + j] = acc[i][2 * h + t][j];
-                    }
-                } else if constexpr (VEC) {
-                    float v[8];
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) v[j] = acc[i][2 * h + (j >> 2)][j & 3];
-                    finish_cols<ACT, T, 8>(a.fin, v, bias[h], m, col);
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 8; ++j)
-                        if (j < cols[h]) {
-                            float v[1] = {acc[i][2 * h + (j >> 2)][j & 3]}, b[1] = {bias[h][j]};
-                            finish_cols<ACT, T, 1>(a.fin, v, b, m, col + j);
-                        }
+                        for (int j = 0; j < 4; ++j) if (4 * t + j < cols[h]) o[4 * t + j] = acc[i][2 * h + t][j];
                 }
+            } else if constexpr (VEC) {
+                float v[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) v[j] = acc[i][2 * h + (j >> 2)][j & 3];
+                finish_cols<ACT, T, 8>(a.fin, v, bias[h], m, col);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    if (j < cols[h]) {
+                        float v[1] = {acc[i][2 * h + (j >> 2)][j & 3]}, b[1] = {bias[h][j]};
+                        finish_cols<ACT, T, 1>(a.fin, v, b, m, col + j);
+                    }
             }
         }
-        if (at >= total) return;
     }
 }
 
@@ -389,6 +397,157 @@ __global__ __launch_bounds__(256) void slices_kernel(const float* __restrict__ p
 #pragma unroll
         for (int j = 0; j < V; ++j) b[j] = (float)fin.bias[col + j];
     finish_cols<ACT, T, V>(fin, v, b, row, col);
+}
+
+// ---- many rows, a Q that fits LDS: Q stays there, P streams through registers -----------------------------------------
+// A layer of a few hundred columns on 10^4 .. 10^6 rows is bound by its rows' bytes, and the tile kernel spends its time waiting for
+// them (a tile of four K steps: load, wait, multiply, finish, with two workgroups a CU to overlap).  Here one workgroup a CU stages all
+// of Q in LDS once; after that its waves never meet again: each takes 16 rows, holds them as MFMA fragments (loaded straight from
+// memory, 64 consecutive bytes a row and load) and walks Q's columns 64 at a time, finishing each group before the next -- so a
+// wave needs 16 accumulators whatever n is -- and the next 16 rows, and the next columns' residual, load meanwhile.
+//   m 131 072, n = k = 256 (bf16, gelu with slope, residual; 268 MB): see the figures at rows_fit.
+// SLOPED: P = dy * slope, formed in the registers (the backward pass: dz = dy * act'(z), dx = dz W), and kept in dz for the
+// weights' gradient.
+template <typename T> struct RowsArgs {
+    const T* p; int64_t ldp;
+    const int16_t* slope; int64_t lds;      // SLOPED
+    T* dz; int64_t ldz;
+    const T* q; int64_t ldq;
+    int64_t m; int n, k;
+    Finish<T> fin;
+};
+
+// rows of KS * 64 bytes begin at the same bank (KS >= 4): the dealt Q rows of a fragment sit in sixteen different units instead
+template <int KS> __device__ __forceinline__ int rows_swz(int r) { return KS < 4 ? swz(r) : (r & 3) ^ (((r >> 3) & 3) << 2); }
+
+template <typename T, int KS, bool QT, bool SLOPED, int ACT>
+__global__ __launch_bounds__(512) void rows_kernel(RowsArgs<T> a) {
+    typedef typename Mfma<T>::frag frag;
+    constexpr int THREADS = 512, WAVES = THREADS / 64, UNITS = KS * 4, ROW = KS * 64;
+    constexpr bool EARLY = KS <= 8;          // registers for the next rows from the beginning of a tile; else from its last columns
+    extern __shared__ __attribute__((aligned(16))) char lds[];       // [n rounded up to 64][KS * 32] of Q, [n rounded up to 64] of the bias
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
+    const int64_t tiles = (a.m + 15) / 16, stride = (int64_t)gridDim.x * WAVES;
+    int64_t t = (int64_t)blockIdx.x * WAVES + wave;
+
+    frag next[KS];                           // P as it lies in memory
+    Pack<int16_t, 8> sl[SLOPED ? KS : 1];
+    auto fetch = [&](int64_t tile) {
+        const int64_t row = min(tile * 16 + r, a.m - 1);
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+            const int k = ks * 32 + g * 8;
+            const frag zero = {};
+            next[ks] = k < a.k ? *reinterpret_cast<const frag*>(a.p + row * a.ldp + k) : zero;
+            if (SLOPED && k < a.k) sl[SLOPED ? ks : 0] = *reinterpret_cast<const Pack<int16_t, 8>*>(a.slope + row * a.lds + k);
+        }
+    };
+    Pack<T, 8> res[2];                       // the residual of the columns that come next
+    auto ask = [&](int64_t tile, int n0) {
+        const int64_t m = tile * 16 + r;
+        if (ACT == PARTIAL || !a.fin.res || m >= a.m) return;
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+            if (n0 + 8 * g + 32 * h < a.n) res[h] = *reinterpret_cast<const Pack<T, 8>*>(a.fin.res + m * a.fin.ldr + n0 + 8 * g + 32 * h);
+    };
+    if (t < tiles) { fetch(t); ask(t, 0); }
+
+    // (loads and stores of a wave complete in order: the bias lies in LDS because a load of it among the columns would wait for the
+    // next rows and the last columns' stores; several loads of a thread in flight: one after the other they took longer than the rows)
+    const int n64 = (a.n + 63) / 64 * 64;
+    float* bias = reinterpret_cast<float*>(lds + n64 * ROW);
+    for (int i = threadIdx.x; i < n64; i += THREADS) bias[i] = (a.fin.bias && i < a.n) ? (float)a.fin.bias[i] : 0.f;
+    if (!QT) {
+        constexpr int AHEAD = 8;
+        for (int u0 = threadIdx.x; u0 < n64 * UNITS; u0 += THREADS * AHEAD) {
+            u32x4 v[AHEAD];
+#pragma unroll
+            for (int i = 0; i < AHEAD; ++i) {
+                const int u = u0 + i * THREADS, row = u / UNITS, unit = u % UNITS;
+                v[i] = u32x4{0, 0, 0, 0};
+                if (row < a.n && unit * 8 < a.k) v[i] = *reinterpret_cast<const u32x4*>(a.q + (int64_t)row * a.ldq + unit * 8);
+            }
+#pragma unroll
+            for (int i = 0; i < AHEAD; ++i) {
+                const int u = u0 + i * THREADS, row = u / UNITS, unit = u % UNITS;
+                if (row < n64) *reinterpret_cast<u32x4*>(lds + row * ROW + ((unit ^ rows_swz<KS>(row)) << 4)) = v[i];
+            }
+        }
+    } else {
+        constexpr int AHEAD = 3;
+        const int quads = n64 / 4;
+        for (int u0 = threadIdx.x; u0 < quads * UNITS; u0 += THREADS * AHEAD) {
+            uint64_t d[AHEAD][8];
+#pragma unroll
+            for (int i = 0; i < AHEAD; ++i) {
+                const int u = u0 + i * THREADS, c = u % quads * 4, k0 = u / quads * 8;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const int k = k0 + j;
+                    d[i][j] = (c < a.n && k < a.k) ? *reinterpret_cast<const uint64_t*>(a.q + (int64_t)k * a.ldq + c) : 0;
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < AHEAD; ++i) {
+                const int u = u0 + i * THREADS, c = u % quads * 4, unit = u / quads;
+                if (unit >= UNITS) continue;
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    *reinterpret_cast<u32x4*>(lds + (c + j) * ROW + ((unit ^ rows_swz<KS>(c + j)) << 4)) = block_column(reinterpret_cast<const uint32_t*>(d[i]), j);
+            }
+        }
+    }
+    __syncthreads();
+
+    while (t < tiles) {
+        const int64_t m = t * 16 + r;
+        const bool in = m < a.m;
+        frag p[KS];
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+            const int k = ks * 32 + g * 8;
+            p[ks] = next[ks];
+            if (SLOPED) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) p[ks][j] = (T)((float)next[ks][j] * unpack_slope(sl[SLOPED ? ks : 0].v[j]));
+                if (k >= a.k) p[ks] = frag{};
+                else if (in) *reinterpret_cast<frag*>(a.dz + m * a.ldz + k) = p[ks];
+            }
+        }
+        const int64_t here = t;
+        t += stride;
+        for (int n0 = 0; n0 < a.n; n0 += 64) {
+            const int n = n0 + 8 * g;
+            const bool last = n0 + 64 >= a.n;
+            const Pack<T, 8> mine[2] = {res[0], res[1]};
+            if (!last) ask(here, n0 + 64);
+            else if (t < tiles) ask(t, 0);
+            if (EARLY && n0 == 0 && t < tiles) fetch(t);
+            f32x4 acc[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int row = n0 + q_row(i, r);
+                    acc[i] = Mfma<T>::go(*reinterpret_cast<const frag*>(lds + row * ROW + (((ks * 4 + g) ^ rows_swz<KS>(row)) << 4)), p[ks], acc[i]);
+                }
+            if (!EARLY && last && t < tiles) fetch(t);
+            if (!in) continue;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                if (n + 32 * h >= a.n) continue;
+                float v[8], b[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    v[j] = acc[2 * h + (j >> 2)][j & 3];
+                    b[j] = bias[n + 32 * h + j];
+                }
+                finish_with<ACT, T, 8>(a.fin, v, b, mine[h], m, n + 32 * h);
+            }
+        }
+    }
 }
 
 // ---- few rows: the weights stream from memory once, straight into the MFMA's registers ---------------------------
@@ -459,7 +618,7 @@ __global__ __launch_bounds__(256) void act_back_kernel(const T* __restrict__ gy,
     __shared__ float lds[256 * V];
     const int x = threadIdx.x & (tx - 1), y = threadIdx.x / tx, ty = 256 / tx;
     const int64_t lo = (int64_t)blockIdx.x * rows, hi = min(lo + rows, m);
-    for (int c0 = 0; c0 < packs; c0 += tx) {
+    for (int c0 = blockIdx.y * tx; c0 < packs; c0 += gridDim.y * tx) {
         const int c = c0 + x;
         float s[V] = {};
         if (c < packs) {
@@ -566,27 +725,57 @@ static int launch_tile(const TileArgs<T>& a, hipStream_t s) {
         const hipError_t e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
         if (e != hipSuccess) return (int)e;
     }
-    const int per_cu = LDS > 81920 ? 1 : 2;               // workgroups whose LDS (and registers) a CU holds
-    const unsigned blocks = (unsigned)std::min(a.tiles_m * a.tiles_n * a.slices, 256 * per_cu);
-    hipLaunchKernelGGL(kernel, dim3(blocks), dim3(WM * WN * 64), LDS, s, a);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)(a.tiles_m * a.tiles_n * a.slices)), dim3(WM * WN * 64), LDS, s, a);
     return launch_status();
+}
+
+// Q in LDS for the rows kernel: 32-k pieces a row (0: it does not take the product)
+constexpr int64_t ROWS_MIN = 8192, ROWS_LDS = 155648;
+static int rows_fit(int64_t m, int64_t n, int64_t k, int64_t most_k = 512) {
+    if (m < ROWS_MIN || n == 0 || k == 0 || k > most_k) return 0;
+    for (int ks : {2, 4, 8, 12, 16})
+        if (ks * 32 >= k) return (n + 63) / 64 * 64 * (ks * 64 + 4) <= ROWS_LDS ? ks : 0;
+    return 0;
+}
+
+template <typename T, int KS, bool QT, bool SLOPED, int ACT> static int launch_rows(const RowsArgs<T>& a, hipStream_t s) {
+    auto kernel = rows_kernel<T, KS, QT, SLOPED, ACT>;
+    constexpr int THREADS = 512;
+    const int lds = (a.n + 63) / 64 * 64 * (KS * 64 + 4);
+    if (lds > 65536) {
+        const hipError_t e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+        if (e != hipSuccess) return (int)e;
+    }
+    const int64_t tiles = (a.m + 15) / 16;
+    const int64_t blocks = std::min<int64_t>((tiles + THREADS / 64 - 1) / (THREADS / 64), 256);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(THREADS), lds, s, a);
+    return launch_status();
+}
+template <typename T, bool QT, bool SLOPED, int ACT> static int run_rows(int ks, const RowsArgs<T>& a, hipStream_t s) {
+    if (ks == 2) return launch_rows<T, 2, QT, SLOPED, ACT>(a, s);
+    if (ks == 4) return launch_rows<T, 4, QT, SLOPED, ACT>(a, s);
+    if constexpr (!SLOPED) {                 // (deeper with the slopes would not fit the registers: rows_fit's most_k)
+        if (ks == 12) return launch_rows<T, 12, QT, SLOPED, ACT>(a, s);
+        if (ks == 16) return launch_rows<T, 16, QT, SLOPED, ACT>(a, s);
+    }
+    return launch_rows<T, 8, QT, SLOPED, ACT>(a, s);
 }
 
 // C = P Q^T on the tile kernel, with its finish (ACT: the activation of the finish)
 template <typename T, bool PT, bool QT, int ACT>
 static int product(const T* p, int64_t ldp, int64_t plane, const T* q, int64_t ldq, int64_t m, int64_t n, int64_t k, const Finish<T>& fin,
-                   float* partial, hipStream_t s) {
+                   float* partial, hipStream_t s, float* sums = nullptr) {
     const int terms = plane ? 2 : 1;
     const Plan pl = plan_product(m, n, k, terms);
-    TileArgs<T> a{p, q, ldp, ldq, m, n, k, plane, terms, pl.tiles_m, pl.tiles_n, pl.slices, pl.steps, partial, fin};
+    TileArgs<T> a{p, q, ldp, ldq, m, n, k, plane, terms, pl.tiles_m, pl.tiles_n, pl.slices, pl.steps, sums, partial, fin};
     auto cols_ok = [](const T* x, int64_t ld, int64_t cols) { return (uintptr_t)x % 8 == 0 && ld % 4 == 0 && cols % 4 == 0; };
     const bool vec = fin.vec && (PT ? cols_ok(p, ldp, m) : units_ok(p, ldp, k)) && (QT ? cols_ok(q, ldq, n) : units_ok(q, ldq, k));
     if (pl.slices > 1) {
         const int rc = vec ? launch_tile<T, 128, 128, 2, 2, PT, QT, true, PARTIAL>(a, s) : launch_tile<T, 128, 128, 2, 2, PT, QT, false, PARTIAL>(a, s);
         if (rc) return rc;
-        const int v = fin.vec ? 8 : 1;
+        const int v = fin.vec ? 4 : 1;
         const dim3 blocks((unsigned)((m * (n / v) + 63) / 64));
-        if (v == 8) hipLaunchKernelGGL((slices_kernel<T, 8, ACT>), blocks, dim3(256), 0, s, partial, pl.slices, m, n, fin);
+        if (v == 4) hipLaunchKernelGGL((slices_kernel<T, 4, ACT>), blocks, dim3(256), 0, s, partial, pl.slices, m, n, fin);
         else hipLaunchKernelGGL((slices_kernel<T, 1, ACT>), blocks, dim3(256), 0, s, partial, pl.slices, m, n, fin);
         return launch_status();
     }
@@ -622,7 +811,7 @@ static int matrix_check(const void* p, int64_t ld, int64_t rows, int64_t cols) {
 // speak of, while with few elements the rounding of a single one shows in the result
 constexpr int64_t TWO_TERMS = 16384;
 
-struct BackPlan { int64_t dz, plane, ldz, sums, partial, bytes, rows, blocks; };
+struct BackPlan { int64_t dz, plane, ldz, sums, partial, bytes, rows, blocks, slices; };
 static int64_t round256(int64_t b) { return (b + 255) / 256 * 256; }
 static BackPlan back_plan(int64_t m, int64_t n, int64_t k, int act) {
     BackPlan b{};
@@ -634,7 +823,8 @@ static BackPlan back_plan(int64_t m, int64_t n, int64_t k, int act) {
     b.plane = two ? m * b.ldz : 0;
     int64_t at = 0;
     b.dz = at; at += act == PLNLP_ACT_NONE ? 0 : round256(m * b.ldz * 2 * (two ? 2 : 1));
-    b.sums = at; at += round256(b.blocks * n * 4);
+    b.slices = plan_product(n, k, m, two ? 2 : 1).slices;        // of the weights' gradient, which may bring the column sums
+    b.sums = at; at += round256(std::max(b.blocks, b.slices) * n * 4);
     b.partial = at;
     const int terms = two ? 2 : 1;
     at += round256(std::max(plan_bytes(plan_product(m, k, n, terms), m, k), plan_bytes(plan_product(n, k, m, terms), n, k)));
@@ -678,6 +868,11 @@ extern "C" int plnlp_linear_act(const void* x, int64_t ldx, const void* w, int64
             if (m <= 32) return run(few_rows_kernel<T, 2, 8, A>, 8);
             return run(few_rows_kernel<T, 4, 8, A>, 8);
         }
+        const int ks = rows_fit(m, n, k);
+        if (ks && fin.vec && units_ok(x, ldx, k) && units_ok(w, ldw, k)) {
+            const RowsArgs<T> a{(const T*)x, ldx, nullptr, 0, nullptr, 0, (const T*)w, ldw, m, (int)n, (int)k, fin};
+            return run_rows<T, false, false, A>(ks, a, s);
+        }
         if (need && (!workspace || workspace_bytes < need)) return PLNLP_E_WORKSPACE;
         if ((uintptr_t)workspace % 16) return PLNLP_E_ALIGN;
         return product<T, false, false, A>((const T*)x, ldx, 0, (const T*)w, ldw, m, n, k, fin, (float*)workspace, s);
@@ -713,32 +908,44 @@ extern "C" int plnlp_linear_act_backward(const void* gy, int64_t ldg, const int1
         const bool has_act = act != PLNLP_ACT_NONE;
         const T* dz = has_act ? (const T*)(ws + b.dz) : (const T*)gy;
         const int64_t ldz = has_act ? b.ldz : ldg, plane = b.plane;
-        if (m > 0 && n > 0 && (has_act || db)) {
-            const bool vec = units_ok(gy, ldg, n) && (!has_act || units_ok(slope, lds, n));
+        float* sums = (float*)(ws + b.sums);
+        float* partial = (float*)(ws + b.partial);
+        const bool want_dx = dx && m > 0 && k > 0, want_dw = dw && n > 0 && k > 0;
+        const bool vec = units_ok(gy, ldg, n) && (!has_act || units_ok(slope, lds, n));
+        // many rows and weights that fit LDS: dz is formed on the way to dx, its column sums come with dw
+        const Finish<T> fin_x = make_finish<T>(nullptr, nullptr, 0, nullptr, 0, dx, lddx, k);
+        const int ks = want_dx && vec && !plane && fin_x.vec && (uintptr_t)w % 8 == 0 && ldw % 4 == 0 ? rows_fit(m, k, n, has_act ? 256 : 512) : 0;
+        const bool sums_in_dw = ks && want_dw;
+        int64_t sum_blocks = m > 0 ? b.blocks : 0;
+        if (m > 0 && n > 0 && ((has_act && !ks) || (db && !sums_in_dw))) {
             const int64_t packs = vec ? n / 8 : n;
             int tx = 1;
             while (tx < 64 && tx < packs) tx <<= 1;
             auto run = [&](auto kernel) {
-                hipLaunchKernelGGL(kernel, dim3((unsigned)b.blocks), dim3(256), 0, s, (const T*)gy, ldg, slope, lds, (T*)(ws + b.dz), ldz, plane, m,
-                                   (int)packs, tx, b.rows, db ? (float*)(ws + b.sums) : nullptr);
+                const unsigned slabs = (unsigned)std::min<int64_t>((packs + tx - 1) / tx, 64);
+                hipLaunchKernelGGL(kernel, dim3((unsigned)b.blocks, slabs), dim3(256), 0, s, (const T*)gy, ldg, slope, lds, (T*)(ws + b.dz), ldz, plane, m,
+                                   (int)packs, tx, b.rows, db ? sums : nullptr);
                 return launch_status();
             };
             const int e = has_act ? (vec ? run(act_back_kernel<T, 8, true>) : run(act_back_kernel<T, 1, true>))
                                   : (vec ? run(act_back_kernel<T, 8, false>) : run(act_back_kernel<T, 1, false>));
             if (e) return e;
         }
-        if (db && n > 0) {
-            hipLaunchKernelGGL((col_join_kernel<T>), dim3((unsigned)((n + 15) / 16)), dim3(1024), 0, s, (const float*)(ws + b.sums), (int)(m > 0 ? b.blocks : 0), n, (T*)db);
-            if (int e = launch_status()) return e;
+        if (ks) {
+            const RowsArgs<T> a{(const T*)gy, ldg, slope, lds, (T*)(ws + b.dz), ldz, (const T*)w, ldw, m, (int)k, (int)n, fin_x};
+            if (int e = has_act ? run_rows<T, true, true, PLNLP_ACT_NONE>(ks, a, s) : run_rows<T, true, false, PLNLP_ACT_NONE>(ks, a, s)) return e;
+        } else if (want_dx) {
+            if (int e = product<T, false, true, PLNLP_ACT_NONE>(dz, ldz, plane, (const T*)w, ldw, m, k, n, fin_x, partial, s)) return e;
         }
-        float* partial = (float*)(ws + b.partial);
-        if (dx && m > 0 && k > 0) {
-            const Finish<T> fin = make_finish<T>(nullptr, nullptr, 0, nullptr, 0, dx, lddx, k);
-            if (int e = product<T, false, true, PLNLP_ACT_NONE>(dz, ldz, plane, (const T*)w, ldw, m, k, n, fin, partial, s)) return e;
-        }
-        if (dw && n > 0 && k > 0) {
+        if (want_dw) {
             const Finish<T> fin = make_finish<T>(nullptr, nullptr, 0, nullptr, 0, dw, lddw, k);
-            if (int e = product<T, true, true, PLNLP_ACT_NONE>(dz, ldz, plane, (const T*)x, ldx, n, k, m, fin, partial, s)) return e;
+            if (sums_in_dw) sum_blocks = b.slices;
+            if (int e = product<T, true, true, PLNLP_ACT_NONE>(dz, ldz, plane, (const T*)x, ldx, n, k, m, fin, partial, s,
+                                                               sums_in_dw && db ? sums : nullptr)) return e;
+        }
+        if (db && n > 0) {
+            hipLaunchKernelGGL((col_join_kernel<T>), dim3((unsigned)((n + 15) / 16)), dim3(1024), 0, s, (const float*)sums, (int)sum_blocks, n, (T*)db);
+            if (int e = launch_status()) return e;
         }
         return 0;
     });

@@ -239,6 +239,9 @@ def check_linear(P, x, w, b, r, gy, act, dtype):
 LINEAR_SHAPES = [(1, 1, 1), (1, 16, 64), (1, 200, 4096), (3, 17, 72), (16, 256, 256), (17, 40, 1024), (32, 8, 8), (33, 136, 520), (64, 128, 128),
                  (65, 128, 128), (100, 64, 64), (128, 128, 64), (129, 130, 65), (300, 520, 8), (257, 72, 2056), (777, 515, 130), (5, 515, 1003),
                  (1500, 200, 200), (4000, 24, 48)]
+# many rows and weights that fit LDS: full and ragged groups of 64 columns, K of whole and ragged 32-pieces up to the deepest taken
+# (and the first that is not), rows that end inside a group of 16; the last two fall back for their strides and widths
+MANY_ROWS = [(8192, 256, 256), (8200, 200, 72), (10007, 8, 8), (9000, 136, 264), (8195, 64, 512), (8192, 264, 96), (8300, 512, 64), (8300, 72, 520), (8201, 40, 36), (8209, 33, 64)]
 
 
 @gpu
@@ -247,6 +250,28 @@ LINEAR_SHAPES = [(1, 1, 1), (1, 16, 64), (1, 200, 4096), (3, 17, 72), (16, 256, 
 def test_linear_shapes(P, m, n, k, dtype):
     act = ("gelu", "silu", "none", "gelu_tanh")[(m + n + k) % 4]
     check_linear(P, *linear_case(P, m, n, k, dtype, act, True, True), act, dtype)
+
+
+@gpu
+@pytest.mark.parametrize("m,n,k", MANY_ROWS)
+@pytest.mark.parametrize("dtype,act,pad", [(BF16, "gelu", 0), (F16, "silu", 8), (BF16, "none", 0), (F16, "gelu_tanh", 3)])
+def test_linear_many_rows(P, m, n, k, dtype, act, pad):
+    check_linear(P, *linear_case(P, m, n, k, dtype, act, True, (m + pad) % 2 == 0, pad), act, dtype)
+
+
+@gpu
+def test_linear_many_rows_some_gradients(P):
+    """each gradient alone: which of them brings the others' sums differs"""
+    x, w, b, r, gy = linear_case(P, 8500, 96, 64, BF16, "silu", True, True)
+    full = torch.autograd.grad(P.linear_act(x, w, b, residual=r, activation="silu"), [x, w, b, r], gy)
+    for i, leaf in enumerate((x, w, b, r)):
+        args = [t if j == i else t.detach() for j, t in enumerate((x, w, b, r))]
+        got, = torch.autograd.grad(P.linear_act(*args[:3], residual=args[3], activation="silu"), [leaf], gy)
+        if i == 2:        # summed from dz before it is rounded here, after it there: u of each term
+            slack = U[BF16] * (gy.double().abs() * 1.1).sum(0) + U[BF16] * full[2].double().abs()
+            within(got, full[2].double(), slack)
+        else:
+            assert torch.equal(got, full[i])
 
 
 @gpu
