@@ -16,6 +16,11 @@ inline int dtype_size(int d) { return d == PLNLP_DTYPE_F32 ? 4 : 2; }
 // V consecutive elements as one access (V * sizeof(T) bytes, at most 16 per load instruction; aligned to that)
 template <typename T, int V> struct alignas(V * sizeof(T) > 16 ? 16 : V * sizeof(T)) Pack { T v[V]; };
 
+// the same at any alignment of whole elements (global memory takes it, at a part of the rate where rows straddle lines)
+template <typename T, int V> struct __attribute__((packed, aligned(sizeof(T)))) LoosePack { T v[V]; };
+template <typename T, int V, bool LOOSE> struct PackOf { typedef Pack<T, V> type; };
+template <typename T, int V> struct PackOf<T, V, true> { typedef LoosePack<T, V> type; };
+
 template <typename T, int V> __device__ __forceinline__ void load_f32(const T* p, float (&x)[V]) {
     const Pack<T, V> k = *reinterpret_cast<const Pack<T, V>*>(p);
 #pragma unroll

@@ -110,30 +110,35 @@ template <typename T> struct Finish {
 };
 constexpr int PARTIAL = -1; // in the place of an activation: the sum is one K slice's, stored as it is
 
-// V consecutive columns of row m from column n on (all inside the matrix); b = the bias there, res = the residual there (if f.res)
-template <int ACT, typename T, int V>
-__device__ __forceinline__ void finish_with(const Finish<T>& f, float (&v)[V], const float (&b)[V], const Pack<T, V>& res, int64_t m, int64_t n) {
+// V consecutive columns of row m from column n on (all inside the matrix); b = the bias there, res = the residual there (if f.res).
+// LOOSE: at any alignment
+template <int ACT, bool LOOSE, typename T, int V>
+__device__ __forceinline__ void finish_with(const Finish<T>& f, float (&v)[V], const float (&b)[V], const typename PackOf<T, V, LOOSE>::type& res,
+                                            int64_t m, int64_t n) {
 #pragma unroll
     for (int j = 0; j < V; ++j) v[j] += b[j];
     float s[V];
     if (ACT != PLNLP_ACT_NONE && f.slope) {
-        Pack<int16_t, V> q;
+        typedef typename PackOf<int16_t, V, LOOSE>::type P;
+        P q;
 #pragma unroll
         for (int j = 0; j < V; ++j) { v[j] = act_of<ACT, true>(v[j], s[j]); q.v[j] = pack_slope(s[j]); }
-        *reinterpret_cast<Pack<int16_t, V>*>(f.slope + m * f.ldp + n) = q;
+        *reinterpret_cast<P*>(f.slope + m * f.ldp + n) = q;
     } else
 #pragma unroll
         for (int j = 0; j < V; ++j) v[j] = act_of<ACT, false>(v[j], s[j]);
-    if (f.res)
+    typedef typename PackOf<T, V, LOOSE>::type P;
+    P o;
 #pragma unroll
-        for (int j = 0; j < V; ++j) v[j] += (float)res.v[j];
-    store_f32<T, V>(f.out + m * f.ldo + n, v);
+    for (int j = 0; j < V; ++j) o.v[j] = (T)(f.res ? v[j] + (float)res.v[j] : v[j]);
+    *reinterpret_cast<P*>(f.out + m * f.ldo + n) = o;
 }
-template <int ACT, typename T, int V>
+template <int ACT, bool LOOSE, typename T, int V>
 __device__ __forceinline__ void finish_cols(const Finish<T>& f, float (&v)[V], const float (&b)[V], int64_t m, int64_t n) {
-    Pack<T, V> res;
-    if (f.res) res = *reinterpret_cast<const Pack<T, V>*>(f.res + m * f.ldr + n);
-    finish_with<ACT, T, V>(f, v, b, res, m, n);
+    typedef typename PackOf<T, V, LOOSE>::type P;
+    P res;
+    if (f.res) res = *reinterpret_cast<const P*>(f.res + m * f.ldr + n);
+    finish_with<ACT, LOOSE, T, V>(f, v, b, res, m, n);
 }
 
 // ---- the tile kernel --------------------------------------------------------------------------------------------
@@ -158,60 +163,6 @@ __device__ __forceinline__ int swz(int r) { return ((r >> 1) & 1) ^ (((r >> 3) &
 // tiles 2h and 2h + 1 are eight consecutive columns, and the four groups' stores 64 consecutive bytes
 __device__ __forceinline__ int q_row(int t, int r) { return 32 * (t >> 1) + 8 * (r >> 2) + 4 * (t & 1) + (r & 3); }
 
-// registers of one operand's tile (R rows x BK), one thread's share
-template <int R, int THREADS> struct Stage { u32x4 r[R * 8 / THREADS]; };
-
-template <typename T, bool VEC> __device__ __forceinline__ u32x4 load_unit(const T* p, int valid) {     // 8 elements, `valid` of them real
-    if (VEC) return *reinterpret_cast<const u32x4*>(p);
-    union { T t[8]; u32x4 u; } x;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) x.t[j] = j < valid ? p[j] : (T)0.f;
-    return x.u;
-}
-
-// rows r0 .. r0 + R of an operand with k contiguous (`base` = its element (r0, k0)); rows past `rows` repeat the last (their results are
-// not stored), k past `left` reads as zero
-template <typename T, int R, int THREADS, bool VEC>
-__device__ __forceinline__ void fetch_rows(Stage<R, THREADS>& s, const T* base, int64_t ld, int rows, int64_t left) {
-#pragma unroll
-    for (int i = 0; i < R * 8 / THREADS; ++i) {
-        const int unit = threadIdx.x + i * THREADS, row = min(unit >> 3, rows - 1), k = (unit & 7) * 8;
-        const T* p = base + (int64_t)row * ld;
-        if (left >= BK) s.r[i] = load_unit<T, VEC>(p + k, 8);
-        else {
-            const int valid = (int)min(left - k, (int64_t)8);
-            s.r[i] = valid > 0 ? load_unit<T, VEC>(p + k, valid) : u32x4{0, 0, 0, 0};
-        }
-    }
-}
-template <int R, int THREADS> __device__ __forceinline__ void store_rows(const Stage<R, THREADS>& s, char* lds) {
-#pragma unroll
-    for (int i = 0; i < R * 8 / THREADS; ++i) {
-        const int unit = threadIdx.x + i * THREADS, row = unit >> 3, u = unit & 7;
-        *reinterpret_cast<u32x4*>(lds + row * 128 + ((u ^ swz(row)) << 4)) = s.r[i];
-    }
-}
-
-// the same tile of an operand with k along its rows (`base` = its element (k0, r0), ld between k's): 8 k x 4 columns a thread
-template <typename T, int R, int THREADS, bool VEC>
-__device__ __forceinline__ void fetch_cols(Stage<R, THREADS>& s, const T* base, int64_t ld, int cols, int64_t left) {
-    static_assert(R * 2 == THREADS, "one 8 x 4 block a thread");
-    const int c = (threadIdx.x % (R / 4)) * 4, g = threadIdx.x / (R / 4);
-    uint64_t* d = reinterpret_cast<uint64_t*>(s.r);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const int k = g * 8 + i;
-        if (VEC) {
-            const T* p = base + min(c, cols - 4);          // (columns are whole groups of four here)
-            d[i] = k < left ? *reinterpret_cast<const uint64_t*>(p + (int64_t)k * ld) : 0;
-        } else {
-            union { T t[4]; uint64_t u; } x;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) x.t[j] = (k < left && c + j < cols) ? base[(int64_t)k * ld + c + j] : (T)0.f;
-            d[i] = x.u;
-        }
-    }
-}
 // column j of an 8 k x 4 columns block held as eight rows of two words: its eight k
 __device__ __forceinline__ u32x4 block_column(const uint32_t* d, int j) {
     u32x4 o;
@@ -222,14 +173,105 @@ __device__ __forceinline__ u32x4 block_column(const uint32_t* d, int j) {
     }
     return o;
 }
-template <int R, int THREADS> __device__ __forceinline__ void store_cols(const Stage<R, THREADS>& s, char* lds) {
-    const int c = (threadIdx.x % (R / 4)) * 4, g = threadIdx.x / (R / 4);
-    const uint32_t* d = reinterpret_cast<const uint32_t*>(s.r);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) *reinterpret_cast<u32x4*>(lds + (c + j) * 128 + ((g ^ swz(c + j)) << 4)) = block_column(d, j);
-}
 
-template <typename T, int BM, int BN, int WM, int WN, bool PT, bool QT, bool VEC, int ACT>
+// How an operand's tile is read: element by element (any matrix), 16 bytes at any alignment (k >= BK), or 16 bytes at a time through a
+// buffer descriptor (16-byte aligned rows of whole units)
+enum { BY_ELEMENT = 0, LOOSELY = 1, ALIGNED = 2 };
+
+// One operand's tile of R rows x BK on its way to LDS: this thread's share.  Every step issues the same loads, whatever the matrix's
+// edges: rows past the last repeat it (their results are not stored); the last step of a k that is no multiple of BK begins early,
+// and what it reads twice is cleared on the way to LDS.
+template <typename T, int R, int THREADS, bool COLS, int MODE> struct Operand {
+    static constexpr int N = R * 8 / THREADS;
+    u32x4 reg[N];
+    uint32_t off[COLS ? 1 : N];            // ALIGNED: bytes from the tile's (uniform) first element
+    int skip, valid;                       // of the step in reg: k in [skip, valid) are real and not read before
+
+    static __device__ __forceinline__ int row_of(int i) { return (int)(threadIdx.x + i * THREADS) >> 3; }
+    static __device__ __forceinline__ int unit() { return threadIdx.x & 7; }
+    static __device__ __forceinline__ int col() { return (int)(threadIdx.x % (R / 4)) * 4; }          // COLS: 8 k x 4 columns a thread
+    static __device__ __forceinline__ int group() { return (int)threadIdx.x / (R / 4); }
+
+    // rows: of the tile inside the matrix; k: the matrix's depth (COLS: at least BK unless BY_ELEMENT)
+    __device__ __forceinline__ void begin(int64_t ld, int rows, int64_t k) {
+        static_assert(!COLS || R * 2 == THREADS, "one 8 x 4 block a thread");
+        if (MODE != ALIGNED) return;
+        if (COLS) off[0] = (uint32_t)((int64_t)(group() * 8) * ld + min(col(), rows - 4)) * 2;        // (whole groups of four columns)
+        else
+#pragma unroll
+            for (int i = 0; i < N; ++i) off[COLS ? 0 : i] = (uint32_t)(min(row_of(i), rows - 1) * ld + min((int64_t)unit() * 8, k - 8)) * 2;
+    }
+    // `base`: the tile's element at depth k0
+    __device__ __forceinline__ void fetch(const T* base, int64_t ld, int rows, int64_t k0, int64_t k) {
+        const int left = (int)min(k - k0, (int64_t)BK), back = MODE != BY_ELEMENT && k >= BK ? BK - left : 0;
+        skip = back;
+        valid = left + back;
+        base -= COLS ? back * ld : back;
+        // (a buffer descriptor of the step's first element: the loads then take one 32-bit register of addresses each)
+        const auto at = __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, -1, 0x00027000);
+        if (COLS) {
+            uint64_t* d = reinterpret_cast<uint64_t*>(reg);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int kk = group() * 8 + i;
+                if (MODE == ALIGNED) d[i] = __builtin_bit_cast(uint64_t, __builtin_amdgcn_raw_buffer_load_b64(at, off[0], (int)(i * ld * 2), 0));
+                else if (MODE == LOOSELY)
+                    d[i] = __builtin_bit_cast(uint64_t, *reinterpret_cast<const LoosePack<T, 4>*>(base + kk * ld + min(col(), rows - 4)));
+                else {
+                    union { T t[4]; uint64_t u; } x;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) x.t[j] = (kk < left && col() + j < rows) ? base[kk * ld + col() + j] : (T)0.f;
+                    d[i] = x.u;
+                }
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const T* row = base + min(row_of(i), rows - 1) * ld;
+                if (MODE == ALIGNED) reg[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(at, off[COLS ? 0 : i], 0, 0));
+                else if (MODE == LOOSELY) reg[i] = __builtin_bit_cast(u32x4, *reinterpret_cast<const LoosePack<T, 8>*>(row + unit() * 8));
+                else {
+                    union { T t[8]; u32x4 u; } x;
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) x.t[j] = unit() * 8 + j < left ? row[unit() * 8 + j] : (T)0.f;
+                    reg[i] = x.u;
+                }
+            }
+        }
+    }
+    // into LDS rows of 128 bytes
+    __device__ __forceinline__ void store(char* lds, int rows) {
+        if (COLS) {
+            uint64_t* d = reinterpret_cast<uint64_t*>(reg);
+            if (MODE != BY_ELEMENT && (skip > 0 || valid < BK))
+#pragma unroll
+                for (int i = 0; i < 8; ++i) if (group() * 8 + i < skip || group() * 8 + i >= valid) d[i] = 0;
+            if (MODE == LOOSELY && (rows & 3)) {          // the last block of columns was read up to three columns early
+                const int early = min(max(col() - (rows - 4), 0), 3);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) d[i] >>= 16 * early;
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                *reinterpret_cast<u32x4*>(lds + (col() + j) * 128 + ((group() ^ swz(col() + j)) << 4)) = block_column(reinterpret_cast<const uint32_t*>(reg), j);
+        } else {
+            if (MODE != BY_ELEMENT && (skip > 0 || valid < BK)) {
+                const int lo = skip - unit() * 8, hi = valid - unit() * 8;      // elements [lo, hi) of the unit stay
+#pragma unroll
+                for (int h = 0; h < 4; ++h) {
+                    const uint32_t keep = (2 * h >= lo && 2 * h < hi ? 0xffffu : 0u) | (2 * h + 1 >= lo && 2 * h + 1 < hi ? 0xffff0000u : 0u);
+#pragma unroll
+                    for (int i = 0; i < N; ++i) reg[i][h] &= keep;
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+                *reinterpret_cast<u32x4*>(lds + row_of(i) * 128 + ((unit() ^ swz(row_of(i))) << 4)) = reg[i];
+        }
+    }
+};
+
+template <typename T, int BM, int BN, int WM, int WN, bool PT, bool QT, int MODE, int ACT>
 __global__ __launch_bounds__(WM * WN * 64, 2) void tile_kernel(TileArgs<T> a) {
     constexpr int THREADS = WM * WN * 64, TM = BM / WM / 16;         // 16-row pieces of a wave's part; it is 64 columns wide
     static_assert(BN / WN == 64, "a wave covers 64 columns");
@@ -270,50 +312,95 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void tile_kernel(TileArgs<T> a) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) ones[j] = (T)1.f;
 
-    Stage<BM, THREADS> sp;
-    Stage<BN, THREADS> sq;
-    auto fetch = [&](int step) {
-        const int at = first + step, term = at >= term_steps;
-        const int64_t k = (int64_t)(at - (term ? term_steps : 0)) * BK, left = a.k - k;
+    Operand<T, BM, THREADS, PT, MODE> sp;
+    Operand<T, BN, THREADS, QT, MODE> sq;
+    if (steps > 0) { sp.begin(a.ldp, rows_p, a.k); sq.begin(a.ldq, rows_q, a.k); }
+    // (a step past the last fetches the last again: the loads in flight at any point are the same in every step)
+    auto fetch_p = [&](int step) {
+        const int at = first + min(step, steps - 1), term = at >= term_steps;
+        const int64_t k = (int64_t)(at - (term ? term_steps : 0)) * BK;
         const T* p = a.p + (term ? a.plane : 0);
-        if (PT) fetch_cols<T, BM, THREADS, VEC>(sp, p + k * a.ldp + m0, a.ldp, rows_p, left);
-        else fetch_rows<T, BM, THREADS, VEC>(sp, p + m0 * a.ldp + k, a.ldp, rows_p, left);
-        if (QT) fetch_cols<T, BN, THREADS, VEC>(sq, a.q + k * a.ldq + n0, a.ldq, rows_q, left);
-        else fetch_rows<T, BN, THREADS, VEC>(sq, a.q + n0 * a.ldq + k, a.ldq, rows_q, left);
+        sp.fetch(PT ? p + k * a.ldp + m0 : p + m0 * a.ldp + k, a.ldp, rows_p, k, a.k);
     };
-    auto stage = [&](int buf) {
-        char* b = lds + buf * BUF;
-        if (PT) store_cols<BM, THREADS>(sp, b); else store_rows<BM, THREADS>(sp, b);
-        if (QT) store_cols<BN, THREADS>(sq, b + BM * 128); else store_rows<BN, THREADS>(sq, b + BM * 128);
+    auto fetch_q = [&](int step) {
+        const int at = first + min(step, steps - 1);
+        const int64_t k = (int64_t)(at - (at >= term_steps ? term_steps : 0)) * BK;
+        sq.fetch(QT ? a.q + k * a.ldq + n0 : a.q + n0 * a.ldq + k, a.ldq, rows_q, k, a.k);
+    };
+    auto stage_p = [&](int buf) { sp.store(lds + buf * BUF, rows_p); };
+    auto stage_q = [&](int buf) { sq.store(lds + buf * BUF + BM * 128, rows_q); };
+    auto q_frag = [&](const char* b, int ks, int t) {
+        const int row = wn + q_row(t, r);
+        return *reinterpret_cast<const frag*>(b + (BM + row) * 128 + (((ks * 4 + g) ^ swz(row)) << 4));
+    };
+    auto p_frag = [&](const char* b, int ks, int i) {
+        const int row = wm + i * 16 + r;
+        return *reinterpret_cast<const frag*>(b + row * 128 + (((ks * 4 + g) ^ swz(row)) << 4));
     };
     if (steps > 0) {
-        fetch(0);
-        stage(0);
-        if (steps > 1) fetch(1);
+        fetch_p(0);
+        fetch_q(0);
+        stage_p(0);
+        stage_q(0);
+        fetch_p(1);
+        fetch_q(1);
         __syncthreads();
     }
-    for (int step = 0; step < steps; ++step) {
-        const char* b = lds + (step & 1) * BUF;
-        if (step + 1 < steps) stage((step + 1) & 1);      // the other buffer was read before the barrier that ended the last step
-        if (step + 2 < steps) fetch(step + 2);            // a whole step to arrive in
+    if constexpr (BM == 256) {
+        // Two waves a SIMD, half a step apart: while waves 0..3 multiply (32 MFMAs, 512 clocks), waves 4..7 read their next fragments and
+        // move the next tile, and the other way round; a barrier ends each half.  With both in step all of them waited for LDS at
+        // the same time (8192 x 4096 x 4096: 334 us).  A step's buffer is read in halves 4 s (waves 0..3) to 4 s + 3 (waves 4..7), the
+        // other one written in those same halves.  Every wave passes 4 barriers a step and one more, the later half before, the
+        // earlier half after.
+        const bool later = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) >= WM * WN / 2;
+        if (later) __syncthreads();
+        for (int step = 0; step < steps; ++step) {
+            const char* b = lds + (step & 1) * BUF;
 #pragma unroll
-        for (int ks = 0; ks < BK / 32; ++ks) {
-            frag q[4];
+            for (int ks = 0; ks < 2; ++ks) {
+                frag p[TM], q[4];
 #pragma unroll
-            for (int t = 0; t < 4; ++t) {
-                const int row = wn + q_row(t, r);
-                q[t] = *reinterpret_cast<const frag*>(b + (BM + row) * 128 + (((ks * 4 + g) ^ swz(row)) << 4));
-            }
+                for (int t = 0; t < 4; ++t) q[t] = q_frag(b, ks, t);
 #pragma unroll
-            for (int i = 0; i < TM; ++i) {
-                const int row = wm + i * 16 + r;
-                const frag p = *reinterpret_cast<const frag*>(b + row * 128 + (((ks * 4 + g) ^ swz(row)) << 4));
+                for (int i = 0; i < TM; ++i) p[i] = p_frag(b, ks, i);
+                if (ks == 0) { stage_p((step + 1) & 1); fetch_p(step + 2); }
+                else { stage_q((step + 1) & 1); fetch_q(step + 2); }
+                __syncthreads();
+                __builtin_amdgcn_sched_barrier(0);
+                __builtin_amdgcn_s_setprio(1);
 #pragma unroll
-                for (int t = 0; t < 4; ++t) acc[i][t] = Mfma<T>::go(q[t], p, acc[i][t]);
-                if (SUMS) if (sum_p) psum[SUMS ? i : 0] = Mfma<T>::go(ones, p, psum[SUMS ? i : 0]);
+                for (int i = 0; i < TM; ++i)
+#pragma unroll
+                    for (int t = 0; t < 4; ++t) acc[i][t] = Mfma<T>::go(q[t], p[i], acc[i][t]);
+                __builtin_amdgcn_s_setprio(0);
+                __builtin_amdgcn_sched_barrier(0);
+                __syncthreads();
             }
         }
-        __syncthreads();
+        if (!later) __syncthreads();
+    } else {
+        for (int step = 0; step < steps; ++step) {
+            const char* b = lds + (step & 1) * BUF;
+            // (the other buffer was read before the barrier that ended the last step; what is fetched has a whole step to arrive in)
+            stage_p((step + 1) & 1);
+            stage_q((step + 1) & 1);
+            fetch_p(step + 2);
+            fetch_q(step + 2);
+#pragma unroll
+            for (int ks = 0; ks < BK / 32; ++ks) {
+                frag q[4];
+#pragma unroll
+                for (int t = 0; t < 4; ++t) q[t] = q_frag(b, ks, t);
+#pragma unroll
+                for (int i = 0; i < TM; ++i) {
+                    const frag p = p_frag(b, ks, i);
+#pragma unroll
+                    for (int t = 0; t < 4; ++t) acc[i][t] = Mfma<T>::go(q[t], p, acc[i][t]);
+                    if (SUMS) if (sum_p) psum[SUMS ? i : 0] = Mfma<T>::go(ones, p, psum[SUMS ? i : 0]);
+                }
+            }
+            __syncthreads();
+        }
     }
 
     if (SUMS && sum_p && g == 0) {
@@ -341,28 +428,29 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void tile_kernel(TileArgs<T> a) {
         for (int h = 0; h < 2; ++h) {
             const int64_t col = n + 32 * h;
             if (cols[h] <= 0) continue;
+            float v[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = acc[i][2 * h + (j >> 2)][j & 3];
             if constexpr (ACT == PARTIAL) {
                 float* o = a.partial + ((int64_t)slice * a.m + m) * a.n + col;
+                if (MODE == ALIGNED) store_f32<float, 8>(o, v);      // (n is whole groups of eight)
+                else if (cols[h] == 8) {
+                    LoosePack<float, 8> q;
 #pragma unroll
-                for (int t = 0; t < 2; ++t) {
-                    if (VEC) *reinterpret_cast<f32x4*>(o + 4 * t) = acc[i][2 * h + t];      // (n is whole groups of eight)
-                    else
+                    for (int j = 0; j < 8; ++j) q.v[j] = v[j];
+                    *reinterpret_cast<LoosePack<float, 8>*>(o) = q;
+                } else
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) if (4 * t + j < cols[h]) o[4 * t + j] = acc[i][2 * h + t][j];
+                    for (int j = 0; j < 8; ++j) if (j < cols[h]) o[j] = v[j];
+            } else if (MODE == ALIGNED) finish_cols<ACT, false, T, 8>(a.fin, v, bias[h], m, col);
+            else if (cols[h] == 8) finish_cols<ACT, true, T, 8>(a.fin, v, bias[h], m, col);
+            else
+                for (int j = 0; j < cols[h]; ++j) {
+                    float x[1] = {v[0]}, y[1] = {bias[h][0]};
+#pragma unroll
+                    for (int c = 1; c < 8; ++c) if (c == j) { x[0] = v[c]; y[0] = bias[h][c]; }
+                    finish_cols<ACT, true, T, 1>(a.fin, x, y, m, col + j);
                 }
-            } else if constexpr (VEC) {
-                float v[8];
-#pragma unroll
-                for (int j = 0; j < 8; ++j) v[j] = acc[i][2 * h + (j >> 2)][j & 3];
-                finish_cols<ACT, T, 8>(a.fin, v, bias[h], m, col);
-            } else {
-#pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    if (j < cols[h]) {
-                        float v[1] = {acc[i][2 * h + (j >> 2)][j & 3]}, b[1] = {bias[h][j]};
-                        finish_cols<ACT, T, 1>(a.fin, v, b, m, col + j);
-                    }
-            }
         }
     }
 }
@@ -396,7 +484,7 @@ __global__ __launch_bounds__(256) void slices_kernel(const float* __restrict__ p
     if (fin.bias)
 #pragma unroll
         for (int j = 0; j < V; ++j) b[j] = (float)fin.bias[col + j];
-    finish_cols<ACT, T, V>(fin, v, b, row, col);
+    finish_cols<ACT, V == 1, T, V>(fin, v, b, row, col);
 }
 
 // ---- many rows, a Q that fits LDS: Q stays there, P streams through registers -----------------------------------------
@@ -544,17 +632,30 @@ __global__ __launch_bounds__(512) void rows_kernel(RowsArgs<T> a) {
                     v[j] = acc[2 * h + (j >> 2)][j & 3];
                     b[j] = bias[n + 32 * h + j];
                 }
-                finish_with<ACT, T, 8>(a.fin, v, b, mine[h], m, n + 32 * h);
+                finish_with<ACT, false, T, 8>(a.fin, v, b, mine[h], m, n + 32 * h);
             }
         }
     }
 }
 
 // ---- few rows: the weights stream from memory once, straight into the MFMA's registers ---------------------------
+// eight consecutive k of a row of which `left` remain
+template <typename T, bool LOOSE> __device__ __forceinline__ typename Mfma<T>::frag few_unit(const T* p, int64_t left) {
+    typedef typename Mfma<T>::frag frag;
+    frag v = {};
+    if (!LOOSE) {
+        if (left > 0) v = *reinterpret_cast<const frag*>(p);
+    } else if (left >= 8) v = __builtin_bit_cast(frag, *reinterpret_cast<const LoosePack<T, 8>*>(p));
+    else if (left > 0)
+#pragma unroll
+        for (int j = 0; j < 7; ++j) if (j < left) v[j] = p[j];
+    return v;
+}
+
 // A workgroup owns 16 columns of y and all (<= 16 * TM) rows; its waves share K, 64 at a time.  A lane reads 32 consecutive bytes of
 // a weight row (the four lanes of a row 128): which k a lane holds is free as long as x is read the same way.  The waves'
 // sums meet in LDS and are added in wave order.
-template <typename T, int TM, int WAVES, int ACT>
+template <typename T, int TM, int WAVES, bool LOOSE, int ACT>
 __global__ __launch_bounds__(WAVES * 64) void few_rows_kernel(const T* __restrict__ x, int64_t ldx, const T* __restrict__ w, int64_t ldw, int m,
                                                               int64_t n, int64_t k, Finish<T> fin) {
     typedef typename Mfma<T>::frag frag;
@@ -577,11 +678,10 @@ __global__ __launch_bounds__(WAVES * 64) void few_rows_kernel(const T* __restric
             const int64_t at = (u0 + j * WAVES) * 64;
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const bool in = at + g * 16 + h * 8 < k;   // (k is whole groups of eight)
-                const frag zero = {};
-                a[j][h] = in ? *reinterpret_cast<const frag*>(wr + at + h * 8) : zero;
+                const int64_t left = k - (at + g * 16 + h * 8);           // (whole groups of eight unless LOOSE)
+                a[j][h] = few_unit<T, LOOSE>(wr + at + h * 8, left);
 #pragma unroll
-                for (int i = 0; i < TM; ++i) b[j][i][h] = in ? *reinterpret_cast<const frag*>(xr[i] + at + h * 8) : zero;
+                for (int i = 0; i < TM; ++i) b[j][i][h] = few_unit<T, LOOSE>(xr[i] + at + h * 8, left);
             }
         }
 #pragma unroll
@@ -604,7 +704,7 @@ __global__ __launch_bounds__(WAVES * 64) void few_rows_kernel(const T* __restric
         for (int s = 0; s < WAVES; ++s) v[0] += part[s][i][row][c];
         if (mm >= m || nn >= n) continue;
         if (fin.bias) b[0] = (float)fin.bias[nn];
-        finish_cols<ACT, T, 1>(fin, v, b, mm, nn);
+        finish_cols<ACT, true, T, 1>(fin, v, b, mm, nn);
     }
 }
 
@@ -717,9 +817,9 @@ static Plan plan_product(int64_t m, int64_t n, int64_t k, int terms = 1) {
 }
 static int64_t plan_bytes(const Plan& p, int64_t m, int64_t n) { return p.slices > 1 ? (int64_t)p.slices * m * n * 4 : 0; }
 
-template <typename T, int BM, int BN, int WM, int WN, bool PT, bool QT, bool VEC, int ACT>
+template <typename T, int BM, int BN, int WM, int WN, bool PT, bool QT, int MODE, int ACT>
 static int launch_tile(const TileArgs<T>& a, hipStream_t s) {
-    auto kernel = tile_kernel<T, BM, BN, WM, WN, PT, QT, VEC, ACT>;
+    auto kernel = tile_kernel<T, BM, BN, WM, WN, PT, QT, MODE, ACT>;
     constexpr int LDS = 2 * (BM + BN) * 128;
     if (LDS > 65536) {
         const hipError_t e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
@@ -769,19 +869,28 @@ static int product(const T* p, int64_t ldp, int64_t plane, const T* q, int64_t l
     const Plan pl = plan_product(m, n, k, terms);
     TileArgs<T> a{p, q, ldp, ldq, m, n, k, plane, terms, pl.tiles_m, pl.tiles_n, pl.slices, pl.steps, sums, partial, fin};
     auto cols_ok = [](const T* x, int64_t ld, int64_t cols) { return (uintptr_t)x % 8 == 0 && ld % 4 == 0 && cols % 4 == 0; };
-    const bool vec = fin.vec && (PT ? cols_ok(p, ldp, m) : units_ok(p, ldp, k)) && (QT ? cols_ok(q, ldq, n) : units_ok(q, ldq, k));
+    // (32-bit offsets inside a tile; an operand with k along its rows needs a whole step of them)
+    int mode = BY_ELEMENT;
+    if (fin.vec && ldp < ((int64_t)1 << 22) && ldq < ((int64_t)1 << 22) && (k >= BK || !(PT || QT)) && k > 0 &&
+        (PT ? cols_ok(p, ldp, m) : units_ok(p, ldp, k)) && (QT ? cols_ok(q, ldq, n) : units_ok(q, ldq, k))) mode = ALIGNED;
+    else if (k >= BK && (!PT || m >= 4) && (!QT || n >= 4)) mode = LOOSELY;
+    auto small = [&](auto act) {
+        constexpr int A = decltype(act)::value;
+        return mode == ALIGNED ? launch_tile<T, 128, 128, 2, 2, PT, QT, ALIGNED, A>(a, s)
+             : mode == LOOSELY ? launch_tile<T, 128, 128, 2, 2, PT, QT, LOOSELY, A>(a, s)
+                               : launch_tile<T, 128, 128, 2, 2, PT, QT, BY_ELEMENT, A>(a, s);
+    };
     if (pl.slices > 1) {
-        const int rc = vec ? launch_tile<T, 128, 128, 2, 2, PT, QT, true, PARTIAL>(a, s) : launch_tile<T, 128, 128, 2, 2, PT, QT, false, PARTIAL>(a, s);
-        if (rc) return rc;
+        if (int rc = small(std::integral_constant<int, PARTIAL>{})) return rc;
         const int v = fin.vec ? 4 : 1;
         const dim3 blocks((unsigned)((m * (n / v) + 63) / 64));
         if (v == 4) hipLaunchKernelGGL((slices_kernel<T, 4, ACT>), blocks, dim3(256), 0, s, partial, pl.slices, m, n, fin);
         else hipLaunchKernelGGL((slices_kernel<T, 1, ACT>), blocks, dim3(256), 0, s, partial, pl.slices, m, n, fin);
         return launch_status();
     }
-    if (pl.big && vec) return launch_tile<T, 256, 256, 2, 4, PT, QT, true, ACT>(a, s);
+    if (pl.big && mode == ALIGNED) return launch_tile<T, 256, 256, 2, 4, PT, QT, ALIGNED, ACT>(a, s);
     if (pl.big) { a.tiles_m = (int)((m + 127) / 128); a.tiles_n = (int)((n + 127) / 128); }
-    return vec ? launch_tile<T, 128, 128, 2, 2, PT, QT, true, ACT>(a, s) : launch_tile<T, 128, 128, 2, 2, PT, QT, false, ACT>(a, s);
+    return small(std::integral_constant<int, ACT>{});
 }
 
 template <typename T> static Finish<T> make_finish(const void* bias, const void* res, int64_t ldr, int16_t* slope, int64_t ldp, void* out, int64_t ldo,
@@ -858,15 +967,19 @@ extern "C" int plnlp_linear_act(const void* x, int64_t ldx, const void* w, int64
         using T = decltype(tt);
         constexpr int A = decltype(at)::value;
         const Finish<T> fin = make_finish<T>(bias, residual, ldr, slope, lds, out, ldo, n);
-        if (m <= FEW_ROWS && units_ok(x, ldx, k) && units_ok(w, ldw, k)) {
+        if (m <= FEW_ROWS) {
+            const bool aligned = units_ok(x, ldx, k) && units_ok(w, ldw, k);
             const unsigned blocks = (unsigned)((n + 15) / 16);
             auto run = [&](auto kernel, int waves) {
                 hipLaunchKernelGGL(kernel, dim3(blocks), dim3(waves * 64), 0, s, (const T*)x, ldx, (const T*)w, ldw, (int)m, n, k, fin);
                 return launch_status();
             };
-            if (m <= 16) return k >= 1024 ? run(few_rows_kernel<T, 1, 8, A>, 8) : run(few_rows_kernel<T, 1, 4, A>, 4);
-            if (m <= 32) return run(few_rows_kernel<T, 2, 8, A>, 8);
-            return run(few_rows_kernel<T, 4, 8, A>, 8);
+            auto sized = [&](auto loose) {
+                constexpr bool L = decltype(loose)::value;
+                if (m <= 16) return k >= 1024 ? run(few_rows_kernel<T, 1, 8, L, A>, 8) : run(few_rows_kernel<T, 1, 4, L, A>, 4);
+                return m <= 32 ? run(few_rows_kernel<T, 2, 8, L, A>, 8) : run(few_rows_kernel<T, 4, 8, L, A>, 8);
+            };
+            return aligned ? sized(std::false_type{}) : sized(std::true_type{});
         }
         const int ks = rows_fit(m, n, k);
         if (ks && fin.vec && units_ok(x, ldx, k) && units_ok(w, ldw, k)) {
