@@ -13,8 +13,7 @@
 //   dx       P = dz  (k contiguous)            Q = W read with k along its ROWS
 //   dW       P = dz, Q = x, both with k along their rows
 // A tile of P and of Q is staged global -> registers -> LDS as rows of 64 consecutive k (128 bytes); an operand with k along its
-// rows is transposed on the way, in registers (8 k x 4 columns a thread, sixteen v_perm_b32), so the product itself reads one
-// layout.  The 16-byte units of a row are XOR-swizzled (swz) so that the stores of both kinds and the reads hit all LDS banks.
+// rows is transposed on the way, in registers (8 k x 8 columns a thread, 32 v_perm_b32), so the product itself reads one layout.  The 16-byte units of a row are XOR-swizzled (swz) so that the stores of both kinds and the reads hit all LDS banks.
 // Q is the MFMA's first operand and its rows are dealt so that a lane ends up with groups of 8 CONSECUTIVE columns of one row of C: bias,
 // residual and result move as 16-byte accesses straight from the accumulators, with no pass through LDS.
 #include "half.hip.h"
@@ -155,22 +154,22 @@ template <typename T> struct TileArgs {
 };
 
 // Unit u of LDS row r sits at u ^ swz(r).  A 16-byte read serves 16 lanes a clock from 64 banks, two rows of 128 bytes: of the rows
-// 0..15 of a fragment, of the dealt Q rows (q_row) and of a transposed block's rows 4 apart, those of one parity sit in eight
-// different units.
-__device__ __forceinline__ int swz(int r) { return ((r >> 1) & 1) ^ (((r >> 3) & 1) << 1) ^ (((r >> 2) & 1) << 2) ^ (((r >> 4) & 1) * 5); }
+// 0..15 of a fragment, or of the dealt Q rows (q_row), those of one parity sit in eight different units; so do the rows 8 apart that a
+// transposed block's store touches at once (of one parity all: two clocks).
+__device__ __forceinline__ int swz(int r) {
+    return ((r >> 1) & 1) ^ (((r >> 3) & 1) << 1) ^ (((r >> 2) & 1) << 2) ^ (((r >> 4) & 1) * 5) ^ ((r >> 5) & 1);
+}
 
 // Q row (column of C) behind row r of the MFMA's tile t: lane group g = r >> 2 gets columns 32 (t / 2) + 8 g + 4 (t & 1) + 0..3, so its
 // tiles 2h and 2h + 1 are eight consecutive columns, and the four groups' stores 64 consecutive bytes
 __device__ __forceinline__ int q_row(int t, int r) { return 32 * (t >> 1) + 8 * (r >> 2) + 4 * (t & 1) + (r & 3); }
 
-// column j of an 8 k x 4 columns block held as eight rows of two words: its eight k
-__device__ __forceinline__ u32x4 block_column(const uint32_t* d, int j) {
+// column j of a block of 8 k by 4 or 8 columns, held as eight rows of W words: its eight k
+template <int W> __device__ __forceinline__ u32x4 block_column(const uint32_t* d, int j) {
     u32x4 o;
 #pragma unroll
-    for (int h = 0; h < 4; ++h) {
-        const uint32_t a = d[(2 * h) * 2 + (j >> 1)], b = d[(2 * h + 1) * 2 + (j >> 1)];
-        o[h] = __builtin_amdgcn_perm(b, a, (j & 1) ? 0x07060302u : 0x05040100u);
-    }
+    for (int h = 0; h < 4; ++h)
+        o[h] = __builtin_amdgcn_perm(d[(2 * h + 1) * W + (j >> 1)], d[(2 * h) * W + (j >> 1)], (j & 1) ? 0x07060302u : 0x05040100u);
     return o;
 }
 
@@ -178,94 +177,96 @@ __device__ __forceinline__ u32x4 block_column(const uint32_t* d, int j) {
 // buffer descriptor (16-byte aligned rows of whole units)
 enum { BY_ELEMENT = 0, LOOSELY = 1, ALIGNED = 2 };
 
-// One operand's tile of R rows x BK on its way to LDS: this thread's share.  Every step issues the same loads, whatever the matrix's
-// edges: rows past the last repeat it (their results are not stored); the last step of a k that is no multiple of BK begins early,
-// and what it reads twice is cleared on the way to LDS.
-template <typename T, int R, int THREADS, bool COLS, int MODE> struct Operand {
-    static constexpr int N = R * 8 / THREADS;
+// One operand's tile of R rows x BK on its way to LDS, staged by R threads, 8 loads of 16 bytes each: the first half of a workgroup's
+// waves stages P, the other Q.  (With both staged by all, an operand with k along its rows came in blocks of 8 k x 4 columns, 8 bytes a
+// lane, and a wave's load takes the address unit as long for 8 bytes a lane as for 16: dW of 4096 x 4096 over 8192 rows took 351 us.)
+// Every step issues the same loads, whatever the matrix's edges: rows past the last repeat it (their results are not stored); the last
+// step of a k that is no multiple of BK begins early, and what it reads twice is cleared on the way to LDS.
+// COLS: k lies along the operand's rows: blocks of 8 k x 8 columns.
+template <typename T, int R, int MODE> struct Operand {
+    static constexpr int N = 8;
     u32x4 reg[N];
-    uint32_t off[COLS ? 1 : N];            // ALIGNED: bytes from the tile's (uniform) first element
-    int skip, valid;                       // of the step in reg: k in [skip, valid) are real and not read before
+    uint32_t off[2];                       // ALIGNED: bytes from the (uniform) first element of a load -- rows of a tile come R / 8 a load;
+                                           // off[1]: in the last load that holds rows of the matrix, which the loads past it repeat
+    int skip[2], valid[2];                 // of the step in each half of reg: k in [skip, valid) are real and not read before
 
-    static __device__ __forceinline__ int row_of(int i) { return (int)(threadIdx.x + i * THREADS) >> 3; }
-    static __device__ __forceinline__ int unit() { return threadIdx.x & 7; }
-    static __device__ __forceinline__ int col() { return (int)(threadIdx.x % (R / 4)) * 4; }          // COLS: 8 k x 4 columns a thread
-    static __device__ __forceinline__ int group() { return (int)threadIdx.x / (R / 4); }
+    static __device__ __forceinline__ int tid() { return threadIdx.x & (R - 1); }
+    static __device__ __forceinline__ int row_of(int i) { return (tid() + i * R) >> 3; }
+    static __device__ __forceinline__ int unit() { return tid() & 7; }
+    static __device__ __forceinline__ int col() { return tid() % (R / 8) * 8; }
+    static __device__ __forceinline__ int group() { return tid() / (R / 8); }
 
     // rows: of the tile inside the matrix; k: the matrix's depth (COLS: at least BK unless BY_ELEMENT)
-    __device__ __forceinline__ void begin(int64_t ld, int rows, int64_t k) {
-        static_assert(!COLS || R * 2 == THREADS, "one 8 x 4 block a thread");
+    template <bool COLS> __device__ __forceinline__ void begin(int64_t ld, int rows, int64_t k) {
         if (MODE != ALIGNED) return;
-        if (COLS) off[0] = (uint32_t)((int64_t)(group() * 8) * ld + min(col(), rows - 4)) * 2;        // (whole groups of four columns)
+        if (COLS) off[0] = (uint32_t)((int64_t)(group() * 8) * ld + min(col(), rows - 8)) * 2;        // (whole groups of eight columns)
         else
 #pragma unroll
-            for (int i = 0; i < N; ++i) off[COLS ? 0 : i] = (uint32_t)(min(row_of(i), rows - 1) * ld + min((int64_t)unit() * 8, k - 8)) * 2;
+            for (int l = 0; l < 2; ++l)
+                off[l] = (uint32_t)((l ? min(tid() >> 3, (rows - 1) % (R / 8)) : tid() >> 3) * ld + min((int64_t)unit() * 8, k - 8)) * 2;
     }
-    // `base`: the tile's element at depth k0
-    __device__ __forceinline__ void fetch(const T* base, int64_t ld, int rows, int64_t k0, int64_t k) {
+    // loads LO .. HI - 1 of the eight (half of them or all); `base`: the tile's element at depth k0
+    template <bool COLS, int LO, int HI> __device__ __forceinline__ void fetch(const T* base, int64_t ld, int rows, int64_t k0, int64_t k) {
         const int left = (int)min(k - k0, (int64_t)BK), back = MODE != BY_ELEMENT && k >= BK ? BK - left : 0;
-        skip = back;
-        valid = left + back;
+        for (int h = LO / 4; h < HI / 4; ++h) { skip[h] = back; valid[h] = left + back; }
         base -= COLS ? back * ld : back;
         // (a buffer descriptor of the step's first element: the loads then take one 32-bit register of addresses each)
         const auto at = __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, -1, 0x00027000);
-        if (COLS) {
-            uint64_t* d = reinterpret_cast<uint64_t*>(reg);
+        const int last = (rows - 1) / (R / 8);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const int kk = group() * 8 + i;
-                if (MODE == ALIGNED) d[i] = __builtin_bit_cast(uint64_t, __builtin_amdgcn_raw_buffer_load_b64(at, off[0], (int)(i * ld * 2), 0));
-                else if (MODE == LOOSELY)
-                    d[i] = __builtin_bit_cast(uint64_t, *reinterpret_cast<const LoosePack<T, 4>*>(base + kk * ld + min(col(), rows - 4)));
-                else {
-                    union { T t[4]; uint64_t u; } x;
+        for (int i = LO; i < HI; ++i) {
+            const int kk = group() * 8 + i;
+            const T* p = COLS ? base + kk * ld + min(col(), rows - 8) : base + min(row_of(i), rows - 1) * ld + unit() * 8;
+            if (MODE == ALIGNED)
+                reg[i] = __builtin_bit_cast(u32x4, COLS ? __builtin_amdgcn_raw_buffer_load_b128(at, off[0], (int)(i * ld * 2), 0)
+                                                        : __builtin_amdgcn_raw_buffer_load_b128(at, i < last ? off[0] : off[1], (int)(min(i, last) * (R / 8) * ld * 2), 0));
+            else if (MODE == LOOSELY) reg[i] = __builtin_bit_cast(u32x4, *reinterpret_cast<const LoosePack<T, 8>*>(p));
+            else {
+                union { T t[8]; u32x4 u; } x;
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) x.t[j] = (kk < left && col() + j < rows) ? base[kk * ld + col() + j] : (T)0.f;
-                    d[i] = x.u;
-                }
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < N; ++i) {
-                const T* row = base + min(row_of(i), rows - 1) * ld;
-                if (MODE == ALIGNED) reg[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(at, off[COLS ? 0 : i], 0, 0));
-                else if (MODE == LOOSELY) reg[i] = __builtin_bit_cast(u32x4, *reinterpret_cast<const LoosePack<T, 8>*>(row + unit() * 8));
-                else {
-                    union { T t[8]; u32x4 u; } x;
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) x.t[j] = unit() * 8 + j < left ? row[unit() * 8 + j] : (T)0.f;
-                    reg[i] = x.u;
-                }
+                for (int j = 0; j < 8; ++j)
+                    if (COLS) x.t[j] = (kk < left && col() + j < rows) ? base[kk * ld + col() + j] : (T)0.f;
+                    else x.t[j] = unit() * 8 + j < left ? p[j] : (T)0.f;
+                reg[i] = x.u;
             }
         }
     }
-    // into LDS rows of 128 bytes
-    __device__ __forceinline__ void store(char* lds, int rows) {
+    // the same part of them into LDS rows of 128 bytes (COLS: all)
+    template <bool COLS, int LO, int HI> __device__ __forceinline__ void store(char* lds, int rows) {
+        static_assert(!COLS || HI - LO == N, "a block is transposed as a whole");
+        const int skip = this->skip[LO / 4], valid = this->valid[LO / 4];
+        const bool part = MODE != BY_ELEMENT && (skip > 0 || valid < BK);
         if (COLS) {
-            uint64_t* d = reinterpret_cast<uint64_t*>(reg);
-            if (MODE != BY_ELEMENT && (skip > 0 || valid < BK))
+            if (part)
 #pragma unroll
-                for (int i = 0; i < 8; ++i) if (group() * 8 + i < skip || group() * 8 + i >= valid) d[i] = 0;
-            if (MODE == LOOSELY && (rows & 3)) {          // the last block of columns was read up to three columns early
-                const int early = min(max(col() - (rows - 4), 0), 3);
+                for (int i = 0; i < N; ++i) if (group() * 8 + i < skip || group() * 8 + i >= valid) reg[i] = u32x4{0, 0, 0, 0};
+            if (MODE == LOOSELY && (rows & 7)) {          // the last block of columns was read up to seven columns early
+                const int early = min(max(col() - (rows - 8), 0), 7);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) d[i] >>= 16 * early;
+                for (int i = 0; i < N; ++i) {
+                    uint64_t lo = ((uint64_t)reg[i][1] << 32) | reg[i][0], hi = ((uint64_t)reg[i][3] << 32) | reg[i][2];
+                    if (early >= 4) { lo = hi; hi = 0; }
+                    const int by = (early & 3) * 16;
+                    if (by) { lo = (lo >> by) | (hi << (64 - by)); hi >>= by; }
+                    reg[i] = u32x4{(uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32)};
+                }
             }
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                *reinterpret_cast<u32x4*>(lds + (col() + j) * 128 + ((group() ^ swz(col() + j)) << 4)) = block_column(reinterpret_cast<const uint32_t*>(reg), j);
+            for (int j = 0; j < 8; ++j)
+                *reinterpret_cast<u32x4*>(lds + (col() + j) * 128 + ((group() ^ swz(col() + j)) << 4)) =
+                    block_column<4>(reinterpret_cast<const uint32_t*>(reg), j);
         } else {
-            if (MODE != BY_ELEMENT && (skip > 0 || valid < BK)) {
+            if (part) {
                 const int lo = skip - unit() * 8, hi = valid - unit() * 8;      // elements [lo, hi) of the unit stay
 #pragma unroll
                 for (int h = 0; h < 4; ++h) {
                     const uint32_t keep = (2 * h >= lo && 2 * h < hi ? 0xffffu : 0u) | (2 * h + 1 >= lo && 2 * h + 1 < hi ? 0xffff0000u : 0u);
 #pragma unroll
-                    for (int i = 0; i < N; ++i) reg[i][h] &= keep;
+                    for (int i = LO; i < HI; ++i) reg[i][h] &= keep;
                 }
             }
 #pragma unroll
-            for (int i = 0; i < N; ++i)
+            for (int i = LO; i < HI; ++i)
                 *reinterpret_cast<u32x4*>(lds + row_of(i) * 128 + ((unit() ^ swz(row_of(i))) << 4)) = reg[i];
         }
     }
@@ -312,23 +313,36 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void tile_kernel(TileArgs<T> a) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) ones[j] = (T)1.f;
 
-    Operand<T, BM, THREADS, PT, MODE> sp;
-    Operand<T, BN, THREADS, QT, MODE> sq;
-    if (steps > 0) { sp.begin(a.ldp, rows_p, a.k); sq.begin(a.ldq, rows_q, a.k); }
+    static_assert(BM == BN && THREADS == 2 * BM, "half of the threads stage P, half Q");
+    const bool later = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) >= WM * WN / 2;     // the half that stages Q
+    Operand<T, BM, MODE> mine;
+    if (steps > 0) { if (later) mine.template begin<QT>(a.ldq, rows_q, a.k); else mine.template begin<PT>(a.ldp, rows_p, a.k); }
     // (a step past the last fetches the last again: the loads in flight at any point are the same in every step)
-    auto fetch_p = [&](int step) {
+    typedef std::integral_constant<int, 0> Zero;
+    typedef std::integral_constant<int, 4> Half;
+    typedef std::integral_constant<int, 8> All;
+    auto fetch = [&](int step, auto lo, auto hi) {
+        constexpr int LO = decltype(lo)::value, HI = decltype(hi)::value;
         const int at = first + min(step, steps - 1), term = at >= term_steps;
         const int64_t k = (int64_t)(at - (term ? term_steps : 0)) * BK;
-        const T* p = a.p + (term ? a.plane : 0);
-        sp.fetch(PT ? p + k * a.ldp + m0 : p + m0 * a.ldp + k, a.ldp, rows_p, k, a.k);
+        if (later) mine.template fetch<QT, LO, HI>(QT ? a.q + k * a.ldq + n0 : a.q + n0 * a.ldq + k, a.ldq, rows_q, k, a.k);
+        else {
+            const T* p = a.p + (term ? a.plane : 0);
+            mine.template fetch<PT, LO, HI>(PT ? p + k * a.ldp + m0 : p + m0 * a.ldp + k, a.ldp, rows_p, k, a.k);
+        }
     };
-    auto fetch_q = [&](int step) {
-        const int at = first + min(step, steps - 1);
-        const int64_t k = (int64_t)(at - (at >= term_steps ? term_steps : 0)) * BK;
-        sq.fetch(QT ? a.q + k * a.ldq + n0 : a.q + n0 * a.ldq + k, a.ldq, rows_q, k, a.k);
+    auto stage_all = [&](int buf) {
+        char* b = lds + buf * BUF;
+        if (later) mine.template store<QT, 0, 8>(b + BM * 128, rows_q); else mine.template store<PT, 0, 8>(b, rows_p);
     };
-    auto stage_p = [&](int buf) { sp.store(lds + buf * BUF, rows_p); };
-    auto stage_q = [&](int buf) { sq.store(lds + buf * BUF + BM * 128, rows_q); };
+    // half of what a thread stages, where that operand's k is contiguous
+    auto move_half = [&](int step, auto lo, auto hi) {
+        constexpr int LO = decltype(lo)::value, HI = decltype(hi)::value;
+        char* b = lds + (step & 1) * BUF;
+        if constexpr (!QT) if (later) mine.template store<false, LO, HI>(b + BM * 128, rows_q);
+        if constexpr (!PT) if (!later) mine.template store<false, LO, HI>(b, rows_p);
+        fetch(step + 1, lo, hi);
+    };
     auto q_frag = [&](const char* b, int ks, int t) {
         const int row = wn + q_row(t, r);
         return *reinterpret_cast<const frag*>(b + (BM + row) * 128 + (((ks * 4 + g) ^ swz(row)) << 4));
@@ -338,33 +352,34 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void tile_kernel(TileArgs<T> a) {
         return *reinterpret_cast<const frag*>(b + row * 128 + (((ks * 4 + g) ^ swz(row)) << 4));
     };
     if (steps > 0) {
-        fetch_p(0);
-        fetch_q(0);
-        stage_p(0);
-        stage_q(0);
-        fetch_p(1);
-        fetch_q(1);
+        fetch(0, Zero{}, All{});
+        stage_all(0);
+        fetch(1, Zero{}, All{});
         __syncthreads();
     }
     if constexpr (BM == 256) {
         // Two waves a SIMD, half a step apart: while waves 0..3 multiply (32 MFMAs, 512 clocks), waves 4..7 read their next fragments and
         // move the next tile, and the other way round; a barrier ends each half.  With both in step all of them waited for LDS at
         // the same time (8192 x 4096 x 4096: 334 us).  A step's buffer is read in halves 4 s (waves 0..3) to 4 s + 3 (waves 4..7), the
-        // other one written in those same halves.  Every wave passes 4 barriers a step and one more, the later half before, the
-        // earlier half after.
-        const bool later = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) >= WM * WN / 2;
+        // other one written in the same halves.  Every wave passes 4 barriers a step and one more, the later half before,
+        // the earlier half after.
         if (later) __syncthreads();
         for (int step = 0; step < steps; ++step) {
             const char* b = lds + (step & 1) * BUF;
 #pragma unroll
             for (int ks = 0; ks < 2; ++ks) {
+                const bool blocks = later ? QT : PT;
+                if (ks == 1 && blocks) {         // (before the fragments are read: their registers are not there to spare)
+                    stage_all((step + 1) & 1);
+                    fetch(step + 2, Zero{}, All{});
+                    __builtin_amdgcn_sched_barrier(0);
+                }
                 frag p[TM], q[4];
 #pragma unroll
                 for (int t = 0; t < 4; ++t) q[t] = q_frag(b, ks, t);
 #pragma unroll
                 for (int i = 0; i < TM; ++i) p[i] = p_frag(b, ks, i);
-                if (ks == 0) { stage_p((step + 1) & 1); fetch_p(step + 2); }
-                else { stage_q((step + 1) & 1); fetch_q(step + 2); }
+                if (!blocks) { if (ks == 0) move_half(step + 1, Zero{}, Half{}); else move_half(step + 1, Half{}, All{}); }
                 __syncthreads();
                 __builtin_amdgcn_sched_barrier(0);
                 __builtin_amdgcn_s_setprio(1);
@@ -382,10 +397,8 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void tile_kernel(TileArgs<T> a) {
         for (int step = 0; step < steps; ++step) {
             const char* b = lds + (step & 1) * BUF;
             // (the other buffer was read before the barrier that ended the last step; what is fetched has a whole step to arrive in)
-            stage_p((step + 1) & 1);
-            stage_q((step + 1) & 1);
-            fetch_p(step + 2);
-            fetch_q(step + 2);
+            stage_all((step + 1) & 1);
+            fetch(step + 2, Zero{}, All{});
 #pragma unroll
             for (int ks = 0; ks < BK / 32; ++ks) {
                 frag q[4];
@@ -420,10 +433,22 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void tile_kernel(TileArgs<T> a) {
     for (int h = 0; h < 2; ++h)
 #pragma unroll
         for (int j = 0; j < 8; ++j) bias[h][j] = (ACT != PARTIAL && a.fin.bias && j < cols[h]) ? (float)a.fin.bias[n + 32 * h + j] : 0.f;
+    // (the residual two rows ahead: a load waited for next to its use would wait for the last row's stores as well)
+    constexpr bool AHEAD = MODE == ALIGNED && ACT != PARTIAL;
+    Pack<T, 8> res[AHEAD ? 3 : 1][2];
+    auto ask = [&](int i) {
+        const int64_t m = m0 + wm + i * 16 + r;
+        if (!a.fin.res || i >= TM || m >= a.m) return;
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+            if (cols[h] > 0) res[i % 3][h] = *reinterpret_cast<const Pack<T, 8>*>(a.fin.res + m * a.fin.ldr + n + 32 * h);
+    };
+    if constexpr (AHEAD) { ask(0); ask(1); }
 #pragma unroll
     for (int i = 0; i < TM; ++i) {
         const int64_t m = m0 + wm + i * 16 + r;
         if (m >= a.m) continue;
+        if constexpr (AHEAD) ask(i + 2);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             const int64_t col = n + 32 * h;
@@ -442,7 +467,7 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void tile_kernel(TileArgs<T> a) {
                 } else
 #pragma unroll
                     for (int j = 0; j < 8; ++j) if (j < cols[h]) o[j] = v[j];
-            } else if (MODE == ALIGNED) finish_cols<ACT, false, T, 8>(a.fin, v, bias[h], m, col);
+            } else if constexpr (AHEAD) finish_with<ACT, false, T, 8>(a.fin, v, bias[h], res[i % 3][h], m, col);
             else if (cols[h] == 8) finish_cols<ACT, true, T, 8>(a.fin, v, bias[h], m, col);
             else
                 for (int j = 0; j < cols[h]; ++j) {
@@ -581,7 +606,7 @@ __global__ __launch_bounds__(512) void rows_kernel(RowsArgs<T> a) {
                 if (unit >= UNITS) continue;
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
-                    *reinterpret_cast<u32x4*>(lds + (c + j) * ROW + ((unit ^ rows_swz<KS>(c + j)) << 4)) = block_column(reinterpret_cast<const uint32_t*>(d[i]), j);
+                    *reinterpret_cast<u32x4*>(lds + (c + j) * ROW + ((unit ^ rows_swz<KS>(c + j)) << 4)) = block_column<2>(reinterpret_cast<const uint32_t*>(d[i]), j);
             }
         }
     }
@@ -796,19 +821,24 @@ constexpr int64_t LINEAR_MAX = (int64_t)1 << 31;
 
 static bool units_ok(const void* p, int64_t ld, int64_t along) { return (uintptr_t)p % 16 == 0 && ld % 8 == 0 && along % 8 == 0; }
 
-// tile shape and K slices of a product: 256 x 256 tiles (LDS reads per MFMA two thirds of 128 x 128's) where they alone fill the chip,
-// else 128 x 128, K cut until two workgroups a CU have work -- slices of at least four steps
+// Tile shape and K slices of a product.  256 x 256 tiles read LDS and the caches half as often an MFMA as 128 x 128 ones, but one
+// workgroup of them fills a CU: they are taken where they leave less than an eighth of their area empty and make at least three
+// quarters of the chip's 256 workgroups, alone or with K cut into slices of at least 24 steps.  Else 128 x 128: alone
+// where they make three quarters of a workgroup a CU (4096 x 1024 x 1024: 20 us, in two slices 32), else with K cut until two
+// workgroups a CU have work, into slices of at least four steps.  (us: 8192 x 4096 x 4096 258 against 345; dW of 4096 x 4000 over 8192
+// rows 230 against 372; of 2048 x 1024 over 16384 rows, eight slices, 83 against 107)
 struct Plan { bool big; int tiles_m, tiles_n, slices, steps; };
 static Plan plan_product(int64_t m, int64_t n, int64_t k, int terms = 1) {
     Plan p{};
     const int64_t steps = (k + BK - 1) / BK * terms;
     auto tiles = [](int64_t a, int64_t b) { return (a + b - 1) / b; };
-    p.big = tiles(m, 256) * tiles(n, 256) >= 256 && k >= 512 && n % 256 == 0;
+    const int64_t t256 = tiles(m, 256) * tiles(n, 256), cut = t256 ? std::max<int64_t>(1, 256 / t256) : 1;
+    p.big = m > 0 && n > 0 && (double)t256 * 65536 * 0.875 <= (double)m * n && t256 * cut >= 192 && steps / cut >= (cut > 1 ? 24 : 8);
     const int b = p.big ? 256 : 128;
     p.tiles_m = (int)tiles(m, b);
     p.tiles_n = (int)tiles(n, b);
     const int64_t t = (int64_t)p.tiles_m * p.tiles_n;
-    int64_t s = (p.big || t == 0) ? 1 : 512 / t;
+    int64_t s = p.big ? cut : t == 0 || t >= 192 ? 1 : 512 / t;
     s = std::max<int64_t>(1, std::min(s, steps / 4));
     p.steps = (int)((steps + s - 1) / s);
     p.slices = p.steps ? (int)((steps + p.steps - 1) / p.steps) : 1;
@@ -868,29 +898,26 @@ static int product(const T* p, int64_t ldp, int64_t plane, const T* q, int64_t l
     const int terms = plane ? 2 : 1;
     const Plan pl = plan_product(m, n, k, terms);
     TileArgs<T> a{p, q, ldp, ldq, m, n, k, plane, terms, pl.tiles_m, pl.tiles_n, pl.slices, pl.steps, sums, partial, fin};
-    auto cols_ok = [](const T* x, int64_t ld, int64_t cols) { return (uintptr_t)x % 8 == 0 && ld % 4 == 0 && cols % 4 == 0; };
     // (32-bit offsets inside a tile; an operand with k along its rows needs a whole step of them)
     int mode = BY_ELEMENT;
     if (fin.vec && ldp < ((int64_t)1 << 22) && ldq < ((int64_t)1 << 22) && (k >= BK || !(PT || QT)) && k > 0 &&
-        (PT ? cols_ok(p, ldp, m) : units_ok(p, ldp, k)) && (QT ? cols_ok(q, ldq, n) : units_ok(q, ldq, k))) mode = ALIGNED;
-    else if (k >= BK && (!PT || m >= 4) && (!QT || n >= 4)) mode = LOOSELY;
-    auto small = [&](auto act) {
+        units_ok(p, ldp, PT ? m : k) && units_ok(q, ldq, QT ? n : k)) mode = ALIGNED;
+    else if (k >= BK && (!PT || m >= 8) && (!QT || n >= 8)) mode = LOOSELY;
+    auto run = [&](auto act) {
         constexpr int A = decltype(act)::value;
+        if (pl.big && mode == ALIGNED) return launch_tile<T, 256, 256, 2, 4, PT, QT, ALIGNED, A>(a, s);
+        if (pl.big) { a.tiles_m = (int)((m + 127) / 128); a.tiles_n = (int)((n + 127) / 128); }
         return mode == ALIGNED ? launch_tile<T, 128, 128, 2, 2, PT, QT, ALIGNED, A>(a, s)
              : mode == LOOSELY ? launch_tile<T, 128, 128, 2, 2, PT, QT, LOOSELY, A>(a, s)
                                : launch_tile<T, 128, 128, 2, 2, PT, QT, BY_ELEMENT, A>(a, s);
     };
-    if (pl.slices > 1) {
-        if (int rc = small(std::integral_constant<int, PARTIAL>{})) return rc;
-        const int v = fin.vec ? 4 : 1;
-        const dim3 blocks((unsigned)((m * (n / v) + 63) / 64));
-        if (v == 4) hipLaunchKernelGGL((slices_kernel<T, 4, ACT>), blocks, dim3(256), 0, s, partial, pl.slices, m, n, fin);
-        else hipLaunchKernelGGL((slices_kernel<T, 1, ACT>), blocks, dim3(256), 0, s, partial, pl.slices, m, n, fin);
-        return launch_status();
-    }
-    if (pl.big && mode == ALIGNED) return launch_tile<T, 256, 256, 2, 4, PT, QT, ALIGNED, ACT>(a, s);
-    if (pl.big) { a.tiles_m = (int)((m + 127) / 128); a.tiles_n = (int)((n + 127) / 128); }
-    return small(std::integral_constant<int, ACT>{});
+    if (pl.slices == 1) return run(std::integral_constant<int, ACT>{});
+    if (int rc = run(std::integral_constant<int, PARTIAL>{})) return rc;
+    const int v = fin.vec ? 4 : 1;
+    const dim3 blocks((unsigned)((m * (n / v) + 63) / 64));
+    if (v == 4) hipLaunchKernelGGL((slices_kernel<T, 4, ACT>), blocks, dim3(256), 0, s, partial, pl.slices, m, n, fin);
+    else hipLaunchKernelGGL((slices_kernel<T, 1, ACT>), blocks, dim3(256), 0, s, partial, pl.slices, m, n, fin);
+    return launch_status();
 }
 
 template <typename T> static Finish<T> make_finish(const void* bias, const void* res, int64_t ldr, int16_t* slope, int64_t ldp, void* out, int64_t ldo,

@@ -295,9 +295,11 @@ def test_linear_relu_at_its_border(P, m, n, k, dtype):
 
 
 @gpu
-@pytest.mark.parametrize("m,n,k,dtype", [(16384, 1024, 512, BF16), (16390, 1280, 576, F16)])
+@pytest.mark.parametrize("m,n,k,dtype", [(16384, 1024, 512, BF16), (16390, 1280, 576, F16), (12552, 1000, 1032, BF16), (1792, 8200, 520, F16),
+                                         (512, 2048, 3000, BF16)])
 def test_linear_large_tiles(P, m, n, k, dtype):
-    """the 256 x 256 tiles, forward and both gradients, with ragged rows; checked on sampled rows and columns"""
+    """the 256 x 256 tiles, forward and both gradients, alone and with K in slices, with ragged rows, columns and depths; dx checked on
+    sampled rows"""
     x, w, b, r, gy = linear_case(P, m, n, k, dtype, "silu", True, True)
     y = P.linear_act(x, w, b, residual=r, activation="silu")
     dx, dw, db, dr = torch.autograd.grad(y, [x, w, b, r], gy)
