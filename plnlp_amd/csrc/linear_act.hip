@@ -520,11 +520,12 @@ __global__ __launch_bounds__(256) void slices_kernel(const float* __restrict__ p
 // wave needs 16 accumulators whatever n is -- and the next 16 rows, and the next columns' residual, load meanwhile.
 //   m 131 072, n = k = 256 (bf16, gelu with slope, residual; 268 MB): see the figures at rows_fit.
 // SLOPED: P = dy * slope, formed in the registers (the backward pass: dz = dy * act'(z), dx = dz W), and kept in dz for the
-// weights' gradient.
+// weights' gradient; its column sums are taken here, before it is rounded.
 template <typename T> struct RowsArgs {
     const T* p; int64_t ldp;
     const int16_t* slope; int64_t lds;      // SLOPED
     T* dz; int64_t ldz;
+    float* sums;                            // SLOPED, nullable: [workgroups, k] column sums of dz
     const T* q; int64_t ldq;
     int64_t m; int n, k;
     Finish<T> fin;
@@ -532,6 +533,18 @@ template <typename T> struct RowsArgs {
 
 // rows of KS * 64 bytes begin at the same bank (KS >= 4): the dealt Q rows of a fragment sit in sixteen different units instead
 template <int KS> __device__ __forceinline__ int rows_swz(int r) { return KS < 4 ? swz(r) : (r & 3) ^ (((r >> 3) & 3) << 2); }
+
+// the sum over the 16 lanes of a row of the wave, in each of them
+__device__ __forceinline__ float row_sum(float v) {
+    auto turned = [](float x, auto by) {
+        return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x120 + decltype(by)::value, 0xf, 0xf, true));
+    };
+    v += turned(v, std::integral_constant<int, 8>{});
+    v += turned(v, std::integral_constant<int, 4>{});
+    v += turned(v, std::integral_constant<int, 2>{});
+    v += turned(v, std::integral_constant<int, 1>{});
+    return v;
+}
 
 template <typename T, int KS, bool QT, bool SLOPED, int ACT>
 __global__ __launch_bounds__(512) void rows_kernel(RowsArgs<T> a) {
@@ -612,6 +625,7 @@ __global__ __launch_bounds__(512) void rows_kernel(RowsArgs<T> a) {
     }
     __syncthreads();
 
+    float sums[SLOPED ? KS / 2 : 1] = {};          // of the tiles' 16 rows: lane r keeps every 16th of its group's 8 KS columns
     while (t < tiles) {
         const int64_t m = t * 16 + r;
         const bool in = m < a.m;
@@ -622,7 +636,14 @@ __global__ __launch_bounds__(512) void rows_kernel(RowsArgs<T> a) {
             p[ks] = next[ks];
             if (SLOPED) {
 #pragma unroll
-                for (int j = 0; j < 8; ++j) p[ks][j] = (T)((float)next[ks][j] * unpack_slope(sl[SLOPED ? ks : 0].v[j]));
+                for (int j = 0; j < 8; ++j) {
+                    const float d = (float)next[ks][j] * unpack_slope(sl[SLOPED ? ks : 0].v[j]);
+                    p[ks][j] = (T)d;
+                    if (a.sums) {
+                        const float all = row_sum(in && k < a.k ? d : 0.f);
+                        sums[SLOPED ? ks / 2 : 0] += r == (ks & 1) * 8 + j ? all : 0.f;
+                    }
+                }
                 if (k >= a.k) p[ks] = frag{};
                 else if (in) *reinterpret_cast<frag*>(a.dz + m * a.ldz + k) = p[ks];
             }
@@ -659,6 +680,19 @@ __global__ __launch_bounds__(512) void rows_kernel(RowsArgs<T> a) {
                 }
                 finish_with<ACT, false, T, 8>(a.fin, v, b, mine[h], m, n + 32 * h);
             }
+        }
+    }
+    if constexpr (SLOPED) {
+        if (!a.sums) return;
+        __syncthreads();                           // (Q is done with)
+        float* part = reinterpret_cast<float*>(lds);
+#pragma unroll
+        for (int i = 0; i < KS / 2; ++i) part[wave * KS * 32 + (2 * i + (r >> 3)) * 32 + g * 8 + (r & 7)] = sums[i];
+        __syncthreads();
+        for (int c = threadIdx.x; c < a.k; c += THREADS) {
+            float v = 0.f;
+            for (int w = 0; w < WAVES; ++w) v += part[w * KS * 32 + c];
+            a.sums[(int64_t)blockIdx.x * a.k + c] = v;
         }
     }
 }
@@ -868,6 +902,8 @@ static int rows_fit(int64_t m, int64_t n, int64_t k, int64_t most_k = 512) {
     return 0;
 }
 
+static int64_t rows_blocks(int64_t m) { return std::min<int64_t>((m + 127) / 128, 256); }      // eight waves of 16 rows, one workgroup a CU
+
 template <typename T, int KS, bool QT, bool SLOPED, int ACT> static int launch_rows(const RowsArgs<T>& a, hipStream_t s) {
     auto kernel = rows_kernel<T, KS, QT, SLOPED, ACT>;
     constexpr int THREADS = 512;
@@ -876,9 +912,7 @@ template <typename T, int KS, bool QT, bool SLOPED, int ACT> static int launch_r
         const hipError_t e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
         if (e != hipSuccess) return (int)e;
     }
-    const int64_t tiles = (a.m + 15) / 16;
-    const int64_t blocks = std::min<int64_t>((tiles + THREADS / 64 - 1) / (THREADS / 64), 256);
-    hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(THREADS), lds, s, a);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)rows_blocks(a.m)), dim3(THREADS), lds, s, a);
     return launch_status();
 }
 template <typename T, bool QT, bool SLOPED, int ACT> static int run_rows(int ks, const RowsArgs<T>& a, hipStream_t s) {
@@ -959,8 +993,8 @@ static BackPlan back_plan(int64_t m, int64_t n, int64_t k, int act) {
     b.plane = two ? m * b.ldz : 0;
     int64_t at = 0;
     b.dz = at; at += act == PLNLP_ACT_NONE ? 0 : round256(m * b.ldz * 2 * (two ? 2 : 1));
-    b.slices = plan_product(n, k, m, two ? 2 : 1).slices;        // of the weights' gradient, which may bring the column sums
-    b.sums = at; at += round256(std::max(b.blocks, b.slices) * n * 4);
+    b.slices = plan_product(n, k, m, two ? 2 : 1).slices;        // of the weights' gradient, which may bring the column sums of dy
+    b.sums = at; at += round256(std::max(std::max(b.blocks, b.slices), rows_blocks(m)) * n * 4);
     b.partial = at;
     const int terms = two ? 2 : 1;
     at += round256(std::max(plan_bytes(plan_product(m, k, n, terms), m, k), plan_bytes(plan_product(n, k, m, terms), n, k)));
@@ -1010,7 +1044,7 @@ extern "C" int plnlp_linear_act(const void* x, int64_t ldx, const void* w, int64
         }
         const int ks = rows_fit(m, n, k);
         if (ks && fin.vec && units_ok(x, ldx, k) && units_ok(w, ldw, k)) {
-            const RowsArgs<T> a{(const T*)x, ldx, nullptr, 0, nullptr, 0, (const T*)w, ldw, m, (int)n, (int)k, fin};
+            const RowsArgs<T> a{(const T*)x, ldx, nullptr, 0, nullptr, 0, nullptr, (const T*)w, ldw, m, (int)n, (int)k, fin};
             return run_rows<T, false, false, A>(ks, a, s);
         }
         if (need && (!workspace || workspace_bytes < need)) return PLNLP_E_WORKSPACE;
@@ -1052,12 +1086,13 @@ extern "C" int plnlp_linear_act_backward(const void* gy, int64_t ldg, const int1
         float* partial = (float*)(ws + b.partial);
         const bool want_dx = dx && m > 0 && k > 0, want_dw = dw && n > 0 && k > 0;
         const bool vec = units_ok(gy, ldg, n) && (!has_act || units_ok(slope, lds, n));
-        // many rows and weights that fit LDS: dz is formed on the way to dx, its column sums come with dw
+        // many rows and weights that fit LDS: dz and its column sums are formed on the way to dx; without an activation dz is dy and
+        // its sums come with dw
         const Finish<T> fin_x = make_finish<T>(nullptr, nullptr, 0, nullptr, 0, dx, lddx, k);
         const int ks = want_dx && vec && !plane && fin_x.vec && (uintptr_t)w % 8 == 0 && ldw % 4 == 0 ? rows_fit(m, k, n, has_act ? 256 : 512) : 0;
-        const bool sums_in_dw = ks && want_dw;
+        const bool sums_in_dx = ks && has_act, sums_in_dw = ks && !has_act && want_dw;
         int64_t sum_blocks = m > 0 ? b.blocks : 0;
-        if (m > 0 && n > 0 && ((has_act && !ks) || (db && !sums_in_dw))) {
+        if (m > 0 && n > 0 && ((has_act && !ks) || (db && !sums_in_dx && !sums_in_dw))) {
             const int64_t packs = vec ? n / 8 : n;
             int tx = 1;
             while (tx < 64 && tx < packs) tx <<= 1;
@@ -1072,7 +1107,8 @@ extern "C" int plnlp_linear_act_backward(const void* gy, int64_t ldg, const int1
             if (e) return e;
         }
         if (ks) {
-            const RowsArgs<T> a{(const T*)gy, ldg, slope, lds, (T*)(ws + b.dz), ldz, (const T*)w, ldw, m, (int)k, (int)n, fin_x};
+            const RowsArgs<T> a{(const T*)gy, ldg, slope, lds, (T*)(ws + b.dz), ldz, db ? sums : nullptr, (const T*)w, ldw, m, (int)k, (int)n, fin_x};
+            if (sums_in_dx) sum_blocks = rows_blocks(m);
             if (int e = has_act ? run_rows<T, true, true, PLNLP_ACT_NONE>(ks, a, s) : run_rows<T, true, false, PLNLP_ACT_NONE>(ks, a, s)) return e;
         } else if (want_dx) {
             if (int e = product<T, false, true, PLNLP_ACT_NONE>(dz, ldz, plane, (const T*)w, ldw, m, k, n, fin_x, partial, s)) return e;

@@ -267,9 +267,8 @@ def test_linear_many_rows_some_gradients(P):
     for i, leaf in enumerate((x, w, b, r)):
         args = [t if j == i else t.detach() for j, t in enumerate((x, w, b, r))]
         got, = torch.autograd.grad(P.linear_act(*args[:3], residual=args[3], activation="silu"), [leaf], gy)
-        if i == 2:        # summed from dz before it is rounded here, after it there: u of each term
-            slack = U[BF16] * (gy.double().abs() * 1.1).sum(0) + U[BF16] * full[2].double().abs()
-            within(got, full[2].double(), slack)
+        if i == 2:        # summed in another order
+            within(got, full[2].double(), (gy.double().abs() * 1.13).sum(0) * 8502 * ADD + 2 * U[BF16] * full[2].double().abs())
         else:
             assert torch.equal(got, full[i])
 
