@@ -33,6 +33,29 @@ template <typename T, int V> __device__ __forceinline__ void store_f32(T* p, con
     *reinterpret_cast<Pack<T, V>*>(p) = k;
 }
 
+// ... past the caches, for what is larger than they are and so would only drive out what the next kernel reads
+template <typename T, int V> __device__ __forceinline__ void stream_f32(T* p, const float (&x)[V]) {
+    Pack<T, V> k;
+#pragma unroll
+    for (int i = 0; i < V; ++i) k.v[i] = (T)x[i];
+    if constexpr (sizeof(k) % 16 == 0) {
+        struct Quads { u32x4 q[sizeof(k) / 16]; };
+        const Quads q = __builtin_bit_cast(Quads, k);
+#pragma unroll
+        for (unsigned i = 0; i < sizeof(k) / 16; ++i) __builtin_nontemporal_store(q.q[i], reinterpret_cast<u32x4*>(p) + i);
+    } else *reinterpret_cast<Pack<T, V>*>(p) = k;
+}
+// a pack that is read once
+template <typename T, int V> __device__ __forceinline__ Pack<T, V> stream_pack(const T* p) {
+    if constexpr (sizeof(Pack<T, V>) % 16 == 0) {
+        struct Quads { u32x4 q[sizeof(Pack<T, V>) / 16]; } k;
+#pragma unroll
+        for (unsigned i = 0; i < sizeof(k) / 16; ++i) k.q[i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p) + i);
+        return __builtin_bit_cast(Pack<T, V>, k);
+    } else return *reinterpret_cast<const Pack<T, V>*>(p);
+}
+constexpr int64_t STREAM_BYTES = (int64_t)128 << 20;       // half of the Infinity Cache
+
 // one call of f with the C++ types of a run-time dtype
 template <typename F> inline int with_dtype(int d, F&& f) {
     if (d == PLNLP_DTYPE_F32) return f(float{});
