@@ -850,7 +850,10 @@ __global__ __launch_bounds__(1024) void col_join_kernel(const float* __restrict_
 }
 
 // ---- host ---------------------------------------------------------------------------------------------------------------
-constexpr int FEW_ROWS = 64;
+// Up to 16 rows the weights' bytes are all there is, whatever their number (1 x 4096 x 4096: 8.5 us against 13.9 on the tile kernel; 1 x
+// 16384 x 4096 25, 5.3 TB/s).  Up to 64 rows every workgroup reads x again for its 16 columns: only small and not too deep weights
+// (us: 64 x 1024 x 1024 7.0 / 9.8, 40 x 2048 x 2048 9.8 / 10.6; but 32 x 1024 x 4096 12.7 / 10.8, 64 x 8192 x 4096 43 / 25).
+static bool few_rows(int64_t m, int64_t n, int64_t k) { return m <= 16 || (m <= 64 && k <= 2048 && n * k <= ((int64_t)1 << 22)); }
 constexpr int64_t LINEAR_MAX = (int64_t)1 << 31;
 
 static bool units_ok(const void* p, int64_t ld, int64_t along) { return (uintptr_t)p % 16 == 0 && ld % 8 == 0 && along % 8 == 0; }
@@ -1005,7 +1008,7 @@ static BackPlan back_plan(int64_t m, int64_t n, int64_t k, int act) {
 }  // namespace plnlp
 
 extern "C" int64_t plnlp_linear_act_workspace_bytes(int64_t m, int64_t n, int64_t k) {
-    if (m <= 0 || n <= 0 || k < 0) return 0;
+    if (m <= 0 || n <= 0 || k < 0 || plnlp::few_rows(m, n, k)) return 0;
     return plnlp::plan_bytes(plnlp::plan_product(m, n, k), m, n);
 }
 
@@ -1028,7 +1031,7 @@ extern "C" int plnlp_linear_act(const void* x, int64_t ldx, const void* w, int64
         using T = decltype(tt);
         constexpr int A = decltype(at)::value;
         const Finish<T> fin = make_finish<T>(bias, residual, ldr, slope, lds, out, ldo, n);
-        if (m <= FEW_ROWS) {
+        if (few_rows(m, n, k)) {
             const bool aligned = units_ok(x, ldx, k) && units_ok(w, ldw, k);
             const unsigned blocks = (unsigned)((n + 15) / 16);
             auto run = [&](auto kernel, int waves) {

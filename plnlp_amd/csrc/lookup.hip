@@ -115,36 +115,21 @@ __global__ __launch_bounds__(1024) void sort_offsets_kernel(uint32_t* __restrict
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, d = blockIdx.x * 64 + lane;
     const int per = (tiles + 15) / 16, lo = wave * per, hi = min(lo + per, tiles);
     const bool in = d < bins;
-    constexpr int KEEP = 32;                       // counts a thread keeps in registers between the two passes over them
-    uint32_t kept[KEEP], s = 0;
-    const bool keep = per <= KEEP;
-    if (keep) {
-#pragma unroll
-        for (int i = 0; i < KEEP; ++i) kept[i] = in && lo + i < hi ? hist[(int64_t)(lo + i) * bins + d] : 0;
-#pragma unroll
-        for (int i = 0; i < KEEP; ++i) s += kept[i];
-    } else
+    uint32_t s = 0;
 #pragma unroll 8
-        for (int t = lo; t < hi; ++t) s += in ? hist[(int64_t)t * bins + d] : 0;
+    for (int t = lo; t < hi; ++t) s += in ? hist[(int64_t)t * bins + d] : 0;
     part[wave][lane] = s;
     __syncthreads();
     uint32_t run = 0;
     for (int w = 0; w < wave; ++w) run += part[w][lane];
     if (!in) return;
     if (wave == 15) total[d] = run + s;
-    if (keep) {
-#pragma unroll
-        for (int i = 0; i < KEEP; ++i) {
-            if (lo + i < hi) hist[(int64_t)(lo + i) * bins + d] = run;
-            run += kept[i];
-        }
-    } else
 #pragma unroll 8
-        for (int t = lo; t < hi; ++t) {
-            const uint32_t c = hist[(int64_t)t * bins + d];
-            hist[(int64_t)t * bins + d] = run;
-            run += c;
-        }
+    for (int t = lo; t < hi; ++t) {
+        const uint32_t c = hist[(int64_t)t * bins + d];
+        hist[(int64_t)t * bins + d] = run;
+        run += c;
+    }
 }
 
 __device__ __forceinline__ uint32_t wave_scan(uint32_t v) {     // inclusive

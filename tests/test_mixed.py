@@ -236,7 +236,7 @@ def check_linear(P, x, w, b, r, gy, act, dtype):
 
 # rows: one, the few-rows kernel's three sizes and their edges, one tile, ragged tiles, K cut into slices; widths odd, even, whole
 # groups of eight, ragged against the 128-wide tile; depths below, at and past a 64-step
-LINEAR_SHAPES = [(1, 1, 1), (1, 16, 64), (1, 200, 4096), (3, 17, 72), (16, 256, 256), (17, 40, 1024), (32, 8, 8), (33, 136, 520), (64, 128, 128),
+LINEAR_SHAPES = [(32, 1024, 4104), (64, 2049, 2056), (1, 1, 1), (1, 16, 64), (1, 200, 4096), (3, 17, 72), (16, 256, 256), (17, 40, 1024), (32, 8, 8), (33, 136, 520), (64, 128, 128),
                  (65, 128, 128), (100, 64, 64), (128, 128, 64), (129, 130, 65), (300, 520, 8), (257, 72, 2056), (777, 515, 130), (5, 515, 1003),
                  (1500, 200, 200), (4000, 24, 48)]
 # many rows and weights that fit LDS: full and ragged groups of 64 columns, K of whole and ragged 32-pieces up to the deepest taken
