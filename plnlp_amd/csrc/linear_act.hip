@@ -13,7 +13,8 @@
 //   dx       P = dz  (k contiguous)            Q = W read with k along its ROWS
 //   dW       P = dz, Q = x, both with k along their rows
 // A tile of P and of Q is staged global -> registers -> LDS as rows of 64 consecutive k (128 bytes); an operand with k along its
-// rows is transposed on the way, in registers (8 k x 8 columns a thread, 32 v_perm_b32), so the product itself reads one layout.  The 16-byte units of a row are XOR-swizzled (swz) so that the stores of both kinds and the reads hit all LDS banks.
+// rows is transposed on the way, in registers (8 k x 8 columns a thread, 32 v_perm_b32), so the product itself reads one layout.
+// The 16-byte units of a row are XOR-swizzled (swz) so that the stores of both kinds and the reads hit all LDS banks.
 // Q is the MFMA's first operand and its rows are dealt so that a lane ends up with groups of 8 CONSECUTIVE columns of one row of C: bias,
 // residual and result move as 16-byte accesses straight from the accumulators, with no pass through LDS.
 #include "half.hip.h"
@@ -513,12 +514,12 @@ __global__ __launch_bounds__(256) void slices_kernel(const float* __restrict__ p
 }
 
 // ---- many rows, a Q that fits LDS: Q stays there, P streams through registers -----------------------------------------
-// A layer of a few hundred columns on 10^4 .. 10^6 rows is bound by its rows' bytes, and the tile kernel spends its time waiting for
-// them (a tile of four K steps: load, wait, multiply, finish, with two workgroups a CU to overlap).  Here one workgroup a CU stages all
+// A layer of a few hundred columns on 10^4 .. 10^6 rows is bound by its rows' bytes, and a tile of a few K steps (load, wait, multiply,
+// finish) spends most of its time waiting for them.  Here one workgroup a CU stages all
 // of Q in LDS once; after that its waves never meet again: each takes 16 rows, holds them as MFMA fragments (loaded straight from
 // memory, 64 consecutive bytes a row and load) and walks Q's columns 64 at a time, finishing each group before the next -- so a
 // wave needs 16 accumulators whatever n is -- and the next 16 rows, and the next columns' residual, load meanwhile.
-//   m 131 072, n = k = 256 (bf16, gelu with slope, residual; 268 MB): see the figures at rows_fit.
+// What it measured, and against what: at rows_fit.
 // SLOPED: P = dy * slope, formed in the registers (the backward pass: dz = dy * act'(z), dx = dz W), and kept in dz for the
 // weights' gradient; its column sums are taken here, before it is rounded.
 template <typename T> struct RowsArgs {
@@ -896,10 +897,14 @@ static int launch_tile(const TileArgs<T>& a, hipStream_t s) {
     return launch_status();
 }
 
-// Q in LDS for the rows kernel: 32-k pieces a row (0: it does not take the product)
-constexpr int64_t ROWS_MIN = 8192, ROWS_LDS = 155648;
+// Q in LDS for the rows kernel: 32-k pieces a row (0: it does not take the product).  Every workgroup reads all of Q once, so there
+// have to be rows enough for each: 128 a column of the result (256 workgroups times n k of Q against m k of P, twice).
+//   us, forward with gelu, slope and residual, here / on the tile kernel: 131 072 x 256 x 256 67 / 70 (70 alone on a cold chip: 3.8 TB/s;
+//   91 before either kernel asked for the residual ahead), 32 768 x 256 x 256 19.4 / 20.8 but 16 384 x 256 x 256 17.8 / 15.0;
+//   262 144 x 64 x 256 40 / 64, 16 384 x 64 x 64 6.8 / 10.0, 8192 x 64 x 64 6.3 / 9.7; backward 131 072 x 256 x 256 121 / 127
+constexpr int64_t ROWS_MIN = 8192, ROWS_PER_COLUMN = 128, ROWS_LDS = 155648;
 static int rows_fit(int64_t m, int64_t n, int64_t k, int64_t most_k = 512) {
-    if (m < ROWS_MIN || n == 0 || k == 0 || k > most_k) return 0;
+    if (m < ROWS_MIN || m < ROWS_PER_COLUMN * n || n == 0 || k == 0 || k > most_k) return 0;
     for (int ks : {2, 4, 8, 12, 16})
         if (ks * 32 >= k) return (n + 63) / 64 * 64 * (ks * 64 + 4) <= ROWS_LDS ? ks : 0;
     return 0;

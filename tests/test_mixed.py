@@ -241,7 +241,8 @@ LINEAR_SHAPES = [(32, 1024, 4104), (64, 2049, 2056), (1, 1, 1), (1, 16, 64), (1,
                  (1500, 200, 200), (4000, 24, 48)]
 # many rows and weights that fit LDS: full and ragged groups of 64 columns, K of whole and ragged 32-pieces up to the deepest taken
 # (and the first that is not), rows that end inside a group of 16; the last two fall back for their strides and widths
-MANY_ROWS = [(8192, 256, 256), (8200, 200, 72), (10007, 8, 8), (9000, 136, 264), (8195, 64, 512), (8192, 264, 96), (8300, 512, 64), (8300, 72, 520), (8201, 40, 36), (8209, 33, 64)]
+MANY_ROWS = [(8192, 256, 256), (8200, 200, 72), (10007, 8, 8), (9000, 136, 264), (8195, 64, 512), (8192, 264, 96), (8300, 512, 64), (8300, 72, 520), (8201, 40, 36), (8209, 33, 64), (32770, 256, 256), (33800, 264, 96), (34000, 72, 264), (9001, 64, 200),
+             (65537, 512, 64), (8208, 8, 384)]
 
 
 @gpu
