@@ -973,7 +973,9 @@ template <typename F> static int with_half(int d, F&& f) { return d == PLNLP_DTY
 
 static int linear_check(int64_t m, int64_t n, int64_t k, int act, int dtype) {
     if (m < 0 || n < 0 || k < 0 || m >= LINEAR_MAX || n >= LINEAR_MAX || k >= LINEAR_MAX) return PLNLP_E_SHAPE;
-    if (((m + 127) / 128) * ((n + 127) / 128) >= ((int64_t)1 << 30)) return PLNLP_E_SHAPE;
+    // (workgroups of the three products)
+    const int64_t tm = (m + 127) / 128, tn = (n + 127) / 128, tk = (k + 127) / 128, most = (int64_t)1 << 30;
+    if (tm * tn >= most || tm * tk >= most || tn * tk >= most) return PLNLP_E_SHAPE;
     if (act < PLNLP_ACT_NONE || act > PLNLP_ACT_SILU) return PLNLP_E_UNSUPPORTED;
     if (dtype != PLNLP_DTYPE_BF16 && dtype != PLNLP_DTYPE_F16) return PLNLP_E_UNSUPPORTED;
     return 0;

@@ -227,6 +227,7 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tenso
 # ------------------------------------------------------------------ clipping ----
 _DST_CODES = {t: c << 32 for t, c in L.DTYPE_CODES.items()}
 _SIZES = np.array([4, 2, 2], dtype=np.int64)
+_OVERLAP = "clip_grads: the memory of a clipped tensor overlaps another tensor of the call (a gradient listed twice?)"
 
 
 def _norm_kind(norm_type) -> int:
@@ -313,7 +314,7 @@ def _run_clip(src, dst, sizes, src_codes, dst_codes, kind: int, max_norm: Option
     if max_norm is not None and (n > 1 or src is not dst):
         to = rows[3] >> 32
         if _overlap(rows[0], rows[0] if src is dst else rows[1], rows[2], rows[3] & 3, to):
-            raise ValueError("clip_grads: the memory of a clipped tensor overlaps another tensor of the call (a gradient listed twice?)")
+            raise ValueError(_OVERLAP)
     rows = np.ascontiguousarray(rows.T)
     at = rows.ctypes.data
     need = lib.plnlp_grad_norm_workspace_doubles(at, n)
@@ -355,8 +356,10 @@ def clip_grads(grads: Sequence[torch.Tensor], max_norm: float, *, norm_type: flo
         src = list(map(torch.Tensor.data_ptr, flat))
     if flat_to is not to:
         dst = src if out is None else list(map(torch.Tensor.data_ptr, flat_to))
+    if flat_to is not to and len({t.data_ptr() for t in to if t.numel()}) < sum(t.numel() > 0 for t in to):
+        raise ValueError(_OVERLAP)                   # (the copies of such tensors do not overlap)
     norm = _run_clip(src, dst, sizes, _codes(types, L.DTYPE_CODES), _codes(to_types, _DST_CODES), kind, max_norm)
-    torch.autograd.graph.increment_version(to)       # (written behind autograd's back)
+    torch.autograd.graph.increment_version([t for t in to if not t.is_inference()])      # (written behind autograd's back)
     if flat_to is not to:
         with torch.no_grad():
             for t, c in zip(to, flat_to):

@@ -356,6 +356,11 @@ def test_linear_shapes_of_more_dimensions_and_empty_ones(P):
     assert y.shape == (0, 24) and dx.shape == (0, 16) and not bool(dw.any()) and not bool(db.any())
     x0, w0 = torch.zeros(5, 0, dtype=BF16, device="cuda"), torch.zeros(24, 0, dtype=BF16, device="cuda")
     assert torch.equal(P.linear_act(x0, w0, b), b.detach().expand(5, 24))
+    none = torch.zeros(0, 16, dtype=BF16, device="cuda", requires_grad=True)          # a layer without outputs
+    some = x.view(6, 16).clone().requires_grad_(True)
+    y = P.linear_act(some, none, activation="gelu")
+    dx, dw = torch.autograd.grad(y, [some, none], torch.zeros_like(y))
+    assert y.shape == (6, 0) and dx.shape == (6, 16) and not bool(dx.any()) and dw.shape == (0, 16)
     # a bias and a residual shared by broadcasting: the caller expands, autograd sums
     one = rand((1, 24), BF16, 5).requires_grad_(True)
     y = P.linear_act(x.view(6, 16), w, b, residual=one.expand(6, 24))
@@ -478,6 +483,24 @@ def test_clip_views_alignment_and_neighbours(P):
 
 
 @gpu
+def test_clip_refuses_what_it_would_scale_twice(P):
+    a, b = rand((30, 8), BF16, 1), rand((20,), F32, 2)
+    for grads, out in (([a, b, a], None), ([a.t(), a.t()], None), ([a[:, ::2], a[:, ::2]], None), ([a, a[3:5]], None),
+                       ([a, b], [b.new_empty(240), a.view(-1)[:20]])):
+        keep = [g.clone() for g in grads]
+        with pytest.raises(ValueError):
+            P.clip_grads(grads, 0.1, out=out)
+        assert all(torch.equal(g, k) for g, k in zip(grads, keep))
+    with torch.inference_mode():
+        c = torch.ones(10, device="cuda")
+        P.clip_grads([c], 1.0)
+        assert float(c.norm()) == pytest.approx(1.0, abs=1e-5)
+    version = a._version
+    P.clip_grads([a], 0.1)
+    assert a._version > version                               # autograd is told that the gradient changed
+
+
+@gpu
 def test_clip_more_partials_than_a_workgroup_joins(P):
     grads = [torch.full((1,), 0.5, dtype=(BF16, F32)[i % 2], device="cuda") for i in range(4300)]
     want = 0.5 * math.sqrt(4300)
@@ -549,11 +572,12 @@ def test_a_training_step_of_all_three(P):
 
 
 @gpu
-def test_captured_and_replayed(P):
+@pytest.mark.parametrize("n,width", [(5000, 64), (40000, 256), (7, 96), (2048, 1024)])
+def test_captured_and_replayed(P, n, width):
     """the three operators with their gradients in one graph, replayed with other inputs and eager work between: eager's bits each time"""
-    table = rand((300, 64), BF16, 1).requires_grad_(True)
-    w, b = rand((64, 64), BF16, 2, 0.1).requires_grad_(True), rand((64,), BF16, 3).requires_grad_(True)
-    ids, gy = torch.zeros(5000, dtype=torch.int64, device="cuda"), torch.zeros(5000, 64, dtype=BF16, device="cuda")
+    table = rand((300, width), BF16, 1).requires_grad_(True)
+    w, b = rand((width, width), BF16, 2, 0.1).requires_grad_(True), rand((width,), BF16, 3).requires_grad_(True)
+    ids, gy = torch.zeros(n, dtype=torch.int64, device="cuda"), torch.zeros(n, width, dtype=BF16, device="cuda")
 
     def step():
         x = P.embedding_lookup(table, ids, scale=0.5)
@@ -572,8 +596,8 @@ def test_captured_and_replayed(P):
     with torch.cuda.graph(graph):
         held = step()
     for i in range(4):
-        ids.copy_(torch.randint(-1, 300 if i % 2 else 4, (5000,), generator=torch.Generator(device="cuda").manual_seed(i), device="cuda"))
-        gy.copy_(rand((5000, 64), BF16, 20 + i, 0.1))
+        ids.copy_(torch.randint(-1, 300 if i % 2 else 4, (n,), generator=torch.Generator(device="cuda").manual_seed(i), device="cuda"))
+        gy.copy_(rand((n, width), BF16, 20 + i, 0.1))
         graph.replay()
         torch.cuda.synchronize()
         got = [t.clone() for t in held]
