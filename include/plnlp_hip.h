@@ -657,10 +657,11 @@ int plnlp_embedding_grad(const void* gy, int64_t ldg, int gy_dtype, const void* 
 #define PLNLP_ACT_GELU_TANH 3   /* z (1 + tanh(sqrt(2/pi) (z + 0.044715 z^3))) / 2           */
 #define PLNLP_ACT_SILU      4   /* z / (1 + exp(-z))                                         */
 /* out = act(x w^T + bias) + residual for x [m, k], w [n, k] (nn.Linear's layout), bias [n] (nullable), residual [m, n] (nullable),
- * all of one 16-bit type (dtype BF16 or F16), rows ld* elements apart (at most 2^31), any alignment of whole elements; 16-byte
- * aligned rows and k, n % 8 == 0 take the wide loads.  slope (nullable): act'(x w^T + bias), what the backward pass reads, int16 in
- * steps of 2^-14 (20000: NaN).  out may be residual itself (same rows); otherwise outputs alias nothing.  workspace: plnlp_linear_act_workspace_bytes(m, n, k) bytes,
- * 16-byte aligned (0: none needed). */
+ * all of one 16-bit type (dtype BF16 or F16), rows ld* elements apart, any alignment of whole elements; 16-byte aligned rows
+ * and k, n % 8 == 0 take the wide loads.  m, k < 2^31, n < 2^26, and less than 2^24 tiles of 128 x 128 in each of [m, n],
+ * [m, k] and [n, k].  slope (nullable): act'(x w^T + bias), what the backward pass reads, int16 in steps of 2^-14 (20000: NaN).
+ * out may be residual itself (same rows); otherwise outputs alias nothing.  workspace: plnlp_linear_act_workspace_bytes(m, n, k)
+ * bytes, 16-byte aligned (0: none needed). */
 int64_t plnlp_linear_act_workspace_bytes(int64_t m, int64_t n, int64_t k);
 int plnlp_linear_act(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, const void* residual, int64_t ldr,
                      int act, int64_t m, int64_t n, int64_t k, int16_t* slope, int64_t lds, void* out, int64_t ldo, int dtype,

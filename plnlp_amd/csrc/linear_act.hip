@@ -180,7 +180,8 @@ enum { BY_ELEMENT = 0, LOOSELY = 1, ALIGNED = 2 };
 
 // One operand's tile of R rows x BK on its way to LDS, staged by R threads, 8 loads of 16 bytes each: the first half of a workgroup's
 // waves stages P, the other Q.  (With both staged by all, an operand with k along its rows came in blocks of 8 k x 4 columns, 8 bytes a
-// lane, and a wave's load takes the address unit as long for 8 bytes a lane as for 16: dW of 4096 x 4096 over 8192 rows took 351 us.)
+// lane, and a wave's load takes the address unit as long for 8 bytes a lane as for 16: dW of 4096 x 4096 over 8192 rows took 351 us
+// against 234.)
 // Every step issues the same loads, whatever the matrix's edges: rows past the last repeat it (their results are not stored); the last
 // step of a k that is no multiple of BK begins early, and what it reads twice is cleared on the way to LDS.
 // COLS: k lies along the operand's rows: blocks of 8 k x 8 columns.
@@ -361,7 +362,7 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void tile_kernel(TileArgs<T> a) {
     if constexpr (BM == 256) {
         // Two waves a SIMD, half a step apart: while waves 0..3 multiply (32 MFMAs, 512 clocks), waves 4..7 read their next fragments and
         // move the next tile, and the other way round; a barrier ends each half.  With both in step all of them waited for LDS at
-        // the same time (8192 x 4096 x 4096: 334 us).  A step's buffer is read in halves 4 s (waves 0..3) to 4 s + 3 (waves 4..7), the
+        // the same time (8192 x 4096 x 4096: 334 us against 258).  A step's buffer is read in halves 4 s (waves 0..3) to 4 s + 3 (waves 4..7), the
         // other one written in the same halves.  Every wave passes 4 barriers a step and one more, the later half before,
         // the earlier half after.
         if (later) __syncthreads();
@@ -572,7 +573,7 @@ __global__ __launch_bounds__(512) void rows_kernel(RowsArgs<T> a) {
     Pack<T, 8> res[2];                       // the residual of the columns that come next
     auto ask = [&](int64_t tile, int n0) {
         const int64_t m = tile * 16 + r;
-        if (ACT == PARTIAL || !a.fin.res || m >= a.m) return;
+        if (!a.fin.res || m >= a.m) return;
 #pragma unroll
         for (int h = 0; h < 2; ++h)
             if (n0 + 8 * g + 32 * h < a.n) res[h] = *reinterpret_cast<const Pack<T, 8>*>(a.fin.res + m * a.fin.ldr + n0 + 8 * g + 32 * h);
@@ -855,7 +856,7 @@ __global__ __launch_bounds__(1024) void col_join_kernel(const float* __restrict_
 // 16384 x 4096 25, 5.3 TB/s).  Up to 64 rows every workgroup reads x again for its 16 columns: only small and not too deep weights
 // (us: 64 x 1024 x 1024 7.0 / 9.8, 40 x 2048 x 2048 9.8 / 10.6; but 32 x 1024 x 4096 12.7 / 10.8, 64 x 8192 x 4096 43 / 25).
 static bool few_rows(int64_t m, int64_t n, int64_t k) { return m <= 16 || (m <= 64 && k <= 2048 && n * k <= ((int64_t)1 << 22)); }
-constexpr int64_t LINEAR_MAX = (int64_t)1 << 31;
+constexpr int64_t LINEAR_MAX = (int64_t)1 << 31, LINEAR_MAX_N = (int64_t)1 << 26;   // rows and depth; columns
 
 static bool units_ok(const void* p, int64_t ld, int64_t along) { return (uintptr_t)p % 16 == 0 && ld % 8 == 0 && along % 8 == 0; }
 
@@ -972,9 +973,9 @@ template <typename T> static Finish<T> make_finish(const void* bias, const void*
 template <typename F> static int with_half(int d, F&& f) { return d == PLNLP_DTYPE_BF16 ? f(__bf16{}) : f(_Float16{}); }
 
 static int linear_check(int64_t m, int64_t n, int64_t k, int act, int dtype) {
-    if (m < 0 || n < 0 || k < 0 || m >= LINEAR_MAX || n >= LINEAR_MAX || k >= LINEAR_MAX) return PLNLP_E_SHAPE;
-    // (workgroups of the three products)
-    const int64_t tm = (m + 127) / 128, tn = (n + 127) / 128, tk = (k + 127) / 128, most = (int64_t)1 << 30;
+    if (m < 0 || n < 0 || k < 0 || m >= LINEAR_MAX || n >= LINEAR_MAX_N || k >= LINEAR_MAX) return PLNLP_E_SHAPE;
+    // (a launch holds less than 2^32 threads: 256 for a tile of each of the three products, 64 for a column where columns are joined)
+    const int64_t tm = (m + 127) / 128, tn = (n + 127) / 128, tk = (k + 127) / 128, most = (int64_t)1 << 24;
     if (tm * tn >= most || tm * tk >= most || tn * tk >= most) return PLNLP_E_SHAPE;
     if (act < PLNLP_ACT_NONE || act > PLNLP_ACT_SILU) return PLNLP_E_UNSUPPORTED;
     if (dtype != PLNLP_DTYPE_BF16 && dtype != PLNLP_DTYPE_F16) return PLNLP_E_UNSUPPORTED;

@@ -482,6 +482,18 @@ def test_clip_views_alignment_and_neighbours(P):
         assert torch.equal(v, q)
 
 
+# more workgroups than one dimension of a grid takes (2^32 threads): rows too narrow to share one, too wide for several
+@gpu
+def test_lookup_of_many_rows(P):
+    n = 2 ** 26 + 5
+    table = rand((1000, 129), BF16, 8)
+    ids = torch.randint(0, 1000, (n,), generator=torch.Generator(device="cuda").manual_seed(9), device="cuda", dtype=torch.int32)
+    y = P.embedding_lookup(table, ids)
+    for lo in range(0, n, 2 ** 22):                      # (scale 1: copies)
+        part = y[lo:lo + 2 ** 22]
+        assert torch.equal(part, table[ids[lo:lo + 2 ** 22].long()]), lo
+
+
 @gpu
 def test_clip_refuses_what_it_would_scale_twice(P):
     a, b = rand((30, 8), BF16, 1), rand((20,), F32, 2)
@@ -712,6 +724,8 @@ def test_argument_checks_of_the_library():
     assert lin(d=0) == -4 and lin(act=9) == -4 and lin(m=-1) == -2 and lin(ldx=63) == -2 and lin(ldo=63) == -2 and lin(x=None) == -1 and lin(o=None) == -1
     assert lin(x=A + 1) == -3 and lin(b=A + 1) == -3 and lin(r=A, ldr=3) == -2 and lin(m=0) == 0
     assert lin(m=512, k=4096, ldx=4096, ldw=4096) == -5      # K is cut: the slices need their workspace
+    assert lin(m=2 ** 31) == -2 and lin(n=2 ** 26, ldo=2 ** 26) == -2 and lin(k=2 ** 31, ldx=2 ** 31, ldw=2 ** 31) == -2
+    assert lin(m=2 ** 25, n=2 ** 25, ldo=2 ** 25) == -2      # more tiles than a launch holds
     back = lambda **k: lib.plnlp_linear_act_backward(*{**dict(g=A, ldg=64, p=A, ldp=64, act=2, x=A, ldx=64, w=A, ldw=64, m=512, n=64, k=64, dx=A, lddx=64,
                                                               dw=A, lddw=64, db=A, d=1, ws=A, wb=10, st=None), **k}.values())
     assert back() == -5 and back(ws=None) == -5 and back(p=None) == -1 and back(lddx=3) == -2 and back(d=0) == -4 and back(g=None) == -1
