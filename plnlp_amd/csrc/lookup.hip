@@ -6,7 +6,7 @@
 //
 // The gradient takes no float atomics (their order would change its bits): the ids are SORTED -- (id, position) pairs, ties in
 // the order of the positions -- and the sorted list is cut into ranges of equal length, whatever the ids are.
-//   sort: up to SORT_SMALL ids in one workgroup's LDS (a bitonic network on unique 64-bit words: 1 launch); more in 1 .. 3
+//   sort: up to SORT_SMALL ids in one launch, each placed by counting the pairs before it (sort_small_kernel); more in 1 .. 3
 //     counting passes of at most 11 bits, each stable (histogram of the tiles / offsets along the tiles / scatter).  262 144 ids of
 //     a table of 235 868 rows, two passes: 33 us, six launches of 4 .. 9 us that wait for memory more than they move.
 //   runs: a group of lanes walks one range with eight rows of dy in flight, adds the rows of a run of equal ids and stores the row
@@ -18,7 +18,7 @@
 namespace plnlp {
 
 constexpr int LOOKUP_THREADS = 256;
-constexpr int SORT_SMALL = 4096;          // ids one workgroup sorts in LDS
+constexpr int SORT_SMALL = 8192;          // ids that are placed by counting, in one launch
 constexpr int SORT_BITS = 11;             // widest digit: 2048 counters a wave, 4 waves = 32 KiB of LDS
 
 template <typename I> __device__ __forceinline__ int64_t read_id(const I* ids, int64_t i) { return (int64_t)ids[i]; }
@@ -68,23 +68,67 @@ template <typename I> __device__ __forceinline__ uint32_t sort_key(const I* ids,
     return (id < 0 || id >= n_rows || id == padding) ? (uint32_t)n_rows : (uint32_t)id;
 }
 
-template <typename I, int N>
-__global__ __launch_bounds__(1024) void sort_small_kernel(const I* __restrict__ ids, int n, int64_t n_rows, int64_t padding,
-                                                          uint2* __restrict__ sorted) {
-    __shared__ uint64_t k[N];
-    for (int i = threadIdx.x; i < N; i += 1024)
-        k[i] = i < n ? ((uint64_t)sort_key(ids, i, n_rows, padding) << 32) | (uint32_t)i : ~0ull;
-    __syncthreads();
-    for (int size = 2; size <= N; size <<= 1)
-        for (int stride = size >> 1; stride > 0; stride >>= 1) {
-            for (int i = threadIdx.x; i < N / 2; i += 1024) {
-                const int a = 2 * i - (i & (stride - 1)), b = a + stride;
-                const uint64_t ka = k[a], kb = k[b];
-                if ((ka > kb) == ((a & size) == 0)) { k[a] = kb; k[b] = ka; }
-            }
-            __syncthreads();
+// The sort's launches wait for memory more than they move: further workgroups of them clear dE meanwhile (clear_first).  Bytes; a piece is
+// a row, or 8 KiB where the rows lie side by side.
+constexpr int CLEAR_PIECE = 8192;
+struct Clear {
+    char* at;
+    int64_t ld, width, total;          // of the pieces; the last one ends at `total`
+    int64_t pieces;
+    int unit, tx;                      // bytes a store, lanes a piece
+    int first, launch, launches;       // this launch's workgroups of the sort; its share of the pieces
+};
+__device__ void clear_share(const Clear& c) {
+    const int x = threadIdx.x & (c.tx - 1), y = threadIdx.x / c.tx, ty = blockDim.x / c.tx;
+    const int64_t per = (c.pieces + c.launches - 1) / c.launches, lo = per * c.launch, hi = min(lo + per, c.pieces);
+    for (int64_t p = lo + (int64_t)(blockIdx.x - c.first) * ty + y; p < hi; p += (int64_t)(gridDim.x - c.first) * ty) {
+        char* row = c.at + p * c.ld;
+        const int64_t n = min(c.width, c.total - p * c.ld);
+        for (int64_t b = (int64_t)x * c.unit; b < n; b += (int64_t)c.tx * c.unit) {
+            if (b + c.unit > n)                                        // (elements are two bytes at least)
+                for (int64_t e = b; e < n; e += 2) *reinterpret_cast<uint16_t*>(row + e) = 0;
+            else if (c.unit == 16) *reinterpret_cast<u32x4*>(row + b) = u32x4{0, 0, 0, 0};
+            else if (c.unit == 8) *reinterpret_cast<uint64_t*>(row + b) = 0;
+            else if (c.unit == 4) *reinterpret_cast<uint32_t*>(row + b) = 0;
+            else *reinterpret_cast<uint16_t*>(row + b) = 0;
         }
-    for (int i = threadIdx.x; i < n; i += 1024) sorted[i] = make_uint2((uint32_t)(k[i] >> 32), (uint32_t)k[i]);
+    }
+}
+
+// Up to SORT_SMALL ids: an id's place is the number of pairs that come before its own, counted.  A workgroup places 64 ids, one a lane;
+// its 16 waves share the keys, read from LDS by all lanes at once: before the ids' own positions equal keys count, behind them not.
+template <typename I>
+__global__ __launch_bounds__(1024) void sort_small_kernel(const I* __restrict__ ids, int n, int64_t n_rows, int64_t padding,
+                                                          uint2* __restrict__ sorted, Clear clear) {
+    if ((int)blockIdx.x >= clear.first) { clear_share(clear); return; }
+    __shared__ u32x4 keys[SORT_SMALL / 4];
+    __shared__ uint32_t part[16][64];
+    const uint32_t* k = reinterpret_cast<const uint32_t*>(keys);
+    const int quads = (n + 3) / 4;
+    for (int i = threadIdx.x; i < quads * 4; i += 1024)
+        reinterpret_cast<uint32_t*>(keys)[i] = i < n ? sort_key(ids, i, n_rows, padding) : ~0u;
+    __syncthreads();
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, i0 = blockIdx.x * 64, i = i0 + lane;
+    const uint32_t key = i < n ? k[i] : 0;
+    const int per = (quads + 15) / 16, hi = min((wave + 1) * per, quads), own = min(i0 / 4, hi), behind = min(i0 / 4 + 16, hi);
+    uint32_t before = 0;
+    int q = wave * per;
+#pragma unroll 4
+    for (; q < own; ++q)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) before += keys[q][j] <= key;
+    for (; q < behind; ++q)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) before += keys[q][j] < key + (4 * q + j < i);
+#pragma unroll 4
+    for (; q < hi; ++q)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) before += keys[q][j] < key;
+    part[wave][lane] = before;
+    __syncthreads();
+    if (wave || i >= n) return;
+    for (int w = 1; w < 16; ++w) before += part[w][lane];
+    sorted[before] = make_uint2(key, (uint32_t)i);
 }
 
 // One counting pass sorts by the digit (key >> shift) & (bins - 1).  A tile is 256 * ROUNDS ids; hist[tile][digit].
@@ -92,7 +136,8 @@ __global__ __launch_bounds__(1024) void sort_small_kernel(const I* __restrict__ 
 template <typename I, bool FIRST, int ROUNDS>
 __global__ __launch_bounds__(LOOKUP_THREADS) void sort_count_kernel(const I* __restrict__ ids, const uint2* __restrict__ in, int64_t n,
                                                                     int64_t n_rows, int64_t padding, int shift, int bins,
-                                                                    uint32_t* __restrict__ hist) {
+                                                                    uint32_t* __restrict__ hist, Clear clear) {
+    if ((int)blockIdx.x >= clear.first) { clear_share(clear); return; }
     extern __shared__ uint32_t cnt[];
     const int64_t lo = (int64_t)blockIdx.x * ROUNDS * LOOKUP_THREADS + threadIdx.x;
     uint32_t key[ROUNDS];
@@ -111,7 +156,9 @@ __global__ __launch_bounds__(LOOKUP_THREADS) void sort_count_kernel(const I* __r
 }
 
 // counts -> exclusive offsets along the tiles, and the digits' totals: 64 digits a workgroup, its 16 waves share the tiles
-__global__ __launch_bounds__(1024) void sort_offsets_kernel(uint32_t* __restrict__ hist, int tiles, int bins, uint32_t* __restrict__ total) {
+__global__ __launch_bounds__(1024) void sort_offsets_kernel(uint32_t* __restrict__ hist, int tiles, int bins, uint32_t* __restrict__ total,
+                                                            Clear clear) {
+    if ((int)blockIdx.x >= clear.first) { clear_share(clear); return; }
     __shared__ uint32_t part[16][64];
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, d = blockIdx.x * 64 + lane;
     const int per = (tiles + 15) / 16, lo = wave * per, hi = min(lo + per, tiles);
@@ -146,7 +193,8 @@ template <typename I, bool FIRST, int ROUNDS>
 __global__ __launch_bounds__(LOOKUP_THREADS) void sort_scatter_kernel(const I* __restrict__ ids, const uint2* __restrict__ in, int64_t n,
                                                                       int64_t n_rows, int64_t padding, int shift, int bits,
                                                                       const uint32_t* __restrict__ hist, const uint32_t* __restrict__ total,
-                                                                      uint2* __restrict__ out) {
+                                                                      uint2* __restrict__ out, Clear clear) {
+    if ((int)blockIdx.x >= clear.first) { clear_share(clear); return; }
     constexpr int WAVES = LOOKUP_THREADS / 64;
     extern __shared__ uint32_t lds[];                  // cnt[WAVES][bins]
     __shared__ uint32_t part[WAVES];
@@ -392,6 +440,7 @@ template <typename F> static int with_pack(int v, F&& f) {
 }
 template <typename F> static int with_id(int bytes, F&& f) { return bytes == 8 ? f(int64_t{}) : f(int32_t{}); }
 
+constexpr int64_t CLEAR_TWICE = (int64_t)192 << 20;
 constexpr int64_t LOOKUP_MAX = ((int64_t)1 << 31) - 2, LOOKUP_MAX_WIDTH = (int64_t)1 << 21;
 
 static int lookup_check(int64_t n_rows, int64_t width, int id_bytes, int64_t n_ids, int d0, int d1) {
@@ -408,6 +457,31 @@ static int grad_range(int64_t n, int64_t width) {
     int r = 16;
     while (r < 256 && (double)n * width > (double)r * 2048 * 512) r *= 2;
     return r;
+}
+
+// Is all of dE cleared in the sort's launches, instead of the rows without an id after it?  Rows with an id are then written twice: not
+// where most rows have one, or where there are more bytes of them than the sort hides.  (us, in the sort's launches / after them: 131 071
+// ids of 1 000 003 rows of 200 B 81 / 100, 4096 of 47 / 81; 180 000 of 235 868 rows of 1 KiB 127 / 132, but of 2 KiB 238 / 228; 131 072 of
+// 65 536 rows of 1 KiB 76 / 69)
+static bool clear_first(int64_t n_ids, int64_t n_rows, int64_t row_bytes) {
+    return 4 * n_ids <= 3 * n_rows && n_ids * row_bytes <= CLEAR_TWICE;
+}
+static Clear make_clear(void* grad, int64_t ld, int64_t width, int64_t n_rows) {
+    Clear c{};
+    c.at = (char*)grad;
+    c.total = (n_rows - 1) * ld + width;
+    const bool flat = ld == width;
+    c.ld = flat ? CLEAR_PIECE : ld;
+    c.width = flat ? CLEAR_PIECE : width;
+    c.pieces = flat ? (c.total + CLEAR_PIECE - 1) / CLEAR_PIECE : n_rows;
+    c.unit = 16;
+    while (((uintptr_t)grad | (uintptr_t)c.ld) & (c.unit - 1)) c.unit >>= 1;
+    c.tx = lanes_for((c.width + c.unit - 1) / c.unit, LOOKUP_THREADS);
+    return c;
+}
+static int clear_blocks(const Clear& c, int threads) {
+    const int64_t per = (c.pieces + c.launches - 1) / c.launches, rows = threads / c.tx;
+    return (int)std::min<int64_t>((per + rows - 1) / rows, 262144 / threads);
 }
 
 struct GradWorkspace { int64_t sorted[2], hist, total, head, tail, bytes; };
@@ -480,14 +554,21 @@ extern "C" int plnlp_embedding_grad(const void* gy, int64_t ldg, int gy_dtype, c
     char* ws = (char*)workspace;
     uint2* sorted[2] = {(uint2*)(ws + w.sorted[0]), (uint2*)(ws + w.sorted[1])};
     int cur = 0, rc = 0;
+    const int es = dtype_size(grad_dtype);
+    Clear clear = make_clear(grad, lde * es, width * es, n_rows);
+    const bool cleared = n_ids > 0 && clear_first(n_ids, n_rows, width * es);
+    // workgroups of a launch with `own` of its sort
+    auto with_clear = [&](int own, int threads) {
+        clear.first = own;
+        return dim3((unsigned)(own + (cleared ? clear_blocks(clear, threads) : 0)));
+    };
     if (n_ids && n_ids <= SORT_SMALL) {
+        clear.launches = 1;
+        const dim3 grid = with_clear((int)((n_ids + 63) / 64), 1024);
         rc = with_id(id_bytes, [&](auto it) {
             using I = decltype(it);
-            auto run = [&](auto kernel) {
-                hipLaunchKernelGGL(kernel, dim3(1), dim3(1024), 0, s, (const I*)ids, (int)n_ids, n_rows, padding_id, sorted[0]);
-                return launch_status();
-            };
-            return n_ids <= 256 ? run(sort_small_kernel<I, 256>) : n_ids <= 1024 ? run(sort_small_kernel<I, 1024>) : run(sort_small_kernel<I, SORT_SMALL>);
+            hipLaunchKernelGGL((sort_small_kernel<I>), grid, dim3(1024), 0, s, (const I*)ids, (int)n_ids, n_rows, padding_id, sorted[0], clear);
+            return launch_status();
         });
     } else if (n_ids) {
         int bits = 1;
@@ -497,6 +578,7 @@ extern "C" int plnlp_embedding_grad(const void* gy, int64_t ldg, int gy_dtype, c
         const int tiles = (int)((n_ids + tile - 1) / tile);
         uint32_t* hist = (uint32_t*)(ws + w.hist);
         uint32_t* total = (uint32_t*)(ws + w.total);
+        clear.launches = 3 * passes;
         for (int p = 0; p < passes && !rc; ++p) {
             const int shift = p * digit;
             rc = with_id(id_bytes, [&](auto it) {
@@ -504,11 +586,17 @@ extern "C" int plnlp_embedding_grad(const void* gy, int64_t ldg, int gy_dtype, c
                 auto pass = [&](auto first, auto count) {
                     constexpr bool F = decltype(first)::value;
                     constexpr int R = decltype(count)::value;
-                    hipLaunchKernelGGL((sort_count_kernel<I, F, R>), dim3(tiles), dim3(LOOKUP_THREADS), 4 * bins, s, (const I*)ids,
-                                       sorted[cur], n_ids, n_rows, padding_id, shift, bins, hist);
-                    hipLaunchKernelGGL(sort_offsets_kernel, dim3((bins + 63) / 64), dim3(1024), 0, s, hist, tiles, bins, total);
-                    hipLaunchKernelGGL((sort_scatter_kernel<I, F, R>), dim3(tiles), dim3(LOOKUP_THREADS), 4 * bins * (LOOKUP_THREADS / 64), s,
-                                       (const I*)ids, sorted[cur], n_ids, n_rows, padding_id, shift, digit, hist, total, sorted[cur ^ 1]);
+                    dim3 grid = with_clear(tiles, LOOKUP_THREADS);
+                    clear.launch = 3 * p;
+                    hipLaunchKernelGGL((sort_count_kernel<I, F, R>), grid, dim3(LOOKUP_THREADS), 4 * bins, s, (const I*)ids,
+                                       sorted[cur], n_ids, n_rows, padding_id, shift, bins, hist, clear);
+                    grid = with_clear((bins + 63) / 64, 1024);
+                    clear.launch = 3 * p + 1;
+                    hipLaunchKernelGGL(sort_offsets_kernel, grid, dim3(1024), 0, s, hist, tiles, bins, total, clear);
+                    grid = with_clear(tiles, LOOKUP_THREADS);
+                    clear.launch = 3 * p + 2;
+                    hipLaunchKernelGGL((sort_scatter_kernel<I, F, R>), grid, dim3(LOOKUP_THREADS), 4 * bins * (LOOKUP_THREADS / 64), s,
+                                       (const I*)ids, sorted[cur], n_ids, n_rows, padding_id, shift, digit, hist, total, sorted[cur ^ 1], clear);
                     return launch_status();
                 };
                 auto sized = [&](auto first) {
@@ -520,7 +608,7 @@ extern "C" int plnlp_embedding_grad(const void* gy, int64_t ldg, int gy_dtype, c
         }
     }
     if (rc) return rc;
-    const int gs = dtype_size(gy_dtype), es = dtype_size(grad_dtype);
+    const int gs = dtype_size(gy_dtype);
     const int v = n_ids ? pick_pack(width, gy, ldg, gs, grad, lde, es) : pick_pack(width, grad, lde, es, grad, lde, es);
     const int64_t packs = width / v;
     const int tx = lanes_for(packs, 64);
@@ -531,9 +619,8 @@ extern "C" int plnlp_embedding_grad(const void* gy, int64_t ldg, int gy_dtype, c
         const int64_t ranges = (n_ids + range - 1) / range, run_blocks = (ranges * slabs + ty - 1) / ty;
         const GradArgs<G, E, V> a{(const G*)gy, ldg, sorted[cur], n_ids, n_rows, (int)packs, tx, slabs, range, ranges, run_blocks,
                                   (float*)(ws + w.head), (float*)(ws + w.tail), scale, (E*)grad, lde};
-        const int64_t clear_blocks = (n_rows + CLEAR_ROWS - 1) / CLEAR_ROWS;
-        if (run_blocks + clear_blocks >= ((int64_t)1 << 31)) return PLNLP_E_SHAPE;
-        hipLaunchKernelGGL((grad_runs_kernel<G, E, V>), dim3((unsigned)(run_blocks + clear_blocks)), dim3(LOOKUP_THREADS), 0, s, a);
+        const int64_t clearing = cleared ? 0 : (n_rows + CLEAR_ROWS - 1) / CLEAR_ROWS;
+        hipLaunchKernelGGL((grad_runs_kernel<G, E, V>), dim3((unsigned)(run_blocks + clearing)), dim3(LOOKUP_THREADS), 0, s, a);
         if (int e = launch_status()) return e;
         if (ranges > 1) {
             hipLaunchKernelGGL((grad_joins_kernel<G, E, V>), dim3((unsigned)(ranges - 1), slabs), dim3(LOOKUP_THREADS), 0, s, a);

@@ -57,11 +57,11 @@ def lookup_grad_ref(gy, ids, v, scale, padding=None):
     return out, mag, torch.bincount(flat, minlength=v).double()[:, None]
 
 
-# widths: one element, odd, even without 16-byte rows, one pack, several packs a lane; ids: none, one, a wave, the last one sort
-# takes in LDS and the first it does not, several counting tiles
+# widths: one element, odd, even without 16-byte rows, one pack, several packs a lane; ids: none, one, a wave, the most that are
+# placed in one launch and one more, several counting tiles
 @gpu
 @pytest.mark.parametrize("n_ids,rows,width", [(0, 5, 8), (1, 1, 1), (1, 7, 3), (3, 300, 50), (64, 65, 64), (257, 1000, 8), (4096, 100, 33),
-                                              (4097, 3, 256), (5000, 70001, 40), (20000, 2047, 17), (20000, 2048, 24), (9000, 4200000, 2),
+                                              (4097, 3, 256), (5000, 70001, 40), (8192, 9001, 33), (8193, 40, 5), (20000, 2047, 17), (20000, 2048, 24), (9000, 4200000, 2),
                                               (70000, 500, 1100)])
 @pytest.mark.parametrize("table_t,out_t,id_t", [(BF16, BF16, torch.int64), (F16, F16, torch.int32), (F32, BF16, torch.int32), (F32, F32, torch.int64)])
 def test_lookup(P, n_ids, rows, width, table_t, out_t, id_t):
@@ -480,6 +480,29 @@ def test_clip_views_alignment_and_neighbours(P):
     assert float(P.clip_grads(plain, 0.1)) == float(n)
     for v, q in zip(views, plain):
         assert torch.equal(v, q)
+
+
+# rows of the gradient apart from each other and at every alignment; dE cleared beside the sort (few ids) or behind it (many); what lies
+# between the rows and around them stays
+@gpu
+@pytest.mark.parametrize("n_ids,rows", [(0, 70), (5, 700), (60, 70), (9000, 30000), (9000, 300)])
+@pytest.mark.parametrize("width,ld,shift", [(8, 8, 0), (7, 7, 0), (7, 7, 1), (24, 32, 0), (33, 40, 3), (64, 66, 2), (5, 4100, 1)])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_lookup_gradient_between_other_memory(P, n_ids, rows, width, ld, shift, dtype):
+    from plnlp_amd import _lib as L
+    lib, code = L.load(), L.DTYPE_CODES[dtype]
+    g = torch.Generator(device="cuda").manual_seed(rows + width)
+    ids = torch.randint(-1, rows + 1, (n_ids,), generator=g, device="cuda")
+    gy = rand((n_ids, width), dtype, 3)
+    memory = torch.full((rows * ld + 64,), 7.0, dtype=dtype, device="cuda")
+    ws = torch.empty(lib.plnlp_embedding_grad_workspace_bytes(n_ids, width) + 16, dtype=torch.uint8, device="cuda")
+    grad = memory[shift:shift + rows * ld].view(rows, ld)
+    for _ in range(2):                                      # (over the first call's result as well)
+        L.check(lib.plnlp_embedding_grad(gy.data_ptr(), width, code, ids.data_ptr(), 8, n_ids, 2, 0.5, grad.data_ptr(), ld, code, rows, width,
+                                         ws.data_ptr(), ws.numel(), L.stream_ptr()), "grad")
+        ref, mag, count = lookup_grad_ref(gy, ids, rows, 0.5, padding=2)
+        within(grad[:, :width], ref, ref.abs() * U[dtype] + mag * (count + 4) * ADD + TINY[dtype])
+        assert bool((grad[:, width:] == 7).all()) and bool((memory[:shift] == 7).all()) and bool((memory[shift + rows * ld:] == 7).all())
 
 
 # more workgroups than one dimension of a grid takes (2^32 threads): rows too narrow to share one, too wide for several
