@@ -863,8 +863,11 @@ static bool units_ok(const void* p, int64_t ld, int64_t along) { return (uintptr
 // Tile shape and K slices of a product.  256 x 256 tiles read LDS and the caches half as often an MFMA as 128 x 128 ones, but one
 // workgroup of them fills a CU: they are taken where they leave less than an eighth of their area empty and make at least three
 // quarters of the chip's 256 workgroups, alone or with K cut into slices of at least 24 steps.  Else 128 x 128: alone
-// where they make three quarters of a workgroup a CU (4096 x 1024 x 1024: 20 us, in two slices 32), else with K cut until two
-// workgroups a CU have work, into slices of at least four steps.  (us: 8192 x 4096 x 4096 258 against 345; dW of 4096 x 4000 over 8192
+// where they make three quarters of a workgroup a CU (4096 x 1024 x 1024: 20 us, in two slices 32), else with K cut: a step takes a lone
+// workgroup about 0.7 us and 2^18 sums of a slice, written and read again, about 0.4, which s = sqrt(1.75 steps / (m n / 2^18)) slices
+// balance -- two steps a slice at least, two workgroups a CU at most.  (us, so / with four steps a slice: 300 x 300 x 300 9.7 / 12.1,
+// 1024 x 1024 x 1024 16.5 / 19.9, 2048 x 512 x 512 12.3 / 14.6, 1000 x 256 x 2048 14.1 / 14.2; / with twice as many: 9.7, 20.0, 14.7,
+// 15.2)  (us: 8192 x 4096 x 4096 258 against 345; dW of 4096 x 4000 over 8192
 // rows 230 against 372; of 2048 x 1024 over 16384 rows, eight slices, 83 against 107)
 struct Plan { bool big; int tiles_m, tiles_n, slices, steps; };
 static Plan plan_product(int64_t m, int64_t n, int64_t k, int terms = 1) {
@@ -878,7 +881,8 @@ static Plan plan_product(int64_t m, int64_t n, int64_t k, int terms = 1) {
     p.tiles_n = (int)tiles(n, b);
     const int64_t t = (int64_t)p.tiles_m * p.tiles_n;
     int64_t s = p.big ? cut : t == 0 || t >= 192 ? 1 : 512 / t;
-    s = std::max<int64_t>(1, std::min(s, steps / 4));
+    const int64_t balanced = (int64_t)std::sqrt(1.75 * (double)steps * 262144.0 / std::max(1.0, (double)m * (double)n));
+    s = std::max<int64_t>(1, std::min(s, p.big ? steps / 4 : std::min(steps / 2, balanced)));
     p.steps = (int)((steps + s - 1) / s);
     p.slices = p.steps ? (int)((steps + p.steps - 1) / p.steps) : 1;
     if (p.slices < 1) p.slices = 1;
