@@ -8,7 +8,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libplnlp_hip.so")
 SOURCES = ["csr_aggregate.hip", "csr_aggregate_max.hip", "gemm_f32.hip", "edge_ops.hip", "train_ops.hip", "incidence.hip",
-           "host_perm.hip", "launch_log.hip"]
+           "host_perm.hip", "launch_log.hip", "lookup.hip", "linear_act.hip", "grad_clip.hip"]
 
 
 def needs_build() -> bool:
@@ -40,10 +40,9 @@ def build(force: bool = False, verbose: bool = False) -> str:
     units.append(("gemm_wgw.hip", "gemm_wgw.o", ["-fno-slp-vectorize"]))
     units.append(("gemm_x3b.hip", "gemm_x3b.o", ["-fno-slp-vectorize"]))
     units.append(("aggregate_dense.hip", "aggregate_dense.o", ["-fno-slp-vectorize"]))
-    # (-packed-fp32-ops: the two-lane f32 instructions are not to be formed from these kernels' f32 arithmetic; the host pass
-    # warns that it does not know the feature)
+    # (-packed-fp32-ops: the two-lane f32 instructions are not to be formed from the kernels' f32 arithmetic; the host pass warns
+    # that it does not know the feature.  bench.py's step with it and without: 1.537 / 1.539 ms)
     no_packed = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
-    units += [(src, src.replace(".hip", ".o"), no_packed) for src in ("lookup.hip", "linear_act.hip", "grad_clip.hip")]
     headers = [os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith(".h")]
     headers.append(os.path.join(os.path.dirname(HERE), "include", "plnlp_hip.h"))
     newest_header = max(os.path.getmtime(h) for h in headers)
@@ -56,7 +55,7 @@ def build(force: bool = False, verbose: bool = False) -> str:
                 and os.path.getmtime(obj) >= max(os.path.getmtime(os.path.join(CSRC, src)), newest_header)):
             continue
         cmd = [hipcc, "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-x", "hip", "-c",
-               os.path.join(CSRC, src), "-o", obj] + extra
+               os.path.join(CSRC, src), "-o", obj] + no_packed + extra
         if verbose:
             cmd.insert(1, "-Rpass-analysis=kernel-resource-usage")
         procs.append((src, obj, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)))
