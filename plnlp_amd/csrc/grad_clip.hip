@@ -7,7 +7,7 @@
 //     684 M bf16 elements in 73 tensors: 272 us, 5.0 TB/s.
 //   pass 2 (clip_kernel):  each workgroup adds ALL partials in the same fixed order (a few KiB out of L2), so c needs no launch
 //     of its own, no counter and no atomic: the same bits every run, and nothing that two streams or two graphs could share.
-//     The same tensors, in place: 535 us, 5.1 TB/s read and written (a copy of 2 GiB: 4.9).
+//     The same tensors into others of their type: 535 us, 5.1 TB/s read and written (a copy of 2 GiB: 4.9).
 // The tensors travel in the kernel's arguments (CLIP_LAUNCH a launch), so a captured graph holds them by value.
 #include "half.hip.h"
 
