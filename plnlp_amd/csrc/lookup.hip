@@ -8,7 +8,7 @@
 // the order of the positions -- and the sorted list is cut into ranges of equal length, whatever the ids are.
 //   sort: up to SORT_SMALL ids in one launch, each placed by counting the pairs before it (sort_small_kernel); more in 1 .. 3
 //     counting passes of at most 11 bits, each stable (histogram of the tiles / offsets along the tiles / scatter).  262 144 ids of
-//     a table of 235 868 rows, two passes: 33 us, six launches of 4 .. 9 us that wait for memory more than they move.
+//     a table of 235 868 rows, two passes: 34 us, six launches of 4 .. 9 us that wait for memory more than they move.
 //   runs: a group of lanes walks one range with eight rows of dy in flight, adds the rows of a run of equal ids and stores the row
 //     of dE when the run ends.  A run that crosses the ends of its range leaves an f32 partial there instead; the range in which
 //     it begins adds those up in order (grad_joins_kernel).  So a frequent id costs what its rows cost, spread over the chip.
