@@ -643,6 +643,16 @@ def test_captured_and_replayed(P, n, width):
 
 
 @gpu
+def test_gradients_of_gradients_are_refused(P):
+    x, w, table = rand((5, 8), BF16, 1).requires_grad_(True), rand((4, 8), BF16, 2).requires_grad_(True), rand((7, 8), BF16, 3).requires_grad_(True)
+    for y, leaf in ((P.linear_act(x, w, activation="silu"), x), (P.embedding_lookup(table, torch.arange(3, device="cuda")), table)):
+        g, = torch.autograd.grad(y.float().square().sum(), [leaf], create_graph=True)      # (allowed: the gradient itself is right)
+        assert bool(torch.isfinite(g).all())
+        with pytest.raises(RuntimeError):
+            torch.autograd.grad(g.float().sum(), [leaf])
+
+
+@gpu
 def test_two_streams_at_once(P):
     """the same calls on two streams, each with its own tensors, give what one stream gives"""
     def work(seed):
