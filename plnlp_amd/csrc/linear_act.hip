@@ -149,7 +149,7 @@ template <typename T> struct TileArgs {
     int64_t  plane;                                // P's second term lies this many elements behind its first
     int      terms;                                // 1, or 2: C = (P + P2) Q^T as one sum over twice as many steps
     int      tiles_m, tiles_n, slices, steps;      // steps: BK-steps per slice
-    float*   sums;                                 // nullable [slices, m]: sum_k P(m, k) of each slice (PT)
+    float*   sums;                                 // nullable [slices, m]: sum_k P(m, k) of each slice (PT, tiles of 128 x 128)
     float*   partial;                              // slices > 1: [slices, m, n]
     Finish<T> fin;
 };
@@ -306,7 +306,7 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void tile_kernel(TileArgs<T> a) {
         for (int t = 0; t < 4; ++t) acc[i][t] = f32x4{0.f, 0.f, 0.f, 0.f};
 
     // sums over k of P, the bias gradient where P is dz: one more product, with a Q of ones, in the waves of the first column tile
-    constexpr bool SUMS = PT && BM == 128;      // (a result large enough for 256 x 256 tiles comes with its dz summed already)
+    constexpr bool SUMS = PT && BM == 128;      // (large_tiles)
     const bool sum_p = SUMS && a.sums && n0 == 0 && wn == 0;
     f32x4 psum[SUMS ? TM : 1];
     frag ones;
@@ -938,6 +938,15 @@ template <typename T, bool QT, bool SLOPED, int ACT> static int run_rows(int ks,
     return launch_rows<T, 8, QT, SLOPED, ACT>(a, s);
 }
 
+// how the tile kernel reads a product's operands (32-bit offsets inside a tile; an operand with k along its rows needs a whole step of them)
+static int product_mode(bool vec, bool pt, const void* p, int64_t ldp, bool qt, const void* q, int64_t ldq, int64_t m, int64_t n, int64_t k) {
+    if (vec && ldp < ((int64_t)1 << 22) && ldq < ((int64_t)1 << 22) && (k >= BK || !(pt || qt)) && k > 0 &&
+        units_ok(p, ldp, pt ? m : k) && units_ok(q, ldq, qt ? n : k)) return ALIGNED;
+    return k >= BK && (!pt || m >= 8) && (!qt || n >= 8) ? LOOSELY : BY_ELEMENT;
+}
+// does it run on 256 x 256 tiles?  (Those take no TileArgs::sums: who wants them asks here first.)
+static bool large_tiles(const Plan& pl, int mode) { return pl.big && mode == ALIGNED; }
+
 // C = P Q^T on the tile kernel, with its finish (ACT: the activation of the finish)
 template <typename T, bool PT, bool QT, int ACT>
 static int product(const T* p, int64_t ldp, int64_t plane, const T* q, int64_t ldq, int64_t m, int64_t n, int64_t k, const Finish<T>& fin,
@@ -945,14 +954,10 @@ static int product(const T* p, int64_t ldp, int64_t plane, const T* q, int64_t l
     const int terms = plane ? 2 : 1;
     const Plan pl = plan_product(m, n, k, terms);
     TileArgs<T> a{p, q, ldp, ldq, m, n, k, plane, terms, pl.tiles_m, pl.tiles_n, pl.slices, pl.steps, sums, partial, fin};
-    // (32-bit offsets inside a tile; an operand with k along its rows needs a whole step of them)
-    int mode = BY_ELEMENT;
-    if (fin.vec && ldp < ((int64_t)1 << 22) && ldq < ((int64_t)1 << 22) && (k >= BK || !(PT || QT)) && k > 0 &&
-        units_ok(p, ldp, PT ? m : k) && units_ok(q, ldq, QT ? n : k)) mode = ALIGNED;
-    else if (k >= BK && (!PT || m >= 8) && (!QT || n >= 8)) mode = LOOSELY;
+    const int mode = product_mode(fin.vec, PT, p, ldp, QT, q, ldq, m, n, k);
     auto run = [&](auto act) {
         constexpr int A = decltype(act)::value;
-        if (pl.big && mode == ALIGNED) return launch_tile<T, 256, 256, 2, 4, PT, QT, ALIGNED, A>(a, s);
+        if (large_tiles(pl, mode)) return launch_tile<T, 256, 256, 2, 4, PT, QT, ALIGNED, A>(a, s);
         if (pl.big) { a.tiles_m = (int)((m + 127) / 128); a.tiles_n = (int)((n + 127) / 128); }
         return mode == ALIGNED ? launch_tile<T, 128, 128, 2, 2, PT, QT, ALIGNED, A>(a, s)
              : mode == LOOSELY ? launch_tile<T, 128, 128, 2, 2, PT, QT, LOOSELY, A>(a, s)
@@ -1102,10 +1107,13 @@ extern "C" int plnlp_linear_act_backward(const void* gy, int64_t ldg, const int1
         const bool want_dx = dx && m > 0 && k > 0, want_dw = dw && n > 0 && k > 0;
         const bool vec = units_ok(gy, ldg, n) && (!has_act || units_ok(slope, lds, n));
         // many rows and weights that fit LDS: dz and its column sums are formed on the way to dx; without an activation dz is dy and
-        // its sums come with dw
+        // its sums come with dw, unless so many rows sum up to few results that dw takes the large tiles (393 216 rows of 256 x 256)
         const Finish<T> fin_x = make_finish<T>(nullptr, nullptr, 0, nullptr, 0, dx, lddx, k);
+        const Finish<T> fin_w = make_finish<T>(nullptr, nullptr, 0, nullptr, 0, dw, lddw, k);
         const int ks = want_dx && vec && !plane && fin_x.vec && (uintptr_t)w % 8 == 0 && ldw % 4 == 0 ? rows_fit(m, k, n, has_act ? 256 : 512) : 0;
-        const bool sums_in_dx = ks && has_act, sums_in_dw = ks && !has_act && want_dw;
+        const bool sums_in_dx = ks && has_act;
+        const bool sums_in_dw = ks && !has_act && want_dw &&
+                                !large_tiles(plan_product(n, k, m), product_mode(fin_w.vec, true, dz, ldz, true, x, ldx, n, k, m));
         int64_t sum_blocks = m > 0 ? b.blocks : 0;
         if (m > 0 && n > 0 && ((has_act && !ks) || (db && !sums_in_dx && !sums_in_dw))) {
             const int64_t packs = vec ? n / 8 : n;
@@ -1129,9 +1137,8 @@ extern "C" int plnlp_linear_act_backward(const void* gy, int64_t ldg, const int1
             if (int e = product<T, false, true, PLNLP_ACT_NONE>(dz, ldz, plane, (const T*)w, ldw, m, k, n, fin_x, partial, s)) return e;
         }
         if (want_dw) {
-            const Finish<T> fin = make_finish<T>(nullptr, nullptr, 0, nullptr, 0, dw, lddw, k);
             if (sums_in_dw) sum_blocks = b.slices;
-            if (int e = product<T, true, true, PLNLP_ACT_NONE>(dz, ldz, plane, (const T*)x, ldx, n, k, m, fin, partial, s,
+            if (int e = product<T, true, true, PLNLP_ACT_NONE>(dz, ldz, plane, (const T*)x, ldx, n, k, m, fin_w, partial, s,
                                                                sums_in_dw && db ? sums : nullptr)) return e;
         }
         if (db && n > 0) {
