@@ -69,3 +69,33 @@ def test_bias_gradient_of_very_many_rows_through_the_layer(P):
     dx, dw, db = torch.autograd.grad(layer(x), [x, layer.lin.weight, layer.lin.bias], gy)
     assert torch.equal(db, gy.float().sum(0).to(BF16))
     assert torch.equal(dw, (gy.float().t() @ x.detach().float()).to(BF16))
+
+
+# The sums over rows (dw, db) and over columns (dx) bit for bit, so that a lost K slice, tile, last step or workgroup's part shows: each
+# kernel that takes them (tiles of 128 and 256, rows in LDS or streamed, column sums beside dx, beside dw or on their own), whole and
+# ragged rows.  With relu a slope of 1 is written down; without an activation none is read.
+@gpu
+@pytest.mark.parametrize("m,n,k", [(777, 520, 136), (16384, 1024, 512), (16390, 1280, 576), (12552, 1000, 1032), (1792, 8200, 520), (32770, 256, 256),
+                                   (33800, 264, 96), (34000, 72, 264), (65537, 512, 64), (8300, 72, 520), (8209, 33, 64), (131072, 256, 256),
+                                   (40001, 200, 200)])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("act", ["none", "relu"])
+def test_sums_of_whole_numbers(P, m, n, k, dtype, act):
+    slope = torch.full((m, n), 1 << 14, dtype=torch.int16, device="cuda") if act == "relu" else None
+    got, want = backward_of_whole_numbers(P, m, n, k, dtype, act, slope)
+    for name, a, b in zip(("dx", "dw", "db"), got, want):
+        assert torch.equal(a, b), name
+
+
+@gpu
+@pytest.mark.parametrize("m,n,k,act", [(16384, 1024, 512, "silu"), (32770, 256, 256, "gelu"), (65537, 512, 64, "none"), (777, 515, 1003, "gelu_tanh"),
+                                       (1, 4096, 4096, "silu"), (40001, 200, 200, "silu")])
+def test_the_same_bits_twice(P, m, n, k, act):
+    x, w, b = (torch.randn(s, generator=generator(i), device="cuda").to(BF16).requires_grad_(True) for i, s in enumerate(((m, k), (n, k), (n,))))
+    gy = torch.randn((m, n), generator=generator(9), device="cuda").to(BF16)
+
+    def run():
+        y = P.linear_act(x, w, b, activation=act)
+        return [y.detach(), *torch.autograd.grad(y, [x, w, b], gy)]
+    for u, v in zip(run(), run()):
+        assert torch.equal(u, v)
