@@ -659,7 +659,8 @@ int plnlp_embedding_grad(const void* gy, int64_t ldg, int gy_dtype, const void* 
 /* out = act(x w^T + bias) + residual for x [m, k], w [n, k] (nn.Linear's layout), bias [n] (nullable), residual [m, n] (nullable),
  * all of one 16-bit type (dtype BF16 or F16), rows ld* elements apart, any alignment of whole elements; 16-byte aligned rows
  * and k, n % 8 == 0 take the wide loads.  m, k < 2^31, n < 2^26, and less than 2^24 tiles of 128 x 128 in each of [m, n],
- * [m, k] and [n, k].  slope (nullable): act'(x w^T + bias), what the backward pass reads, int16 in steps of 2^-14 (20000: NaN).
+ * [m, k] and [n, k].  slope (nullable): act'(x w^T + bias), what the backward pass reads, as int16 q:
+ * q 2^-14 for q > -5120 (20000: NaN), else the float of bits (q << 14) + 0xc2000000, which is in [-2^-5, -2^-59] (a relative 2^-10).
  * out may be residual itself (same rows); otherwise outputs alias nothing.  workspace: plnlp_linear_act_workspace_bytes(m, n, k)
  * bytes, 16-byte aligned (0: none needed). */
 int64_t plnlp_linear_act_workspace_bytes(int64_t m, int64_t n, int64_t k);

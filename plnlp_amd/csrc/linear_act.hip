@@ -2,9 +2,10 @@
 //   z = x W^T + bias;  y = act(z) + residual;   dz = dy * act'(z);  dx = dz W;  dW = dz^T x;  db = sum_rows dz;  d residual = dy
 // Products on the matrix cores with f32 accumulation; bias, activation and residual on the f32 accumulators, ONE rounding to the
 // stored type.  What is rounded besides:
-//   act'(z), kept for the backward pass as 16-bit FIXED point in steps of 2^-14 (|act'| <= 1.13): an absolute 2^-15, a sixth of what
-//     rounding z to fp16 (a fiftieth of what rounding it to bf16) would do to dz, for the same bytes -- and the backward pass evaluates
-//     no exponential;
+//   act'(z), kept for the backward pass in the 16 bits z itself would take, so that it evaluates no exponential: FIXED point in steps of
+//     2^-14 (|act'| <= 1.13), an absolute 2^-15, around |z| = 1 a sixth of what rounding z to fp16 (a fiftieth of what rounding it to
+//     bf16) would do to dz; and where a unit is saturated (-2^-5 < act' < 0: z below -2.6 for gelu, -4.8 for silu) ten bits of
+//     significand, a relative 2^-10 down to 2^-59, so that the gradients of a layer whose units all are keep their digits;
 //   dz, which the two gradient products read as 16-bit operands: an error of the size of the result's own rounding, averaged over
 //     the sums.  A small dz (see TWO_TERMS) is kept as the sum of two 16-bit terms instead, its few roundings would not average.
 //
@@ -80,14 +81,24 @@ template <int ACT, bool SLOPE> __device__ __forceinline__ float act_of(float z, 
     }
     return z;
 }
-// the slope in steps of 2^-14: adding 1.5 * 2^23 rounds to a whole number and leaves it in the low bits; a NaN becomes SLOPE_NAN, which
-// no slope reaches (the smaller of a NaN and a number is the number)
+// The slope in 16 bits.  Mostly in steps of 2^-14: adding 1.5 * 2^23 rounds to a whole number and leaves it in the low bits; a NaN becomes
+// SLOPE_NAN, which no slope reaches (the smaller of a NaN and a number is the number).  -2^-5 <= slope < 0 is the f32's own sign, exponent
+// and first nine bits, rounded: its upper 18 bits less those of -2^-59, counted up from -32768.  They end at -5120; the steps of the other
+// negative slopes (gelu's reach -0.13) begin at -2121.  What lies between -2^-59 and 0 is 0, in steps.  (us, with the
+// relative form / without: 131 072 x 256 x 256 with gelu forward 76 / 73, backward 131 / 128; 8192 x 4096 x 4096 309 / 308, 544 / 544)
 constexpr float SLOPE_STEP = 1.f / 16384.f;
 constexpr int SLOPE_NAN = 20000;
+constexpr uint32_t SLOPE_TAIL = 0xa2000000u + ((uint32_t)32768 << 14);     // bits of -2^-59, less the shifted -32768 they are kept as
+constexpr int SLOPE_TAIL_LO = -32767, SLOPE_TAIL_HI = -5120;
 __device__ __forceinline__ int16_t pack_slope(float s) {
-    return (int16_t)__float_as_uint(fminf(fmaf(s, 16384.f, 12582912.f), 12582912.f + SLOPE_NAN));
+    const int tail = (int)(__float_as_uint(s) - SLOPE_TAIL + (1u << 13)) >> 14;
+    const int steps = (int)__float_as_uint(fminf(fmaf(s, 16384.f, 12582912.f), 12582912.f + SLOPE_NAN));
+    return (int16_t)((uint32_t)(tail - SLOPE_TAIL_LO) <= (uint32_t)(SLOPE_TAIL_HI - SLOPE_TAIL_LO) ? tail : steps);
 }
-__device__ __forceinline__ float unpack_slope(int16_t q) { return q == SLOPE_NAN ? __builtin_nanf("") : (float)q * SLOPE_STEP; }
+__device__ __forceinline__ float unpack_slope(int16_t q) {
+    const float tail = __uint_as_float(((uint32_t)(int)q << 14) + SLOPE_TAIL);
+    return q <= SLOPE_TAIL_HI ? tail : q == SLOPE_NAN ? __builtin_nanf("") : (float)q * SLOPE_STEP;
+}
 // f(std::integral_constant<int, ACT>{}) of a run-time activation
 template <typename F> __host__ __device__ __forceinline__ int with_act(int act, F&& f) {
     switch (act) {

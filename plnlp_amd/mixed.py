@@ -128,7 +128,7 @@ def embedding_lookup(table: torch.Tensor, ids: torch.Tensor, *, scale: float = 1
 # ------------------------------------------------------------------ linear ------
 def _linear_forward(x, weight, bias, residual, act: int, keep: bool):
     """(y [m, n], slope or None) of matrices as _rows gives them; the activation's derivative is kept where the backward pass will
-    read it: int16 [m, n] in steps of 2^-14"""
+    read it: int16 [m, n], as plnlp_linear_act codes it"""
     stream = _stream(x, weight, bias, residual)
     lib = L.load()
     m, k = x.shape
@@ -182,7 +182,8 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tenso
     x: [..., K]; weight: [N, K] (torch.nn.Linear's layout); bias: [N]; residual: the result's shape [..., N]; all bf16 or all
     fp16.  activation: "none", "relu", "gelu" (z Phi(z)), "gelu_tanh" or "silu".  The product is summed in fp32; bias,
     activation and residual act on the fp32 sums, which are rounded once.  The activation's derivative is kept
-    for the backward pass in steps of 2^-14, where a gradient is wanted.
+    for the backward pass in 16 bits, where a gradient is wanted: in steps of 2^-14, and between -2^-5 and 0 (saturated units) to
+    2^-10 of itself.
     fp32 matrices are the business of ops.LinearFn."""
     dtype = x.dtype
     if dtype not in _HALF:

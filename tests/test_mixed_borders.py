@@ -99,3 +99,51 @@ def test_the_same_bits_twice(P, m, n, k, act):
         return [y.detach(), *torch.autograd.grad(y, [x, w, b], gy)]
     for u, v in zip(run(), run()):
         assert torch.equal(u, v)
+
+
+# ------------------------------------------------------------------ saturated units ------
+def slope_ref(z, name):
+    if name == "silu":
+        s = torch.sigmoid(z)
+        return s * (1 + z * (1 - s))
+    if name == "gelu":
+        return 0.5 * torch.special.erfc(-z * math.sqrt(0.5)) + z * torch.exp(-z * z / 2) / math.sqrt(2 * math.pi)
+    c, a = math.sqrt(2 / math.pi), 0.044715
+    s = torch.sigmoid(2 * c * (z + a * z ** 3))          # (1 + tanh) / 2 without its cancellation
+    return s + z * s * torch.sigmoid(-2 * c * (z + a * z ** 3)) * 2 * c * (1 + 3 * a * z * z)
+
+
+# Every unit far on the flat side, where the derivative is 10^-2 .. 10^-9: the gradients in RELATIVE terms.  The kept derivative is off by
+# 2^-10 of itself there; the f32 exponentials (arguments below 64: 64 * 2^-23 * ln 2) and the fitted normal distribution (1.2e-5, in a sum
+# that it is an eighth of) by less than 2e-5; z itself by e_z, which the derivative's logarithm follows at a rate below 10 (gelu: |z|;
+# gelu_tanh: 1.6 (1 + 0.13 z^2); silu: 1).  dz is rounded to the type before dx and dw are taken, db sums it unrounded; what
+# remains of each is the sums' f32 additions and one rounding.  gy and x are positive: nothing cancels in dw and db.
+@gpu
+@pytest.mark.parametrize("act,center,spread,dtype,gain", [("gelu", -4.0, 0.15, BF16, 1.0), ("gelu", -5.5, 0.2, BF16, 1.0), ("gelu", -4.2, 0.1, F16, 512.0),
+                                                          ("gelu_tanh", -4.0, 0.2, BF16, 1.0), ("gelu_tanh", -5.0, 0.1, BF16, 1.0),
+                                                          ("silu", -6.0, 0.3, BF16, 1.0), ("silu", -10.0, 0.5, BF16, 1.0), ("silu", -22.0, 1.0, BF16, 1.0),
+                                                          ("silu", -10.0, 0.5, F16, 512.0)])
+@pytest.mark.parametrize("m,n,k", [(4, 64, 64), (40, 96, 64), (300, 136, 72), (300, 131, 77), (8200, 200, 72), (8192, 256, 256)])
+def test_gradients_of_saturated_units(P, act, center, spread, dtype, gain, m, n, k):
+    u, tiny = U[dtype], TINY[dtype]
+    x = (0.5 + torch.rand((m, k), generator=generator(1), device="cuda")).to(dtype).requires_grad_(True)
+    w = (torch.randn((n, k), generator=generator(2), device="cuda") * spread / math.sqrt(k)).to(dtype).requires_grad_(True)
+    b = torch.full((n,), center, dtype=dtype, device="cuda", requires_grad=True)
+    gy = ((0.5 + torch.rand((m, n), generator=generator(3), device="cuda")) * gain).to(dtype)
+    xd, wd, g = x.detach().double(), w.detach().double(), gy.double()
+    z = xd @ wd.t() + b.detach().double()
+    assert -30 < float(z.min()) and float(z.max()) < -2.5 and bool((slope_ref(z, act) < 0).all())
+    e_z = (xd.abs() @ wd.abs().t()) * (k + 2) * ADD + z.abs() * ADD
+    dz = g * slope_ref(z, act)
+    relative = 2.0 ** -10 + 2e-5 + 10 * e_z
+    e_sum = dz.abs() * relative                                    # of the dz that db sums
+    e_dz = dz.abs() * (relative + u * 1.01) + tiny                 # of the rounded one
+    dx, dw, db = torch.autograd.grad(P.linear_act(x, w, b, activation=act), [x, w, b], gy)
+    for name, got, want, bound in (("db", db, dz.sum(0), e_sum.sum(0) + dz.abs().sum(0) * (m + 2) * ADD),
+                                   ("dw", dw, dz.t() @ xd, e_dz.t() @ xd.abs() + (dz.t().abs() @ xd.abs()) * (m + 2) * ADD),
+                                   ("dx", dx, dz @ wd, e_dz @ wd.abs() + (dz.abs() @ wd.abs()) * (n + 2) * ADD)):
+        bound = bound + want.abs() * u * 1.01 + tiny
+        over = (got.double() - want).abs() - bound
+        assert not bool(torch.isnan(over).any()) and float(over.max()) <= 0.0, (name, float(((got.double() - want).abs() / want.abs()).max()))
+        if name != "dx":                                           # the bounds say something: within 2 % of what they bound
+            assert float((bound / want.abs()).median()) <= 0.02, name
