@@ -631,8 +631,9 @@ int plnlp_transpose_f32(const float* x, int64_t ldx, float* y, int64_t ldy,
 
 /* ---- 16-bit storage: rows by id, a linear layer, gradient clipping (csrc/lookup.hip, linear_act.hip, grad_clip.hip) ------
  * Additions within ABI 12 (nothing that was there changed).  Tensors may be f32, bf16 or f16 (PLNLP_DTYPE_*); every sum is
- * held in f32 or f64 and every result is rounded once, to nearest even.  All entry points are deterministic, keep no state
- * between calls and may be captured into a hipGraph (fill and copy nodes are never recorded). */
+ * held in f32 or f64 and every result is rounded once, to nearest even; plnlp_linear_act_backward says what it rounds besides.  All
+ * entry points are deterministic, keep no state between calls and may be captured into a hipGraph (fill and copy nodes are never
+ * recorded). */
 #define PLNLP_DTYPE_F32  0
 #define PLNLP_DTYPE_BF16 1
 #define PLNLP_DTYPE_F16  2
@@ -668,7 +669,8 @@ int plnlp_linear_act(const void* x, int64_t ldx, const void* w, int64_t ldw, con
                      int act, int64_t m, int64_t n, int64_t k, int16_t* slope, int64_t lds, void* out, int64_t ldo, int dtype,
                      void* workspace, int64_t workspace_bytes, void* stream);
 /* its gradients from gy = d out: dz = gy * slope; dx = dz w, dw = dz^T x, db = column sums of dz (each nullable: not wanted);
- * the residual's gradient is gy itself.  act NONE: slope is not read.  workspace as above, by its own byte count. */
+ * the residual's gradient is gy itself.  For dx and dw, dz is rounded to the type (m n <= 16384: kept as two terms of it); act NONE: slope
+ * is not read and nothing is rounded.  workspace as above, by its own byte count. */
 int64_t plnlp_linear_act_backward_workspace_bytes(int64_t m, int64_t n, int64_t k, int act);
 int plnlp_linear_act_backward(const void* gy, int64_t ldg, const int16_t* slope, int64_t lds, int act, const void* x, int64_t ldx,
                               const void* w, int64_t ldw, int64_t m, int64_t n, int64_t k, void* dx, int64_t lddx,

@@ -7,7 +7,8 @@
 //     bf16) would do to dz; and where a unit is saturated (-2^-5 < act' < 0: z below -2.6 for gelu, -4.8 for silu) ten bits of
 //     significand, a relative 2^-10 down to 2^-59, so that the gradients of a layer whose units all are keep their digits;
 //   dz, which the two gradient products read as 16-bit operands: an error of the size of the result's own rounding, averaged over
-//     the sums.  A small dz (see TWO_TERMS) is kept as the sum of two 16-bit terms instead, its few roundings would not average.
+//     the sums, and infinite past the type's range (fp16: |dy| above 57 900 where act' > 1).  A small dz (see TWO_TERMS) is kept as the
+//     sum of two 16-bit terms instead: its few roundings would not average.
 //
 // One tile kernel serves the three products, written as C[m, n] = sum_k P(m, k) Q(n, k):
 //   forward  P = x   (k contiguous)            Q = W (k contiguous)
@@ -815,12 +816,20 @@ __global__ __launch_bounds__(256) void act_back_kernel(const T* __restrict__ gy,
                     }
                     if (SLOPE) {
                         T* o = dz + (i + u * ty) * ldz + col;
-                        store_f32<T, V>(o, z);
                         if (plane) {
+                            // (past the type's range: its largest number and the rest; infinities and NaN have none)
+                            constexpr float MOST = std::is_same<T, _Float16>::value ? 65504.f : 3.38953139e38f;
+                            float rest[V];
 #pragma unroll
-                            for (int j = 0; j < V; ++j) z[j] -= (float)(T)z[j];
-                            store_f32<T, V>(o + plane, z);
+                            for (int j = 0; j < V; ++j) {
+                                const float all = z[j];
+                                const bool finite = fabsf(all) < __builtin_inff();
+                                if (finite) z[j] = fminf(fmaxf(all, -MOST), MOST);
+                                rest[j] = finite ? all - (float)(T)z[j] : 0.f;
+                            }
+                            store_f32<T, V>(o + plane, rest);
                         }
+                        store_f32<T, V>(o, z);
                     }
                 }
             };

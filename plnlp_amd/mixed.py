@@ -6,7 +6,8 @@ grad_clip.hip), next to the fp32 operators of plnlp_amd/ops.py:
   grad_norm          the norm of a list of gradients taken as one vector
   clip_grads         the gradients scaled so that this norm stays below a limit (in place, or into other tensors)
 
-All sums are held in 32 bits or more and every result is rounded once.  All are deterministic.  Work is enqueued on the current
+All sums are held in 32 bits or more and every result is rounded once; what linear_act's backward pass rounds on the way, its docstring
+says.  All are deterministic.  Work is enqueued on the current
 stream of the current device, on which every tensor has to be; nothing waits for it.  All may be captured into a graph.
 Like the rest of the package there is no CPU path."""
 from __future__ import annotations
@@ -183,7 +184,8 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tenso
     fp16.  activation: "none", "relu", "gelu" (z Phi(z)), "gelu_tanh" or "silu".  The product is summed in fp32; bias,
     activation and residual act on the fp32 sums, which are rounded once.  The activation's derivative is kept
     for the backward pass in 16 bits, where a gradient is wanted: in steps of 2^-14, and between -2^-5 and 0 (saturated units) to
-    2^-10 of itself.
+    2^-10 of itself.  The gradients of x and weight are products with dz = dy * derivative rounded to the operands' type, past whose
+    range it is infinite (up to 16 384 elements of dz: kept in two terms, to the square of one rounding); bias' sums dz unrounded.
     fp32 matrices are the business of ops.LinearFn."""
     dtype = x.dtype
     if dtype not in _HALF:

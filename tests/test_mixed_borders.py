@@ -147,3 +147,40 @@ def test_gradients_of_saturated_units(P, act, center, spread, dtype, gain, m, n,
         assert not bool(torch.isnan(over).any()) and float(over.max()) <= 0.0, (name, float(((got.double() - want).abs() / want.abs()).max()))
         if name != "dx":                                           # the bounds say something: within 2 % of what they bound
             assert float((bound / want.abs()).median()) <= 0.02, name
+
+
+# ------------------------------------------------------------------ the edge of a type ------
+@gpu
+@pytest.mark.parametrize("m,n,k", [(2, 8, 8), (20, 24, 64)])
+@pytest.mark.parametrize("dtype,most", [(F16, 60000.0), (BF16, 2.9e38)])
+def test_small_dz_at_the_edge_of_the_type(P, m, n, k, dtype, most):
+    """few elements of dz, kept as two terms: dy * act'(z) past the type's largest number (act' = 1.129 at z = 1.414, gelu) gives the
+    product's own finite values, an infinite dy gives infinities and a NaN stays in its row, in all three gradients"""
+    x = torch.zeros(m, k, dtype=dtype, device="cuda")
+    x[:, 0] = 1.0
+    w = torch.full((n, k), 2.0 ** -10, dtype=dtype, device="cuda")
+    w[:, 0] = 1.4140625
+    x.requires_grad_(True), w.requires_grad_(True)
+    b = torch.zeros(n, dtype=dtype, device="cuda", requires_grad=True)
+    gy = torch.zeros(m, n, dtype=dtype, device="cuda")
+    gy[0, 0] = most
+    slope = float(0.5 * (1 + math.erf(1.4140625 * math.sqrt(0.5))) + 1.4140625 * math.exp(-1.4140625 ** 2 / 2) / math.sqrt(2 * math.pi))
+    dz = float(gy[0, 0]) * slope
+    limit = torch.finfo(dtype).max
+    if dtype == F16:
+        assert dz > limit
+    dx, dw, db = torch.autograd.grad(P.linear_act(x, w, b, activation="gelu"), [x, w, b], gy)
+    # the slope is kept in steps of 2^-14 and computed to 2e-5, two terms hold dz to u^2, the result is rounded once
+    for got in dx[0, 1:].double():
+        assert abs(float(got) - dz * 2.0 ** -10) <= dz * 2.0 ** -10 * (2.0 ** -15 + 2e-5 + 2 * U[dtype])
+    assert not bool(dx[1:].any())
+    if dtype == F16:
+        assert float(dw[0, 0]) == math.inf and float(db[0]) == math.inf          # (these are dz itself: past the type)
+    assert not bool(torch.isnan(dx).any() or torch.isnan(dw[1:]).any() or torch.isnan(db).any())
+    gy[0, 0] = math.inf
+    dx, dw, db = torch.autograd.grad(P.linear_act(x, w, b, activation="gelu"), [x, w, b], gy)
+    assert bool((dx[0] == math.inf).all()) and not bool(dx[1:].any())
+    assert float(dw[0, 0]) == math.inf and not bool(dw[1:].any()) and float(db[0]) == math.inf and not bool(db[1:].any())
+    gy[0, 0] = math.nan
+    dx, dw, db = torch.autograd.grad(P.linear_act(x, w, b, activation="gelu"), [x, w, b], gy)
+    assert bool(torch.isnan(dx[0]).all()) and not bool(dx[1:].any()) and bool(torch.isnan(dw[0]).all()) and math.isnan(float(db[0]))
