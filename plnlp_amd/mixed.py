@@ -9,7 +9,8 @@ grad_clip.hip), next to the fp32 operators of plnlp_amd/ops.py:
 All sums are held in 32 bits or more and every result is rounded once; what linear_act's backward pass rounds on the way, its docstring
 says.  All are deterministic.  Work is enqueued on the current
 stream of the current device, on which every tensor has to be; nothing waits for it.  All may be captured into a graph.
-Like the rest of the package there is no CPU path."""
+Like the rest of the package there is no CPU path.  Gradients are those of reverse mode, of first order: second ones, and operands with
+a forward-mode tangent, are refused."""
 from __future__ import annotations
 
 import math
@@ -17,6 +18,7 @@ from typing import List, Optional, Sequence
 
 import numpy as np
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib as L
@@ -33,6 +35,16 @@ def _stream(*tensors: Optional[torch.Tensor]) -> int:
         if t is not None and t.get_device() != device:
             L.require_device(*tensors)
     return L.stream_ptr()
+
+
+def _no_tangent(what: str, *tensors: Optional[torch.Tensor]) -> None:
+    """refuses operands with a forward-mode tangent, which no operator here carries on (the kernels see addresses alone); outside a
+    dual level, where there are none, nothing is asked"""
+    if getattr(forward_ad, "_current_level", 0) < 0:
+        return
+    for t in tensors:
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+            raise NotImplementedError(f"{what}: there is no forward-mode derivative, and an operand carries a tangent")
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
@@ -121,6 +133,7 @@ def embedding_lookup(table: torch.Tensor, ids: torch.Tensor, *, scale: float = 1
         if not -table.shape[0] <= padding_idx < table.shape[0]:
             raise ValueError(f"embedding_lookup: padding_idx {padding_idx} is no row of a table of {table.shape[0]}")
         padding = padding_idx % table.shape[0]
+    _no_tangent("embedding_lookup", table)
     if torch.is_grad_enabled() and table.requires_grad:
         return EmbeddingLookupFn.apply(table, ids, float(scale), padding, out_dtype)
     return _lookup_rows(table, ids, float(scale), out_dtype)
@@ -214,6 +227,7 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tenso
         if residual.dtype != dtype:
             raise TypeError(f"linear_act: all operands must have x's type {dtype}; residual is {residual.dtype}")
         grad = grad or residual.requires_grad
+    _no_tangent("linear_act", x, weight, bias, residual)
     if len(shape) != 2:
         rows = math.prod(shape[:-1])
         x = x.reshape(rows, shape[-1])
@@ -297,9 +311,11 @@ def _overlap(src, dst, n, src_types, dst_types) -> bool:
 def grad_norm(grads: Sequence[torch.Tensor], *, norm_type: float = 2.0) -> torch.Tensor:
     """The norm (2, 1 or inf) of all elements of `grads` taken as one vector, as a 0-d fp32 tensor on the device.
     Any mix of bf16, fp16 and fp32, any shapes, empty tensors among them; NaN and infinities go through; the sums are fp64, so
-    neither large nor tiny elements leave the range.  Tensors that are not contiguous are read through a copy."""
+    neither large nor tiny elements leave the range.  Tensors that are not contiguous are read through a copy.  Autograd
+    does not follow: the norm has no graph."""
     kind = _norm_kind(norm_type)
     grads = list(grads)
+    _no_tangent("grad_norm", *grads)
     ptrs, sizes, types = _pointers(grads, "grad_norm: gradients")
     flat = _contiguous(grads)
     if flat is not grads:
@@ -345,11 +361,12 @@ def clip_grads(grads: Sequence[torch.Tensor], max_norm: float, *, norm_type: flo
     if not max_norm >= 0.0:
         raise ValueError(f"clip_grads: max_norm must be 0 or more, not {max_norm}")
     grads = list(grads)
+    to = grads if out is None else list(out)
+    _no_tangent("clip_grads", *grads, *to)
     src, sizes, types = _pointers(grads, "clip_grads: gradients")
     if out is None:
-        to, dst, to_types = grads, src, types
+        dst, to_types = src, types
     else:
-        to = list(out)
         dst, to_sizes, to_types = _pointers(to, "clip_grads: out")
         if to_sizes != sizes:
             raise ValueError("clip_grads: out must hold one tensor of as many elements for each gradient")

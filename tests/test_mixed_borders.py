@@ -184,3 +184,38 @@ def test_small_dz_at_the_edge_of_the_type(P, m, n, k, dtype, most):
     gy[0, 0] = math.nan
     dx, dw, db = torch.autograd.grad(P.linear_act(x, w, b, activation="gelu"), [x, w, b], gy)
     assert bool(torch.isnan(dx[0]).all()) and not bool(dx[1:].any()) and bool(torch.isnan(dw[0]).all()) and math.isnan(float(db[0]))
+
+
+# ------------------------------------------------------------------ refusals ------
+def test_a_forward_mode_tangent_is_refused():
+    """no operator has a forward-mode derivative: an operand that carries a tangent is refused, with a graph and without, before anything
+    else is looked at (no device needed)"""
+    import torch.autograd.forward_ad as fwd
+    import plnlp_amd as P
+    x, w, b, r = (torch.ones(s, dtype=BF16) for s in ((4, 8), (6, 8), (6,), (4, 6)))
+    table, ids = torch.ones(5, 8), torch.zeros(3, dtype=torch.int64)
+    with fwd.dual_level():
+        dual = [fwd.make_dual(t, torch.ones_like(t)) for t in (x, w, b, r)]
+        for i in range(4):
+            args = [d if j == i else t for j, (t, d) in enumerate(zip((x, w, b, r), dual))]
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                P.linear_act(*args[:3], residual=args[3], activation="gelu")
+            with pytest.raises(NotImplementedError, match="forward-mode"), torch.no_grad():
+                P.linear_act(*args[:3], residual=args[3], activation="gelu")
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            P.embedding_lookup(fwd.make_dual(table, torch.ones_like(table)), ids)
+        g = fwd.make_dual(table, torch.ones_like(table))
+        for call in (lambda: P.grad_norm([table, g]), lambda: P.clip_grads([g], 1.0), lambda: P.clip_grads([table], 1.0, out=[g])):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                call()
+        with pytest.raises(P._lib.PlnlpHipError):          # (operands without a tangent go on as ever: there is no CPU path)
+            P.linear_act(x, w, b, residual=r)
+
+
+@gpu
+def test_operands_without_a_tangent_inside_a_dual_level(P):
+    import torch.autograd.forward_ad as fwd
+    x, w = whole((4, 8), BF16, 1), whole((6, 8), BF16, 2)
+    want = P.linear_act(x, w)
+    with fwd.dual_level():
+        assert torch.equal(P.linear_act(x, w), want)
