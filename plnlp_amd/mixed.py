@@ -355,7 +355,8 @@ def clip_grads(grads: Sequence[torch.Tensor], max_norm: float, *, norm_type: flo
     out: where the scaled gradients go -- one tensor of as many elements for each, of any of the three types: 16-bit gradients
     into the fp32 ones an optimiser of fp32 parameters reads; None: in place.  As torch.nn.utils.clip_grad_norm_ has it, a NaN
     norm makes every gradient NaN and an infinite one makes the finite elements zero.  A tensor listed twice, or one whose
-    memory another one's result would overwrite, is refused.  Tensors that are not contiguous are handled through copies."""
+    memory another one's result would overwrite, is refused, and so is a written tensor that is expanded.  Tensors that are not contiguous
+    are handled through copies: what such views share with other tensors of the call is scaled once, from its old value."""
     kind = _norm_kind(norm_type)
     max_norm = float(max_norm)
     if not max_norm >= 0.0:
@@ -378,6 +379,8 @@ def clip_grads(grads: Sequence[torch.Tensor], max_norm: float, *, norm_type: flo
         dst = src if out is None else list(map(torch.Tensor.data_ptr, flat_to))
     if flat_to is not to and len({t.data_ptr() for t in to if t.numel()}) < sum(t.numel() > 0 for t in to):
         raise ValueError(_OVERLAP)                   # (the copies of such tensors do not overlap)
+    if flat_to is not to and any(s == 0 and n > 1 for t, c in zip(to, flat_to) if c is not t for s, n in zip(t.stride(), t.shape)):
+        raise ValueError("clip_grads: the elements of an expanded tensor share memory and cannot be written")
     norm = _run_clip(src, dst, sizes, _codes(types, L.DTYPE_CODES), _codes(to_types, _DST_CODES), kind, max_norm)
     torch.autograd.graph.increment_version([t for t in to if not t.is_inference()])      # (written behind autograd's back)
     if flat_to is not to:

@@ -219,3 +219,25 @@ def test_operands_without_a_tangent_inside_a_dual_level(P):
     want = P.linear_act(x, w)
     with fwd.dual_level():
         assert torch.equal(P.linear_act(x, w), want)
+
+
+@gpu
+def test_clip_refuses_an_expanded_tensor_before_it_writes(P):
+    """a tensor whose elements share memory cannot be written: the call is refused as a whole, the other tensors stay as they were"""
+    a, one = torch.ones(40, device="cuda"), torch.ones(1, 3, dtype=BF16, device="cuda")
+    for grads, out in (([a, one.expand(5, 3)], None), ([a, a.clone()], [a.clone(), torch.zeros(1, device="cuda").expand(40)]),
+                       ([one.expand(5, 3)], None)):
+        keep = [g.clone() for g in grads + (out or [])]
+        with pytest.raises(ValueError, match="share memory"):
+            P.clip_grads(grads, 0.5, out=out)
+        assert all(torch.equal(g, k) for g, k in zip(grads + (out or []), keep))
+    out = [torch.zeros(5, 3, device="cuda")]                       # (read, it counts as the elements it shows)
+    assert float(P.clip_grads([one.expand(5, 3)], 1.0, out=out)) == pytest.approx(math.sqrt(15), rel=1e-6)
+    assert float(out[0].norm()) == pytest.approx(1.0, rel=1e-5)
+    P.clip_grads([torch.ones(0, 3, device="cuda").expand(0, 3), torch.ones(1, 1, device="cuda").expand(1, 1)], 1.0)      # nothing shared
+    a = torch.arange(240, device="cuda").float().view(30, 8)
+    want = a.clone()
+    n = P.clip_grads([a.t(), a[3:5]], 1.0)                         # a strided view and a part of its memory: scaled once, from the old values
+    ref = math.sqrt(float(want.double().square().sum() + want[3:5].double().square().sum()))
+    assert float(n) == pytest.approx(ref, rel=1e-6)
+    assert float((a.double() - want.double() / (ref + 1e-6)).abs().max()) <= 4 * U[F32]          # (elements below 1; factor and product in f32)
