@@ -100,7 +100,10 @@ def group_sqnorm(params: Sequence[torch.nn.Parameter]) -> Optional[torch.Tensor]
 
 def clip_grad_norm_(parameters, max_norm: float, norm_type: float = 2.0) -> torch.Tensor:
     """torch.nn.utils.clip_grad_norm_ for bf16, fp16 and fp32 gradients in any mix: two launches per 128 tensors and no host
-    synchronisation (plnlp_amd.clip_grads); parameters without a gradient are skipped"""
+    synchronisation (plnlp_amd.clip_grads); parameters without a gradient are skipped.  Narrower than torch's: norm_type is 1, 2 or
+    inf; a parameter listed twice, sparse gradients and gradients of the CPU or of a device that is not the current one are refused; and
+    error_if_nonfinite does not exist, since it would wait for the device (a norm that is not finite does to the gradients what clip_grads
+    says)"""
     if isinstance(parameters, torch.Tensor):
         parameters = [parameters]
     grads = [p.grad for p in parameters if p.grad is not None]
