@@ -241,3 +241,24 @@ def test_clip_refuses_an_expanded_tensor_before_it_writes(P):
     ref = math.sqrt(float(want.double().square().sum() + want[3:5].double().square().sum()))
     assert float(n) == pytest.approx(ref, rel=1e-6)
     assert float((a.double() - want.double() / (ref + 1e-6)).abs().max()) <= 4 * U[F32]          # (elements below 1; factor and product in f32)
+
+
+# ------------------------------------------------------------------ the lookup's gradient over many ids ------
+# 2^20 ids and more (the sort's larger tiles), tables whose keys take one, two and three passes; a third of the batch is one id, whose run
+# crosses many ranges, some ids lie outside.  dy is small whole numbers: every sum is exact and rounded once.
+@gpu
+@pytest.mark.parametrize("n", [2 ** 20, 2 ** 20 + 1, 3000017])
+@pytest.mark.parametrize("rows", [1500, 300007, 4300001])
+@pytest.mark.parametrize("width,id_t", [(8, torch.int64), (5, torch.int32), (40, torch.int64)])
+@pytest.mark.parametrize("frequent", [False, True])
+def test_lookup_gradient_of_many_ids(P, n, rows, width, id_t, frequent):
+    ids = torch.randint(-3, rows + 3, (n,), generator=generator(n + rows), device="cuda")
+    if frequent:
+        ids[torch.rand(n, generator=generator(7), device="cuda") < 1 / 3] = rows // 2
+    gy = whole((n, width), BF16, 5, -3, 3)
+    table = torch.zeros(rows, width, device="cuda", requires_grad=True)
+    got, = torch.autograd.grad(P.embedding_lookup(table, ids.to(id_t), padding_idx=rows - 1, out_dtype=BF16), [table], gy)
+    ok = (ids >= 0) & (ids < rows - 1)
+    want = torch.zeros(rows, width, dtype=torch.int64, device="cuda").index_add_(0, ids[ok], gy.long()[ok])
+    assert int(want.abs().max()) < 2 ** 24
+    assert torch.equal(got.long(), want)
