@@ -16,7 +16,7 @@ def needs_build() -> bool:
         return True
     t = os.path.getmtime(LIB)
     deps = [os.path.join(CSRC, f) for f in os.listdir(CSRC)]
-    deps.append(os.path.join(os.path.dirname(HERE), "include", "plnlp_hip.h"))
+    deps += [os.path.join(os.path.dirname(HERE), "include", "plnlp_hip.h"), os.path.abspath(__file__)]
     return any(os.path.getmtime(d) > t for d in deps)
 
 
@@ -45,11 +45,12 @@ def build(force: bool = False, verbose: bool = False) -> str:
     no_packed = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
     headers = [os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith(".h")]
     headers.append(os.path.join(os.path.dirname(HERE), "include", "plnlp_hip.h"))
+    headers.append(os.path.abspath(__file__))                # (the flags stand here)
     newest_header = max(os.path.getmtime(h) for h in headers)
     for src, oname, extra in units:
         obj = os.path.join(HERE, "build", oname)
         objs.append(obj)
-        # a unit is recompiled when its source or any header is newer than its object (the objects carry the time their
+        # a unit is recompiled when its source, any header or this file is newer than its object (the objects carry the time their
         # sources were read, like the library)
         if (not force and os.path.exists(obj)
                 and os.path.getmtime(obj) >= max(os.path.getmtime(os.path.join(CSRC, src)), newest_header)):
