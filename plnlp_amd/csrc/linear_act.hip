@@ -924,9 +924,9 @@ static int launch_tile(const TileArgs<T>& a, hipStream_t s) {
 
 // Q in LDS for the rows kernel: 32-k pieces a row (0: it does not take the product).  Every workgroup reads all of Q once, so there
 // have to be rows enough for each: 128 a column of the result (256 workgroups times n k of Q against m k of P, twice).
-//   us, forward with gelu, slope and residual, here / on the tile kernel: 131 072 x 256 x 256 67 / 70 (70 alone on a cold chip: 3.8 TB/s;
-//   91 before either kernel asked for the residual ahead), 32 768 x 256 x 256 19.4 / 20.8 but 16 384 x 256 x 256 17.8 / 15.0;
-//   262 144 x 64 x 256 40 / 64, 16 384 x 64 x 64 6.8 / 10.0, 8192 x 64 x 64 6.3 / 9.7; backward 131 072 x 256 x 256 121 / 127
+//   us, with gelu, slope and residual, here / on the tile kernel, forward: 131 072 x 256 x 256 74 / 77 (3.6 TB/s), 32 768 x 256 x 256 20.5 /
+//   20.5 but 16 384 x 256 x 256 18.2 / 15.1; 262 144 x 64 x 256 42 / 66, 16 384 x 64 x 64 6.8 / 10.8, 8192 x 64 x 64 6.7 / 10.6;
+//   backward: 124 / 130, 50.5 / 49.4, 43.6 / 37.7, 110 / 121, 20 / 26, 19 / 24
 constexpr int64_t ROWS_MIN = 8192, ROWS_PER_COLUMN = 128, ROWS_LDS = 155648;
 static int rows_fit(int64_t m, int64_t n, int64_t k, int64_t most_k = 512) {
     if (m < ROWS_MIN || m < ROWS_PER_COLUMN * n || n == 0 || k == 0 || k > most_k) return 0;

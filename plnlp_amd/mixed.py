@@ -7,9 +7,9 @@ grad_clip.hip), next to the fp32 operators of plnlp_amd/ops.py:
   clip_grads         the gradients scaled so that this norm stays below a limit (in place, or into other tensors)
 
 All sums are held in 32 bits or more and every result is rounded once; what linear_act's backward pass rounds on the way, its docstring
-says.  All are deterministic.  Work is enqueued on the current
-stream of the current device, on which every tensor has to be; nothing waits for it.  All may be captured into a graph.
-Like the rest of the package there is no CPU path.  Gradients are those of reverse mode, of first order: second ones, and operands with
+says.  All are deterministic.  Work is enqueued on the current stream of the current device, on which every tensor has to be; nothing
+waits for it.  All may be captured into a graph (a backward pass, as any of torch's, only while no graph of the same leaves is alive
+that was recorded before the capture).  Like the rest of the package there is no CPU path.  Gradients are those of reverse mode, of first order: second ones, and operands with
 a forward-mode tangent, are refused."""
 from __future__ import annotations
 
